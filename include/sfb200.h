@@ -232,6 +232,160 @@ int sfb_w8a16_mlp_noalloc(const void* x, int64_t ldx, const int8_t* w1, const fl
                           void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t K, int32_t F, int32_t N,
                           int32_t act, void* stream);
 
+/* ── query/key norms with the position rotation, one pass ─────────────────────
+ * Per head of head_dim channels of q and of k (the reference's qk-norm,
+ * src/models/rdt1b/dit_block.cu:185-196, with a rotary position embedding):
+ *   y = x / sqrt(mean(x²) + eps) · weight      (norm != 0; a NULL weight is 1)
+ *   (a, b) → (a·cos − b·sin, b·cos + a·sin)    over the first rotary_dim channels
+ * in fp32, rounded once.
+ * - Pairs: channels (i, i + rotary_dim/2), or (2i, 2i+1) with interleaved != 0.
+ *   rotary_dim 0: no rotation; else a multiple of 16, at most head_dim.
+ * - cos_table / sin_table: fp32 [table_len, rotary_dim/2], contiguous, the
+ *   angles of each position (made once, in whatever precision the caller
+ *   wants). positions: int32 [batch, seq] with row stride pos_stride_b
+ *   (elements), or NULL for 0..seq-1. A token whose position is outside
+ *   [0, table_len) is not written; the kernel then records SFB_ERR_RANGE in the
+ *   device error word (sfb_device_error).
+ * - q and k may be NULL (with their outputs) to process only the other; the
+ *   outputs may be the inputs (same pointer and strides).
+ * - dtype of q, k, the outputs and the weights: SFB_BF16, SFB_F16 or SFB_F32.
+ *   head_dim: a multiple of 8, at most 256, contiguous; the other dimensions
+ *   by element strides (batch, head, seq). Pointers 16-byte aligned, strides
+ *   multiples of 16 bytes. */
+typedef struct sfb_norm_rope_args {
+    const void* q;
+    const void* k;
+    void*       q_out;
+    void*       k_out;
+    int64_t q_stride[3];
+    int64_t k_stride[3];
+    int64_t q_out_stride[3];
+    int64_t k_out_stride[3];
+    const void*  q_weight;
+    const void*  k_weight;
+    const float* cos_table;
+    const float* sin_table;
+    const int32_t* positions;
+    int64_t pos_stride_b;
+    int32_t table_len;
+    int32_t batch;
+    int32_t seq;
+    int32_t heads;
+    int32_t heads_kv;
+    int32_t head_dim;
+    int32_t rotary_dim;
+    int32_t interleaved;
+    int32_t norm;
+    int32_t dtype;
+    float   eps;
+} sfb_norm_rope_args;
+
+int sfb_qk_norm_rope(const sfb_norm_rope_args* args, void* stream);
+
+/* ── K/V cache held in 4 bits ─────────────────────────────────────────────────
+ * No counterpart in the reference (its cross-attention recomputes K/V every
+ * call, dit_block.cu:288-304). Every token and head holds its head_dim values
+ * as 4-bit codes c in [-8, 7] with one fp16 scale s per 32 channels; the value
+ * is c·s.
+ * - Codes: 8 consecutive channels make one little-endian 32-bit word; channel
+ *   2i of the eight sits in bits [4i, 4i+4), channel 2i+1 in bits
+ *   [16+4i, 16+4i+4); the stored nibble is c + 8.
+ * - sfb_kv4_append makes s = fp16(bf16(max|x| / 7)) and c = clamp(round-half-
+ *   even(x / s), -7, 7), 0 where s is 0. s has 8 significant bits, so c·s is
+ *   exact in fp16, and the attention works on exactly the values held. Groups
+ *   that hold a NaN or an infinity, or whose scale exceeds 9344 (|x| > 65408),
+ *   get a NaN scale: the group reads back as NaN.
+ * A scale written by another program must have at most 8 significant bits and
+ * a magnitude of at most 8128 for the same exactness.
+ * Layout: codes [batch, heads_kv, capacity, head_dim/2] bytes and scales
+ * [batch, heads_kv, capacity, head_dim/32] fp16, the last two dimensions
+ * contiguous; K and V share the strides. head_dim 64 or 128. Code pointers and
+ * strides are multiples of 16 bytes, scale pointers and strides too. */
+typedef struct sfb_kv4_cache {
+    void* k_codes;
+    void* v_codes;
+    void* k_scale;
+    void* v_scale;
+    int64_t code_stride[2];     /* bytes: batch, head */
+    int64_t scale_stride[2];    /* elements: batch, head */
+    int32_t batch;
+    int32_t heads_kv;
+    int32_t capacity;
+    int32_t head_dim;
+} sfb_kv4_cache;
+
+/* Quantises seq new tokens of every session into the cache. k, v: dtype
+ * SFB_BF16, SFB_F16 or SFB_F32, [batch, heads_kv, seq, head_dim] by element
+ * strides (batch, head, seq), 16-byte aligned, strides multiples of 16 bytes.
+ * Token i of session b goes to slot start[b] + i (start: int32 [batch], device;
+ * NULL: slot0 + i). len (optional, int32 [batch], device): only the first
+ * len[b] tokens of session b are written. A slot outside [0, capacity) is not
+ * written; the kernel then records SFB_ERR_RANGE in the device error word. */
+int sfb_kv4_append(const sfb_kv4_cache* cache, const void* k, const int64_t* k_stride, const void* v,
+                   const int64_t* v_stride, int32_t dtype, int32_t seq, const int32_t* start, int32_t slot0,
+                   const int32_t* len, void* stream);
+/* The values of slots [slot0, slot0 + seq) of every session, [batch, heads_kv,
+ * seq, head_dim] by element strides (batch, head, seq): the 16-bit form that
+ * sfb_attention_fwd takes. dtype SFB_F16 (exact), SFB_BF16 (rounded) or
+ * SFB_F32 (exact). Either output may be NULL. */
+int sfb_kv4_read(const sfb_kv4_cache* cache, void* k, const int64_t* k_stride, void* v,
+                 const int64_t* v_stride, int32_t dtype, int32_t slot0, int32_t seq, void* stream);
+
+/* Attention over the 4-bit cache: sfb_attention_fwd's sum with K and V read as
+ * they are held,
+ *   out[b,h,i,:] = softmax_j( scale · q[b,h,i,:]·k[b,hk,j,:] ) · v[b,hk,j,:],
+ * over the slots j < seq_k of the cache.
+ * - q, out: dtype SFB_BF16 or SFB_F16 by element strides (batch, head, seq),
+ *   16-byte aligned, strides multiples of 16 bytes. Queries enter the products
+ *   as fp16: bf16 queries beyond 65504 are not supported (the kernel then
+ *   records SFB_ERR_RANGE in the device error word).
+ * - kv_len (optional, int32 [batch], device): slots j >= kv_len[b] are masked.
+ * - key_mask (optional, uint8 [batch, seq_k], device): as in sfb_attn_args.
+ * - is_causal: the queries are the last seq_q tokens of the session, query i
+ *   sees slot j iff j <= n - seq_q + i with n = min(kv_len[b], seq_k) (n =
+ *   seq_k without kv_len). Queries before the first slot see none.
+ * - A query that sees no slot produces zeros. Masked slots may hold anything.
+ * - heads % heads_kv == 0; scale 0 means 1/sqrt(head_dim).
+ * - num_splits: key splits merged inside one thread-block cluster (0 = choose,
+ *   else 1..16). Allocates nothing, keeps no workspace. */
+typedef struct sfb_kv4_attn_args {
+    const sfb_kv4_cache* cache;
+    const void* q;
+    void*       out;
+    int64_t q_stride[3];
+    int64_t out_stride[3];
+    const int32_t* kv_len;
+    const uint8_t* key_mask;
+    int64_t key_mask_stride_b;
+    int32_t heads;
+    int32_t seq_q;
+    int32_t seq_k;
+    int32_t dtype;
+    int32_t is_causal;
+    int32_t num_splits;
+    float   scale;
+} sfb_kv4_attn_args;
+
+int sfb_kv4_attention(const sfb_kv4_attn_args* args, void* stream);
+
+/* ── 4-bit-weight linear layer ────────────────────────────────────────────────
+ * sfb_w8a16_linear's layer with 4-bit weights and a scale per `group`
+ * consecutive inputs of each output channel:
+ *   y[m,n] = act( Σ_g w_scale[n,g] · Σ_{k in g} x[m,k]·c[n,k] + bias[n] ) + residual[m,n]
+ * x: x_dtype (SFB_BF16 or SFB_F16) [M, K], row stride ldx (a multiple of 8
+ * elements, 16-byte aligned); w: [N, K/2] bytes, contiguous, 16-byte aligned,
+ * codes c in [-8, 7] packed as in sfb_kv4_cache; w_scale: [N, K/group]
+ * contiguous in scale_dtype (SFB_F16, SFB_BF16 or SFB_F32); group: 32, 64 or
+ * 128; K % group == 0. bias: x_dtype [N] or NULL; residual: [M, N] in y_dtype
+ * with row stride ldr, or NULL (may alias y); y: y_dtype (x_dtype or SFB_F32)
+ * [M, N], row stride ldy. act as sfb_w8a16_linear. Any M and N. Codes enter the
+ * products exactly; sums and scales are fp32. Meant for few rows (it is bound
+ * by the weights up to about 64). */
+int sfb_w4a16_linear(const void* x, int64_t ldx, int32_t x_dtype, const void* w, const void* w_scale,
+                     int32_t scale_dtype, int32_t group, const void* bias, const void* residual, int64_t ldr,
+                     void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t N, int32_t K, int32_t act,
+                     void* stream);
+
 /* ── RDT-1B denoising runtime ──────────────────────────────────────────────────
  * The model-level path around the kernels above, replacing for RDT-1B the
  * reference's RDT1BModel::encode_condition / denoise_step

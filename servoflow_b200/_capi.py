@@ -61,6 +61,39 @@ class AttnArgs(ctypes.Structure):
     ]
 
 
+def _scalars(ctype, *names):
+    return [(n, ctype) for n in names]
+
+
+class Kv4Cache(ctypes.Structure):
+    """Mirror of ``sfb_kv4_cache`` (include/sfb200.h), its arrays as single fields."""
+
+    _fields_ = _scalars(ctypes.c_void_p, "k_codes", "v_codes", "k_scale", "v_scale") + _scalars(
+        ctypes.c_int64, "code_stride0", "code_stride1", "scale_stride0", "scale_stride1") + _scalars(
+        ctypes.c_int32, "batch", "heads_kv", "capacity", "head_dim")
+
+
+class Kv4AttnArgs(ctypes.Structure):
+    """Mirror of ``sfb_kv4_attn_args`` (include/sfb200.h)."""
+
+    _fields_ = _scalars(ctypes.c_void_p, "cache", "q", "out") + _scalars(
+        ctypes.c_int64 * 3, "q_stride", "out_stride") + _scalars(ctypes.c_void_p, "kv_len", "key_mask") + _scalars(
+        ctypes.c_int64, "key_mask_stride_b") + _scalars(
+        ctypes.c_int32, "heads", "seq_q", "seq_k", "dtype", "is_causal", "num_splits") + _scalars(
+        ctypes.c_float, "scale")
+
+
+class NormRopeArgs(ctypes.Structure):
+    """Mirror of ``sfb_norm_rope_args`` (include/sfb200.h)."""
+
+    _fields_ = _scalars(ctypes.c_void_p, "q", "k", "q_out", "k_out") + _scalars(
+        ctypes.c_int64 * 3, "q_stride", "k_stride", "q_out_stride", "k_out_stride") + _scalars(
+        ctypes.c_void_p, "q_weight", "k_weight", "cos_table", "sin_table", "positions") + _scalars(
+        ctypes.c_int64, "pos_stride_b") + _scalars(
+        ctypes.c_int32, "table_len", "batch", "seq", "heads", "heads_kv", "head_dim", "rotary_dim",
+        "interleaved", "norm", "dtype") + _scalars(ctypes.c_float, "eps")
+
+
 class SfbError(RuntimeError):
     """A non-zero status returned through the C ABI."""
 
@@ -105,6 +138,21 @@ def _declare(lib: ctypes.CDLL) -> None:
                                   c.c_void_p, c.c_void_p, c.c_void_p, c.c_void_p, c.c_int64,
                                   c.c_void_p, c.c_int64, c.c_int32, c.c_int32, c.c_int32, c.c_int32,
                                   c.c_int32, c.c_int32, c.c_void_p, c.c_size_t, c.c_void_p]
+    lib.sfb_qk_norm_rope.restype = c.c_int
+    lib.sfb_qk_norm_rope.argtypes = [c.POINTER(NormRopeArgs), c.c_void_p]
+    i64x3 = c.POINTER(c.c_int64 * 3)
+    lib.sfb_kv4_append.restype = c.c_int
+    lib.sfb_kv4_append.argtypes = [c.POINTER(Kv4Cache), c.c_void_p, i64x3, c.c_void_p, i64x3, c.c_int32,
+                                   c.c_int32, c.c_void_p, c.c_int32, c.c_void_p, c.c_void_p]
+    lib.sfb_kv4_read.restype = c.c_int
+    lib.sfb_kv4_read.argtypes = [c.POINTER(Kv4Cache), c.c_void_p, i64x3, c.c_void_p, i64x3, c.c_int32,
+                                 c.c_int32, c.c_int32, c.c_void_p]
+    lib.sfb_kv4_attention.restype = c.c_int
+    lib.sfb_kv4_attention.argtypes = [c.POINTER(Kv4AttnArgs), c.c_void_p]
+    lib.sfb_w4a16_linear.restype = c.c_int
+    lib.sfb_w4a16_linear.argtypes = [c.c_void_p, c.c_int64, c.c_int32, c.c_void_p, c.c_void_p, c.c_int32,
+                                     c.c_int32, c.c_void_p, c.c_void_p, c.c_int64, c.c_void_p, c.c_int64,
+                                     c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_void_p]
     lib.sfb_dequantize_int8.restype = c.c_int
     lib.sfb_dequantize_int8.argtypes = [c.c_void_p, c.c_void_p, c.c_int32, c.c_int64, c.c_void_p,
                                         c.c_int32, c.c_int64, c.c_int64, c.c_void_p]

@@ -18,6 +18,17 @@ int w8a16_mlp_launch(const void* x, int64_t ldx, const int8_t* w1, const float* 
 int dequantize_int8_launch(const int8_t* in, const void* scale, int32_t scale_dtype,
                            int64_t scale_numel, void* out, int32_t out_dtype, int64_t rows,
                            int64_t cols, cudaStream_t stream);
+int qk_norm_rope_launch(const sfb_norm_rope_args& a, cudaStream_t s);
+int kv4_append_launch(const sfb_kv4_cache* cache, const void* k, const int64_t* k_st, const void* v,
+                      const int64_t* v_st, int32_t dtype, int32_t seq, const int32_t* start, int32_t slot0,
+                      const int32_t* len, cudaStream_t s);
+int kv4_read_launch(const sfb_kv4_cache* cache, void* k, const int64_t* k_st, void* v, const int64_t* v_st,
+                    int32_t dtype, int32_t slot0, int32_t seq, cudaStream_t s);
+int kv4_attention_launch(const sfb_kv4_attn_args& a, cudaStream_t s);
+int w4a16_linear_launch(const void* x, int64_t ldx, int32_t x_dtype, const void* w, const void* w_scale,
+                        int32_t scale_dtype, int32_t group, const void* bias, const void* residual, int64_t ldr,
+                        void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t N, int32_t K, int32_t act,
+                        cudaStream_t stream);
 }  // namespace sfb
 
 extern "C" {
@@ -154,6 +165,36 @@ int sfb_w8a16_mlp(const void* x, int64_t ldx, const int8_t* w1, const float* s1,
                   int32_t act, void* workspace, size_t workspace_bytes, void* stream) {
     return sfb::w8a16_mlp_launch(x, ldx, w1, s1, b1, w2, s2, b2, residual, ldr, y, ldy, y_dtype, M, K, F, N,
                                  act, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int sfb_qk_norm_rope(const sfb_norm_rope_args* a, void* stream) {
+    if (a == nullptr) return SFB_ERR_INVALID;
+    return sfb::qk_norm_rope_launch(*a, static_cast<cudaStream_t>(stream));
+}
+
+int sfb_kv4_append(const sfb_kv4_cache* cache, const void* k, const int64_t* k_stride, const void* v,
+                   const int64_t* v_stride, int32_t dtype, int32_t seq, const int32_t* start, int32_t slot0,
+                   const int32_t* len, void* stream) {
+    return sfb::kv4_append_launch(cache, k, k_stride, v, v_stride, dtype, seq, start, slot0, len,
+                                  static_cast<cudaStream_t>(stream));
+}
+
+int sfb_kv4_read(const sfb_kv4_cache* cache, void* k, const int64_t* k_stride, void* v, const int64_t* v_stride,
+                 int32_t dtype, int32_t slot0, int32_t seq, void* stream) {
+    return sfb::kv4_read_launch(cache, k, k_stride, v, v_stride, dtype, slot0, seq, static_cast<cudaStream_t>(stream));
+}
+
+int sfb_kv4_attention(const sfb_kv4_attn_args* a, void* stream) {
+    if (a == nullptr) return SFB_ERR_INVALID;
+    return sfb::kv4_attention_launch(*a, static_cast<cudaStream_t>(stream));
+}
+
+int sfb_w4a16_linear(const void* x, int64_t ldx, int32_t x_dtype, const void* w, const void* w_scale,
+                     int32_t scale_dtype, int32_t group, const void* bias, const void* residual, int64_t ldr,
+                     void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t N, int32_t K, int32_t act,
+                     void* stream) {
+    return sfb::w4a16_linear_launch(x, ldx, x_dtype, w, w_scale, scale_dtype, group, bias, residual, ldr, y, ldy,
+                                    y_dtype, M, N, K, act, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

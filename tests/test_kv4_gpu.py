@@ -1,0 +1,401 @@
+"""GPU tests of the 4-bit K/V cache (append, read back) and of the attention
+over it, against plain implementations in 64 bits.
+
+Append and read are exact: same scales and codes, same values.
+
+Attention tolerance, per output element: half a step of the output type on the
+value, plus what the kernel's fp16 probabilities and fp32 sums may add:
+  Σ p|v| · (2^-11 + 2^-15)   the probabilities rounded to fp16 (half a step is
+                             2^-11), and 2^-15 for everything in fp32: logits
+                             of at most 2^6 with a relative error of about
+                             70 · 2^-24 (D products, scaling), the base-2
+                             exponential (2^-22), up to 16384 fp32 additions
+  n · 2^-25 · max|v|         probabilities below fp16's normal range: each is
+                             off by at most 2^-25 while the row's sum is >= 1
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from servoflow_b200 import _capi
+from servoflow_b200.backend import B200Backend
+from servoflow_b200.quant4 import KV4Cache, unpack_codes
+
+pytestmark = pytest.mark.gpu
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+@pytest.fixture(scope="module")
+def be(gpu):
+    b = B200Backend(0)
+    b.device_error(reset=True)
+    yield b
+    assert b.device_error(reset=True) == 0
+
+
+def quantize64(x):
+    """(codes, scales) of float values [..., D] by the format's definition, on the CPU."""
+    g = x.float().numpy().reshape(*x.shape[:-1], -1, 32)
+    amax = np.abs(g).max(-1)
+    s = torch.from_numpy((amax / np.float32(7)).astype(np.float32)).bfloat16().half()
+    f = s.float().numpy()[..., None]
+    with np.errstate(divide="ignore", invalid="ignore"):
+        c = np.where(f > 0, np.clip(np.rint(g / f), -7, 7), 0.0)
+    return torch.from_numpy(c.reshape(x.shape).astype(np.int8)), s
+
+
+def fill(cache, seed, spread=1.0):
+    """Random values in every slot, appended by the kernel's own format (built on the CPU)."""
+    from servoflow_b200.quant4 import pack_codes
+    B, H, C, D = cache.shape
+    g = torch.Generator().manual_seed(seed)
+    for codes, scale in ((cache.k_codes, cache.k_scale), (cache.v_codes, cache.v_scale)):
+        c, s = quantize64(torch.randn(B, H, C, D, generator=g) * spread)
+        codes.copy_(pack_codes(c.to(torch.int32)))
+        scale.copy_(s)
+
+
+# ── append and read ──────────────────────────────────────────────────────────
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,H,S,D,cap,start,layout", [
+    (1, 1, 1, 64, 32, [0], "bhsd"), (2, 3, 5, 64, 64, [0, 59], "bshd"), (3, 2, 33, 128, 96, [1, 63, 30], "bshd"),
+    (1, 4, 67, 64, 67, [0], "bhsd"), (4, 1, 2, 128, 32, [3, 30, 0, 17], "bhsd")])
+def test_append_is_exact(be, gpu, dt, B, H, S, D, cap, start, layout):
+    cache = KV4Cache.allocate(B, H, cap, D)
+    fill(cache, 5)
+    before = [t.clone() for t in (cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale)]
+    g = torch.Generator().manual_seed(S * D + H)
+    kv = [torch.randn(B, H, S, D, generator=g) * (3.0 if i else 0.4) for i in range(2)]
+    kv[0][0, 0, 0, :32] = 0.0                                  # a group of zeros
+    kv[1][-1, -1, -1, 32:64] *= 1e-5                           # a tiny one (below fp16's normal scales in fp32)
+    kv = [x.to(dt) for x in kv]
+    dev = [x.to(gpu) if layout == "bhsd" else x.transpose(1, 2).contiguous().to(gpu) for x in kv]
+    be.kv4_append(cache, *dev, start=torch.tensor(start, dtype=torch.int32, device=gpu), layout=layout)
+    for x, codes, scale, c0, s0 in ((kv[0], cache.k_codes, cache.k_scale, before[0], before[2]),
+                                    (kv[1], cache.v_codes, cache.v_scale, before[1], before[3])):
+        c, s = quantize64(x)
+        for b, at in enumerate(start):
+            c0[b, :, at:at + S] = 0
+            assert torch.equal(unpack_codes(codes[b, :, at:at + S]).cpu(), c[b])
+            assert torch.equal(scale[b, :, at:at + S].cpu(), s[b])
+            # every other slot is as it was
+            mask = torch.ones(codes.shape[2], dtype=torch.bool)
+            mask[at:at + S] = False
+            assert torch.equal(codes[b][:, mask], c0[b][:, mask]) and torch.equal(scale[b][:, mask], s0[b][:, mask])
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,slot0,n,layout", [(64, 0, 64, "bhsd"), (128, 7, 23, "bshd"), (64, 63, 1, "bhsd")])
+def test_read_returns_the_values_held(be, gpu, dt, D, slot0, n, layout):
+    cache = KV4Cache.allocate(2, 3, 64, D)
+    fill(cache, 9)
+    shape = (2, 3, n, D) if layout == "bhsd" else (2, n, 3, D)
+    out = [torch.empty(shape, dtype=dt, device=gpu) for _ in range(2)]
+    be.kv4_read(cache, *out, slot0=slot0, layout=layout)
+    for o, want in zip(out, cache.dequantize()):
+        want = want[:, :, slot0:slot0 + n]
+        assert torch.equal(o if layout == "bhsd" else o.transpose(1, 2), want.to(dt))
+        if dt == torch.float16:                                # c·s is exact in fp16
+            assert torch.equal(want.half().float(), want)
+    one = torch.empty(shape, dtype=dt, device=gpu)
+    be.kv4_read(cache, None, one, slot0=slot0, layout=layout)  # V alone
+    assert torch.equal(one, out[1])
+
+
+def test_append_lens_and_scalar_start(be, gpu):
+    cache = KV4Cache.allocate(3, 2, 32, 64)
+    fill(cache, 3)
+    k0 = cache.k_codes.clone()
+    x = torch.randn(3, 2, 8, 64, generator=torch.Generator().manual_seed(1)).bfloat16()
+    be.kv4_append(cache, x.to(gpu), x.to(gpu), start=20, lens=torch.tensor([0, 8, 3], dtype=torch.int32, device=gpu))
+    c, _ = quantize64(x)
+    assert torch.equal(cache.k_codes[0], k0[0])                                    # length 0: untouched
+    assert torch.equal(unpack_codes(cache.k_codes[1, :, 20:28]).cpu(), c[1])
+    assert torch.equal(unpack_codes(cache.k_codes[2, :, 20:23]).cpu(), c[2, :, :3])
+    assert torch.equal(cache.k_codes[2, :, 23:], k0[2, :, 23:])                    # rows behind the length
+
+
+def test_append_outside_the_cache_is_refused_on_the_device(be, gpu):
+    cache = KV4Cache.allocate(2, 1, 32, 64)
+    fill(cache, 4)
+    k0 = cache.k_codes.clone()
+    x = torch.randn(2, 1, 4, 64, generator=torch.Generator().manual_seed(2)).half()
+    assert be.device_error(reset=True) == 0
+    be.kv4_append(cache, x.to(gpu), x.to(gpu), start=torch.tensor([30, -2], dtype=torch.int32, device=gpu))
+    torch.cuda.synchronize()
+    assert be.device_error(reset=True) == _capi.SFB_ERR_RANGE
+    c, _ = quantize64(x)
+    assert torch.equal(unpack_codes(cache.k_codes[0, :, 30:]).cpu(), c[0, :, :2])   # the two that fit
+    assert torch.equal(unpack_codes(cache.k_codes[1, :, :2]).cpu(), c[1, :, 2:])
+    assert torch.equal(cache.k_codes[0, :, :30], k0[0, :, :30]) and torch.equal(cache.k_codes[1, :, 2:], k0[1, :, 2:])
+
+
+def test_values_that_do_not_fit_make_their_group_nan(be, gpu):
+    x = torch.ones(1, 1, 6, 64)
+    x[0, 0, 1, 3] = float("nan")
+    x[0, 0, 2, 40] = float("inf")
+    x[0, 0, 3, 0] = -float("inf")
+    x[0, 0, 4, 33] = 65408.0                                   # the largest that fits: scale 9344
+    x[0, 0, 5, 33] = 70000.0
+    cache = KV4Cache.allocate(1, 1, 32, 64)
+    be.kv4_append(cache, x.to(gpu), x.to(gpu))
+    out = torch.empty(1, 1, 6, 64, device=gpu)
+    be.kv4_read(cache, out)
+    nan = torch.isnan(out[0, 0].cpu())
+    want = torch.zeros(6, 64, dtype=torch.bool)
+    want[1, :32] = want[2, 32:] = want[3, :32] = want[5, 32:] = True
+    assert torch.equal(nan, want)
+    assert out[0, 0, 4, 33].item() == 65408.0
+
+
+# ── attention ────────────────────────────────────────────────────────────────
+def attn64(q, cache, lens, Sk, causal, mask, scale):
+    """Definition in fp64: ([B, H, Sq, D] output, Σ p|v|)."""
+    k, v = (x.double()[:, :, :Sk] for x in cache.dequantize())
+    B, H, Sq, D = q.shape
+    g = H // k.shape[1]
+    k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+    j = torch.arange(Sk, device=q.device)
+    n = torch.full((B,), Sk, device=q.device) if lens is None else lens.long().clamp(0, Sk)
+    see = (j[None, :] < n[:, None])[:, None, :].expand(B, Sq, Sk)
+    if causal:
+        i = torch.arange(Sq, device=q.device)
+        see = see & (j[None, None] <= (n[:, None] - Sq + i[None])[:, :, None])
+    if mask is not None:
+        see = see & mask[:, None, :].bool()
+    see = see[:, None]
+    k, v = (torch.nan_to_num(x) if torch.isnan(x).any() else x for x in (k, v))     # masked slots may hold NaN
+    s = torch.einsum("bhid,bhjd->bhij", q.double(), k) * scale
+    s = s.masked_fill(~see, -1e300)
+    p = torch.softmax(s, -1) * see
+    return torch.einsum("bhij,bhjd->bhid", p, v), torch.einsum("bhij,bhjd->bhid", p, v.abs()), v.abs().amax()
+
+
+def run_attn(be, gpu, B, H, Hkv, Sq, Sk, D, dt, causal=False, lens=None, mask_p=None, layout="bhsd", scale=0.0,
+             splits=0, seed=0, cap=None, mask=None):
+    cache = KV4Cache.allocate(B, Hkv, max(cap or Sk, 1), D)
+    fill(cache, seed + 11)
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(B, H, Sq, D, generator=g).to(dt).to(gpu)
+    lt = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=gpu)
+    if mask_p is not None:
+        mask = (torch.rand(B, Sk, generator=g) < mask_p).to(gpu)
+    qq = q if layout == "bhsd" else q.transpose(1, 2).contiguous()
+    out = torch.full_like(qq, float("nan"))
+    be.kv4_attention(qq, cache, out, seq_k=Sk, kv_len=lt, mask=mask, scale=scale, is_causal=causal,
+                     num_splits=splits, layout=layout)
+    got = (out if layout == "bhsd" else out.transpose(1, 2)).double()
+    ref, mag, vmax = attn64(q, cache, lt, Sk, causal, mask, scale or 1 / math.sqrt(D))
+    tol = HALF[dt] * ref.abs() + (2.0 ** -11 + 2.0 ** -15) * mag + Sk * 2.0 ** -25 * vmax
+    err = (got - ref).abs()
+    assert not torch.isnan(got).any()
+    assert (err <= tol).all(), f"max excess {(err - tol).max().item():.3e}, max err {err.max().item():.3e}"
+    return q, cache, out
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sk", [1, 15, 16, 17, 100, 515, 4374])
+def test_single_token(be, gpu, dt, D, Sk):
+    run_attn(be, gpu, 2, 4, 4, 1, Sk, D, dt, seed=Sk)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,Hkv,Sq", [(8, 1, 1), (9, 1, 1), (16, 2, 2), (4, 4, 7), (4, 4, 16), (2, 1, 16), (3, 1, 11),
+                                      (2, 2, 67), (2, 2, 72), (2, 2, 73), (6, 2, 50), (1, 1, 300)])
+def test_rows_per_head(be, gpu, D, H, Hkv, Sq):
+    run_attn(be, gpu, 2, H, Hkv, Sq, 333, D, torch.bfloat16, seed=H * Sq)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq,Sk,lens", [(1, 200, [200, 1, 77]), (5, 200, [5, 200, 33]), (67, 130, [67, 130, 128]),
+                                        (9, 64, [3, 0, 8]), (40, 16, [16, 1, 0]), (150, 1000, [1000, 150, 149])])
+def test_causal_and_lengths(be, gpu, D, Sq, Sk, lens):
+    q, _, out = run_attn(be, gpu, 3, 4, 2, Sq, Sk, D, torch.float16, causal=True, lens=lens, layout="bshd", seed=Sq)
+    for b, n in enumerate(lens):                       # queries before the first slot see nothing: zeros
+        assert (out[b, :max(0, Sq - n)] == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq,H,Hkv", [(1, 2, 2), (67, 2, 2), (33, 4, 2), (130, 2, 1)])
+def test_key_masks(be, gpu, D, Sq, H, Hkv):
+    run_attn(be, gpu, 2, H, Hkv, Sq, 261, D, torch.bfloat16, mask_p=0.5, seed=Sq)
+    run_attn(be, gpu, 2, H, Hkv, Sq, 261, D, torch.bfloat16, mask_p=0.02, causal=True, lens=[261, 140], seed=Sq + 1)
+    m = torch.zeros(2, 261, dtype=torch.uint8, device=gpu)
+    m[1, 200] = 3                                      # any nonzero byte keeps its key
+    _, _, out = run_attn(be, gpu, 2, H, Hkv, Sq, 261, D, torch.bfloat16, mask=m, seed=Sq + 2)
+    assert (out[0] == 0).all()                         # a session whose mask leaves nothing
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8, 16])
+@pytest.mark.parametrize("Sq", [1, 20, 67])
+def test_splits(be, gpu, splits, Sq):
+    run_attn(be, gpu, 1, 2, 2, Sq, 700, 64, torch.bfloat16, splits=splits, seed=splits)
+    run_attn(be, gpu, 2, 2, 1, Sq, 40, 128, torch.float16, splits=splits, lens=[40, 17], seed=splits)
+
+
+def test_empty_cases(be, gpu):
+    for Sk, lens in ((0, None), (33, [0, 0])):
+        cache = KV4Cache.allocate(2, 2, 64, 64)
+        q = torch.randn(2, 2, 3, 64, device=gpu).half()
+        out = torch.full_like(q, float("nan"))
+        lt = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=gpu)
+        be.kv4_attention(q, cache, out, seq_k=Sk, kv_len=lt)
+        assert (out == 0).all()
+    q = torch.empty(2, 2, 0, 64, dtype=torch.half, device=gpu)
+    be.kv4_attention(q, cache, torch.empty_like(q))
+
+
+@pytest.mark.parametrize("Sq", [1, 67])
+@pytest.mark.parametrize("D", [64, 128])
+def test_masked_slots_may_hold_nan(be, gpu, Sq, D):
+    B, H, Sk = 2, 2, 150
+    cache = KV4Cache.allocate(B, H, Sk, D)
+    fill(cache, 21)
+    mask = torch.ones(B, Sk, dtype=torch.bool, device=gpu)
+    mask[0, 40] = mask[1, 0] = mask[1, 99] = False
+    lens = torch.tensor([100, 100], dtype=torch.int32, device=gpu)
+    clean_k, clean_v = cache.k_scale.clone(), cache.v_scale.clone()
+    for s in (cache.k_scale, cache.v_scale):
+        s[0, :, 40] = float("nan"); s[1, :, 0] = float("inf"); s[1, :, 99] = float("nan"); s[:, :, 100:] = float("nan")
+    q = torch.randn(B, H, Sq, D, generator=torch.Generator().manual_seed(5)).bfloat16().to(gpu)
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    be.kv4_attention(q, cache, out, kv_len=lens, mask=torch.nn.functional.pad(mask, (0, cache.shape[2] - Sk)))
+    clean = KV4Cache(cache.k_codes, cache.v_codes, clean_k, clean_v)
+    be.kv4_attention(q, clean, want, kv_len=lens, mask=torch.nn.functional.pad(mask, (0, cache.shape[2] - Sk)))
+    assert torch.equal(out, want) and not torch.isnan(out).any()
+
+
+def test_visible_nan_reaches_only_its_rows(be, gpu):
+    cache = KV4Cache.allocate(2, 1, 64, 64)
+    fill(cache, 22)
+    cache.k_scale[0, 0, 5] = float("nan")
+    q = torch.randn(2, 1, 4, 64, generator=torch.Generator().manual_seed(6)).bfloat16().to(gpu)
+    out = torch.empty_like(q)
+    be.kv4_attention(q, cache, out, is_causal=True, seq_k=7)
+    assert not torch.isnan(out[0, 0, :1]).any()        # query 0 sees slots 0..3, query 1 0..4
+    assert not torch.isnan(out[0, 0, 1]).any()
+    assert torch.isnan(out[0, 0, 2:]).all()            # slot 5 visible
+    assert not torch.isnan(out[1]).any()
+    cache.k_scale[0, 0] = float("nan")                 # every visible logit NaN
+    be.kv4_attention(q, cache, out)
+    assert torch.isnan(out[0]).all() and not torch.isnan(out[1]).any()
+
+
+def test_large_logits_and_scale(be, gpu):
+    # logits in the hundreds: the running reference moves far, one key dominates
+    cache = KV4Cache.allocate(1, 1, 640, 64)
+    fill(cache, 23, spread=6.0)
+    q = (torch.randn(1, 1, 9, 64, generator=torch.Generator().manual_seed(7)) * 5).half().to(gpu)
+    out = torch.empty_like(q)
+    be.kv4_attention(q, cache, out, scale=0.5)
+    ref, mag, vmax = attn64(q, cache, None, 640, False, None, 0.5)
+    # logits to about 2^10 of products whose magnitudes sum to 2^12: fp32 sums of 64
+    # terms leave them within 64 · 2^-24 · 2^12 = 2^-6 at worst
+    assert ((out.double() - ref).abs() <= 2.0 ** -5 * mag + 640 * 2.0 ** -25 * vmax).all()
+
+
+def test_out_of_range_queries_are_recorded(be, gpu):
+    cache = KV4Cache.allocate(1, 1, 32, 64)
+    q = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device=gpu)
+    q[..., 3] = 1e6
+    assert be.device_error(reset=True) == 0
+    be.kv4_attention(q, cache, torch.empty_like(q))
+    torch.cuda.synchronize()
+    assert be.device_error(reset=True) == _capi.SFB_ERR_RANGE
+
+
+def test_strided_caches_and_views(be, gpu):
+    # a cache whose batch and head strides have gaps, and Q / out inside wider buffers
+    B, H, C, D, Sq = 2, 2, 96, 64, 3
+    big = KV4Cache.allocate(B, 2 * H, C, D)
+    fill(big, 31)
+    view = KV4Cache(*(t[:, ::2] for t in (big.k_codes, big.v_codes, big.k_scale, big.v_scale)))
+    tight = KV4Cache(*(t[:, ::2].contiguous() for t in (big.k_codes, big.v_codes, big.k_scale, big.v_scale)))
+    wide = torch.randn(B, Sq, 3 * H, D, generator=torch.Generator().manual_seed(8)).bfloat16().to(gpu)
+    q = wide[:, :, H:2 * H]
+    obuf = torch.zeros(B, Sq, 4 * H, D, dtype=torch.bfloat16, device=gpu)
+    want = torch.empty(B, Sq, H, D, dtype=torch.bfloat16, device=gpu)
+    be.kv4_attention(q, view, obuf[:, :, H:2 * H], layout="bshd", seq_k=77)
+    be.kv4_attention(q.contiguous(), tight, want, layout="bshd", seq_k=77)
+    assert torch.equal(obuf[:, :, H:2 * H], want)
+    assert (obuf[:, :, :H] == 0).all() and (obuf[:, :, 2 * H:] == 0).all()
+
+
+def test_same_call_twice_and_graph_replay_give_the_same_bits(be, gpu):
+    cache = KV4Cache.allocate(2, 4, 2048, 64)
+    fill(cache, 41)
+    q = torch.randn(2, 4, 67, 64, generator=torch.Generator().manual_seed(9)).bfloat16().to(gpu)
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    be.kv4_attention(q, cache, a)
+    be.kv4_attention(q, cache, b)
+    assert torch.equal(a, b)
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    c, d = torch.zeros_like(q), torch.zeros_like(q)
+    with torch.cuda.graph(g1):
+        be.kv4_attention(q, cache, c)
+    with torch.cuda.graph(g2):
+        be.kv4_attention(q, cache, d)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for s in (s1, s2):
+        s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s1):
+        g1.replay()
+    with torch.cuda.stream(s2):                        # two graphs at once share nothing
+        g2.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(a, c) and torch.equal(a, d)
+
+
+def test_offsets_past_32_bits(be, gpu):
+    # one head's codes start beyond 4 GB of the buffer: a strided view of a 4.4 GB allocation
+    D, cap, gap = 64, 64, 4_400_000_000
+    buf = torch.zeros(gap + 2 * cap * D, dtype=torch.uint8, device=gpu)
+    code = buf.as_strided((2, 1, cap, D // 2), (gap, cap * D // 2, D // 2, 1))
+    src = KV4Cache.allocate(2, 1, cap, D)
+    fill(src, 51)
+    code.copy_(src.k_codes)
+    vcode = buf[cap * D:].as_strided((2, 1, cap, D // 2), (gap, cap * D // 2, D // 2, 1))
+    vcode.copy_(src.v_codes)
+    far = KV4Cache(code, vcode, src.k_scale, src.v_scale)
+    q = torch.randn(2, 2, 1, D, generator=torch.Generator().manual_seed(10)).bfloat16().to(gpu)
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    be.kv4_attention(q, far, a)
+    be.kv4_attention(q, src, b)
+    assert torch.equal(a, b)
+
+
+def test_wrapper_refusals(be, gpu):
+    cache = KV4Cache.allocate(2, 2, 64, 64)
+    q = torch.zeros(2, 4, 3, 64, dtype=torch.bfloat16, device=gpu)
+    out = torch.empty_like(q)
+    E = _capi.SfbError
+    with pytest.raises(E):
+        be.kv4_attention(q.float(), cache, out.float())
+    with pytest.raises(E):
+        be.kv4_attention(q, cache, out.half())
+    with pytest.raises(E):
+        be.kv4_attention(q[:1], cache, out[:1])
+    with pytest.raises(E):
+        be.kv4_attention(q[:, :3], cache, out[:, :3])                  # heads not a multiple
+    with pytest.raises(E):
+        be.kv4_attention(q, cache, out, seq_k=65)
+    with pytest.raises(E):
+        be.kv4_attention(q, cache, out, kv_len=torch.zeros(2, dtype=torch.int64, device=gpu))
+    with pytest.raises(E):
+        be.kv4_attention(q, cache, out, mask=torch.ones(2, 63, dtype=torch.bool, device=gpu))
+    with pytest.raises(ValueError):
+        be.kv4_attention(q.cpu(), cache, out)
+    with pytest.raises(ValueError):
+        be.kv4_attention(q, cache, out, layout="sbhd")
+    with pytest.raises(E):
+        be.kv4_append(cache, q[:, :2], q[:, :2], start=62)             # past the last slot
+    with pytest.raises(E):
+        be.kv4_append(cache, q, q)
+    with pytest.raises(E):
+        be.kv4_read(cache)
+    bad = KV4Cache(cache.k_codes, cache.v_codes, cache.k_scale.float(), cache.v_scale)
+    with pytest.raises(E):
+        be.kv4_attention(q, bad, out)

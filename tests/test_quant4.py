@@ -1,0 +1,246 @@
+"""CPU tests of the 4-bit formats (servoflow_b200.quant4) and of the refusals of
+the 4-bit and norm-rotation entry points that need no device."""
+import ctypes
+import struct
+
+import pytest
+import torch
+
+from servoflow_b200 import _capi, quant4
+from servoflow_b200._capi import SfbError
+
+
+def test_packing_follows_the_bit_positions():
+    # value 2i of eight at bits 4i, value 2i+1 at bits 16+4i, nibble = c + 8
+    codes = torch.tensor([[-8, 7, 0, 1, -1, 3, 5, -4], [2, 2, -3, 6, 7, -8, 0, -7]], dtype=torch.int32)
+    packed = quant4.pack_codes(codes)
+    assert packed.shape == (2, 4) and packed.dtype == torch.uint8
+    for row, b in zip(codes.tolist(), packed.tolist()):
+        word = struct.unpack("<I", bytes(b))[0]
+        got = [((word >> (4 * (e // 2) + 16 * (e % 2))) & 15) - 8 for e in range(8)]
+        assert got == row
+
+
+@pytest.mark.parametrize("shape", [(8,), (3, 64), (2, 5, 128), (0, 32)])
+def test_unpack_inverts_pack(shape):
+    g = torch.Generator().manual_seed(1)
+    codes = torch.randint(-8, 8, shape, generator=g, dtype=torch.int32)
+    assert torch.equal(quant4.unpack_codes(quant4.pack_codes(codes)).to(torch.int32), codes)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_pack_w4_error_is_half_a_step(group):
+    g = torch.Generator().manual_seed(group)
+    w = torch.randn(24, 256, generator=g) * 0.05
+    w[3] = 0                                           # a row of zeros: scale 0, codes 0
+    packed, s = quant4.pack_w4(w, group, torch.float32)
+    assert packed.shape == (24, 128) and s.shape == (24, 256 // group)
+    back = quant4.unpack_codes(packed).float().unflatten(1, (-1, group)) * s.unsqueeze(-1)
+    # fp32 scales: max|w| / 7 up to one rounding, so no code is clamped by more than that
+    assert ((back.flatten(1) - w).abs() <= (s.unsqueeze(-1).expand(-1, -1, group).flatten(1)) * (0.5 + 1e-5)).all()
+    assert (s[3] == 0).all() and (back[3] == 0).all()
+
+
+def test_packing_refusals():
+    with pytest.raises(SfbError):
+        quant4.pack_codes(torch.zeros(4, 12, dtype=torch.int32))
+    with pytest.raises(SfbError):
+        quant4.pack_w4(torch.zeros(4, 96), 64)
+    with pytest.raises(SfbError):
+        quant4.pack_w4(torch.zeros(4, 96), 48)
+    with pytest.raises(SfbError):
+        quant4.KV4Cache.allocate(1, 1, 32, 96, device="cpu")
+
+
+def test_cache_allocation_is_zero_and_rounded():
+    c = quant4.KV4Cache.allocate(2, 3, 33, 64, device="cpu")
+    assert c.shape == (2, 3, 64, 64)
+    k, v = c.dequantize()
+    assert (k == 0).all() and (v == 0).all() and k.shape == (2, 3, 64, 64)
+    with pytest.raises(ValueError):                    # the struct needs a CUDA cache
+        c.struct()
+
+
+def _offsets(struct_name, fields):
+    import os
+    import subprocess
+    import tempfile
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    prints = ", ".join(f"offsetof({struct_name}, {f})" for f in fields)
+    src = ("#include <stddef.h>\n#include <stdio.h>\n#include \"sfb200.h\"\n"
+           f"int main(void) {{ printf(\"{'%zu ' * (len(fields) + 1)}\\n\", {prints}, sizeof({struct_name})); "
+           "return 0; }\n")
+    with tempfile.TemporaryDirectory() as d:
+        c = os.path.join(d, "t.c")
+        with open(c, "w") as f:
+            f.write(src)
+        exe = os.path.join(d, "t")
+        subprocess.run(["gcc", "-I", os.path.join(root, "include"), c, "-o", exe], check=True)
+        return list(map(int, subprocess.run([exe], capture_output=True, text=True).stdout.split()))
+
+
+def test_struct_mirrors_have_the_c_layout():
+    for name, py, rename in (("sfb_kv4_cache", _capi.Kv4Cache,
+                              {"code_stride0": "code_stride[0]", "code_stride1": "code_stride[1]",
+                               "scale_stride0": "scale_stride[0]", "scale_stride1": "scale_stride[1]"}),
+                             ("sfb_kv4_attn_args", _capi.Kv4AttnArgs, {}),
+                             ("sfb_norm_rope_args", _capi.NormRopeArgs, {})):
+        fields = [f for f, _ in py._fields_]
+        want = [getattr(py, f).offset for f in fields] + [ctypes.sizeof(py)]
+        assert _offsets(name, [rename.get(f, f) for f in fields]) == want, name
+
+
+def _cache(**over):
+    c = _capi.Kv4Cache()
+    c.k_codes = c.v_codes = c.k_scale = c.v_scale = 0x1000
+    c.code_stride0, c.code_stride1, c.scale_stride0, c.scale_stride1 = 8192, 2048, 512, 128
+    c.batch, c.heads_kv, c.capacity, c.head_dim = 2, 4, 64, 64
+    for k, v in over.items():
+        setattr(c, k, v)
+    return c
+
+
+BAD_CACHES = [
+    (dict(k_codes=None), _capi.SFB_ERR_INVALID), (dict(v_scale=None), _capi.SFB_ERR_INVALID),
+    (dict(head_dim=96), _capi.SFB_ERR_SHAPE), (dict(head_dim=0), _capi.SFB_ERR_SHAPE),
+    (dict(heads_kv=0), _capi.SFB_ERR_SHAPE), (dict(capacity=-1), _capi.SFB_ERR_SHAPE),
+    (dict(k_codes=0x1008), _capi.SFB_ERR_ALIGN), (dict(v_scale=0x1002), _capi.SFB_ERR_ALIGN),
+    (dict(code_stride1=2056), _capi.SFB_ERR_ALIGN), (dict(scale_stride0=514), _capi.SFB_ERR_ALIGN),
+]
+
+
+@pytest.mark.parametrize("over,status", BAD_CACHES)
+def test_bad_caches_are_refused_by_every_entry_point(over, status):
+    lib = _capi.lib()
+    c = _cache(**over)
+    st = (ctypes.c_int64 * 3)(8192, 64, 256)
+    assert lib.sfb_kv4_append(ctypes.byref(c), 0x2000, st, 0x2000, st, _capi.SFB_BF16, 1, None, 0, None, None) == status
+    assert lib.sfb_kv4_read(ctypes.byref(c), 0x2000, st, 0x2000, st, _capi.SFB_F16, 0, 1, None) == status
+    a = _capi.Kv4AttnArgs()
+    a.cache, a.q, a.out = ctypes.addressof(c), 0x2000, 0x3000
+    a.heads, a.seq_q, a.seq_k, a.dtype = 4, 1, 32, _capi.SFB_BF16
+    assert lib.sfb_kv4_attention(ctypes.byref(a), None) == status
+
+
+def test_append_and_read_refusals():
+    lib = _capi.lib()
+    c = ctypes.byref(_cache())
+    st = (ctypes.c_int64 * 3)(8192, 64, 256)
+    odd = (ctypes.c_int64 * 3)(8192, 64, 255)
+    E = _capi
+    append = lambda cc, k, ks, v, vs, dt, seq, slot: lib.sfb_kv4_append(cc, k, ks, v, vs, dt, seq, None, slot, None, None)
+    assert append(None, 0x2000, st, 0x2000, st, E.SFB_BF16, 1, 0) == E.SFB_ERR_INVALID
+    assert append(c, None, st, 0x2000, st, E.SFB_BF16, 1, 0) == E.SFB_ERR_INVALID
+    assert append(c, 0x2000, None, 0x2000, st, E.SFB_BF16, 1, 0) == E.SFB_ERR_INVALID
+    assert append(c, 0x2000, st, 0x2000, st, E.SFB_I8, 1, 0) == E.SFB_ERR_DTYPE
+    assert append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, -1, 0) == E.SFB_ERR_SHAPE
+    assert append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 65, 0) == E.SFB_ERR_SHAPE      # past the capacity
+    assert append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 1, 64) == E.SFB_ERR_SHAPE
+    assert append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 1, -1) == E.SFB_ERR_SHAPE
+    assert append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 2 ** 31 - 1, 2 ** 31 - 1) == E.SFB_ERR_SHAPE
+    assert append(c, 0x2008, st, 0x2000, st, E.SFB_BF16, 1, 0) == E.SFB_ERR_ALIGN
+    assert append(c, 0x2000, st, 0x2000, odd, E.SFB_BF16, 1, 0) == E.SFB_ERR_ALIGN
+    assert append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 0, 0) == E.SFB_OK              # nothing to do
+    read = lambda k, ks, v, vs, dt, slot, seq: lib.sfb_kv4_read(c, k, ks, v, vs, dt, slot, seq, None)
+    assert read(None, st, None, st, E.SFB_F16, 0, 1) == E.SFB_ERR_INVALID
+    assert read(0x2000, st, None, None, E.SFB_I32, 0, 1) == E.SFB_ERR_DTYPE
+    assert read(0x2000, st, None, None, E.SFB_F16, 0, 65) == E.SFB_ERR_SHAPE
+    assert read(0x2000, st, None, None, E.SFB_F16, -1, 1) == E.SFB_ERR_SHAPE
+    assert read(0x2004, st, None, None, E.SFB_F16, 0, 1) == E.SFB_ERR_ALIGN
+    assert read(0x2000, st, None, None, E.SFB_F16, 64, 0) == E.SFB_OK
+
+
+def test_attention_refusals():
+    lib, E = _capi.lib(), _capi
+    c = _cache()
+
+    def call(**over):
+        a = _capi.Kv4AttnArgs()
+        a.cache, a.q, a.out = ctypes.addressof(c), 0x2000, 0x3000
+        a.heads, a.seq_q, a.seq_k, a.dtype = 8, 3, 64, E.SFB_BF16
+        a.q_stride[0] = a.q_stride[1] = a.q_stride[2] = a.out_stride[0] = a.out_stride[1] = a.out_stride[2] = 64
+        for k, v in over.items():
+            if k in ("q_stride", "out_stride"):
+                getattr(a, k)[2] = v
+            else:
+                setattr(a, k, v)
+        return lib.sfb_kv4_attention(ctypes.byref(a), None)
+
+    assert lib.sfb_kv4_attention(None, None) == E.SFB_ERR_INVALID
+    assert call(cache=None) == E.SFB_ERR_INVALID
+    assert call(q=None) == E.SFB_ERR_INVALID
+    assert call(dtype=E.SFB_F32) == E.SFB_ERR_DTYPE
+    assert call(heads=6) == E.SFB_ERR_SHAPE
+    assert call(heads=0) == E.SFB_ERR_SHAPE
+    assert call(seq_k=65) == E.SFB_ERR_SHAPE
+    assert call(seq_k=-1) == E.SFB_ERR_SHAPE
+    assert call(seq_q=-1) == E.SFB_ERR_SHAPE
+    assert call(seq_q=2 ** 31 - 1) == E.SFB_ERR_SHAPE
+    assert call(num_splits=17) == E.SFB_ERR_INVALID
+    assert call(q=0x2002) == E.SFB_ERR_ALIGN
+    assert call(q_stride=67) == E.SFB_ERR_ALIGN
+    assert call(out_stride=68) == E.SFB_ERR_ALIGN
+    assert call(seq_q=0) == E.SFB_OK
+
+
+def test_norm_rope_refusals():
+    lib, E = _capi.lib(), _capi
+
+    def call(**over):
+        a = _capi.NormRopeArgs()
+        a.q = a.q_out = a.k = a.k_out = 0x1000
+        for f in ("q_stride", "k_stride", "q_out_stride", "k_out_stride"):
+            for i in range(3):
+                getattr(a, f)[i] = 64
+        a.cos_table = a.sin_table = 0x4000
+        a.table_len, a.batch, a.seq, a.heads, a.heads_kv, a.head_dim = 10, 2, 3, 4, 2, 64
+        a.rotary_dim, a.norm, a.dtype, a.eps = 64, 1, E.SFB_BF16, 1e-6
+        for k, v in over.items():
+            if k.endswith("_stride"):
+                getattr(a, k)[1] = v
+            else:
+                setattr(a, k, v)
+        return lib.sfb_qk_norm_rope(ctypes.byref(a), None)
+
+    assert lib.sfb_qk_norm_rope(None, None) == E.SFB_ERR_INVALID
+    assert call(q=None) == E.SFB_ERR_INVALID                      # an output without its input
+    assert call(q=None, q_out=None, k=None, k_out=None) == E.SFB_ERR_INVALID
+    assert call(cos_table=None) == E.SFB_ERR_INVALID
+    assert call(dtype=E.SFB_I8) == E.SFB_ERR_DTYPE
+    assert call(head_dim=60) == E.SFB_ERR_SHAPE
+    assert call(head_dim=264, rotary_dim=0) == E.SFB_ERR_SHAPE
+    assert call(rotary_dim=8) == E.SFB_ERR_SHAPE
+    assert call(rotary_dim=80) == E.SFB_ERR_SHAPE
+    assert call(batch=-1) == E.SFB_ERR_SHAPE
+    assert call(q=0x1004, q_out=0x1004) == E.SFB_ERR_ALIGN
+    assert call(k_out_stride=65) == E.SFB_ERR_ALIGN
+    assert call(sin_table=0x4004) == E.SFB_ERR_ALIGN
+    assert call(batch=0) == E.SFB_OK
+    assert call(seq=0) == E.SFB_OK
+
+
+def test_linear_refusals():
+    lib, E = _capi.lib(), _capi
+
+    def call(x=0x1000, ldx=256, xd=E.SFB_BF16, w=0x2000, ws=0x3000, sd=E.SFB_F16, G=64, b=None, r=None, ldr=0,
+             y=0x5000, ldy=40, yd=E.SFB_BF16, M=3, N=40, K=256, act=0):
+        return lib.sfb_w4a16_linear(x, ldx, xd, w, ws, sd, G, b, r, ldr, y, ldy, yd, M, N, K, act, None)
+
+    for name in ("x", "w", "ws", "y"):
+        assert call(**{name: None}) == E.SFB_ERR_INVALID
+    assert call(act=3) == E.SFB_ERR_INVALID
+    assert call(G=16) == E.SFB_ERR_SHAPE
+    assert call(K=96, ldx=96, G=64) == E.SFB_ERR_SHAPE
+    assert call(M=-1) == E.SFB_ERR_SHAPE
+    assert call(N=0) == E.SFB_ERR_SHAPE
+    assert call(ldx=248) == E.SFB_ERR_SHAPE
+    assert call(ldy=39) == E.SFB_ERR_SHAPE
+    assert call(r=0x6000, ldr=39) == E.SFB_ERR_SHAPE
+    assert call(xd=E.SFB_F32) == E.SFB_ERR_DTYPE
+    assert call(yd=E.SFB_F16) == E.SFB_ERR_DTYPE
+    assert call(sd=E.SFB_I8) == E.SFB_ERR_DTYPE
+    assert call(x=0x1008) == E.SFB_ERR_ALIGN
+    assert call(w=0x2004) == E.SFB_ERR_ALIGN
+    assert call(ldx=260) == E.SFB_ERR_ALIGN
+    assert call(y=0x5001) == E.SFB_ERR_ALIGN
+    assert call(M=0) == E.SFB_OK
