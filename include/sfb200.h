@@ -349,7 +349,6 @@ int sfb_kv4_read(const sfb_kv4_cache* cache, void* k, const int64_t* k_stride, v
  * - num_splits: key splits merged inside one thread-block cluster (0 = choose,
  *   else 1..16). Allocates nothing, keeps no workspace. */
 typedef struct sfb_kv4_attn_args {
-    const sfb_kv4_cache* cache;
     const void* q;
     void*       out;
     int64_t q_stride[3];
@@ -366,7 +365,7 @@ typedef struct sfb_kv4_attn_args {
     float   scale;
 } sfb_kv4_attn_args;
 
-int sfb_kv4_attention(const sfb_kv4_attn_args* args, void* stream);
+int sfb_kv4_attention(const sfb_kv4_cache* cache, const sfb_kv4_attn_args* args, void* stream);
 
 /* ── 4-bit-weight linear layer ────────────────────────────────────────────────
  * sfb_w8a16_linear's layer with 4-bit weights and a scale per `group`

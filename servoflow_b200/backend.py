@@ -123,51 +123,42 @@ _HALVES = (torch.float16, torch.bfloat16)
 _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
 
 
-def _one_device(first: torch.Tensor, name: str, *others) -> torch.device:
+def _device_index(name: str, first: torch.Tensor, *others) -> int:
     """The CUDA device of `first`; raises unless every other tensor (or None) is on it."""
-    _check_device(first, name)
-    dev = first.device
-    for t, n in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{n} must be on {name}'s device {dev}, not {t.device}")
-    return dev
+    i = first.get_device()
+    if i < 0:
+        _check_device(first, name)
+    for t in others:
+        if t is not None and t.get_device() != i:
+            raise ValueError(f"every tensor of a call must be on {name}'s device cuda:{i}, not {t.device}")
+    return i
 
 
-def _layout(layout: str):
-    """Positions of (batch, head, seq) in a 4-D shape."""
-    if layout == "bhsd":
-        return 0, 1, 2
-    if layout == "bshd":
-        return 0, 2, 1
-    raise ValueError(f"unknown layout {layout!r}")
+_ORDER = {"bhsd": (0, 1, 2), "bshd": (0, 2, 1)}     # positions of (batch, head, seq) in a 4-D shape
 
 
-def _strides3(t: torch.Tensor, order) -> "ctypes.Array":
-    st = t.stride()
-    return (ctypes.c_int64 * 3)(st[order[0]], st[order[1]], st[order[2]])
+def _order(layout: str):
+    try:
+        return _ORDER[layout]
+    except KeyError:
+        raise ValueError(f"unknown layout {layout!r}") from None
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
-class _on_device:
-    """Makes a tensor's device current around a library call, and picks the
-    stream: the caller's, or that device's current one."""
-
-    __slots__ = ("_index", "_prev")
-
-    def __init__(self, device: torch.device):
-        self._index = device.index
-
-    def __enter__(self):
-        self._prev = torch.cuda.current_device()
-        if self._prev != self._index:
-            torch.cuda.set_device(self._index)
-
-    def __exit__(self, *exc):
-        if self._prev != self._index:
-            torch.cuda.set_device(self._prev)
+def _call(fn, what: str, index: int, stream, *args) -> None:
+    """Calls a library function on device `index`, on the given stream or that
+    device's current one, and raises for its status."""
+    current = torch.cuda.current_device()
+    if current != index:
+        with torch.cuda.device(index):
+            return _call(fn, what, index, stream, *args)
+    s = torch._C._cuda_getCurrentRawStream(index) if stream is None else _stream_handle(stream)
+    status = fn(*args, s)
+    if status != 0:
+        raise _capi.SfbError(status, what)
 
 
 class B200Backend:
@@ -259,64 +250,70 @@ class B200Backend:
         k_out, which may be q and k. k (with k_out) or q (with q_out) may be
         None. Raises for shapes and types; a position outside the tables leaves
         its token unwritten and records SFB_ERR_RANGE (device_error)."""
-        order = _layout(layout)
-        x, x_name = (q, "q") if q is not None else (k, "k")
+        o = _order(layout)
+        x = q if q is not None else k
         if x is None or (q is None) != (q_out is None) or (k is None) != (k_out is None):
             raise _capi.SfbError(_capi.SFB_ERR_INVALID, "q or k with its output expected")
-        dev = _one_device(x, x_name, (q_out, "q_out"), (k, "k"), (k_out, "k_out"), (q_weight, "q_weight"),
-                          (k_weight, "k_weight"), (cos, "cos"), (sin, "sin"), (positions, "positions"))
+        dev = _device_index("q" if q is not None else "k", x, q_out, k, k_out, q_weight, k_weight, cos, sin, positions)
         dt = x.dtype
         if dt not in _FLOATS:
             raise _capi.SfbError(_capi.SFB_ERR_DTYPE, f"dtype {dt}")
-        a = _capi.NormRopeArgs()
-        D = x.shape[-1]
-        for t, o, w, n in ((q, q_out, q_weight, "q"), (k, k_out, k_weight, "k")):
+        B, _, _, D = shape = x.shape if x.dim() == 4 else self._not_4d("q")
+        S = shape[o[2]]
+
+        def side(t, out, w, name):
+            """Pointers, head count and strides of one of q and k."""
             if t is None:
-                continue
-            if t.dim() != 4 or o.shape != t.shape or t.shape[3] != D or t.shape[0] != x.shape[0] \
-                    or t.shape[order[2]] != x.shape[order[2]]:
-                raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"inconsistent {n} shapes")
-            if D > 1 and (t.stride(3) != 1 or o.stride(3) != 1):
-                raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"{n}: head_dim must be contiguous")
-            if t.dtype != dt or o.dtype != dt or (w is not None and w.dtype != dt):
+                return 0, 0, 0, 0, (0, 0, 0), (0, 0, 0)
+            sh, st, so = t.shape, t.stride(), out.stride()
+            if len(sh) != 4 or out.shape != sh or sh[0] != B or sh[o[2]] != S or sh[3] != D:
+                raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"inconsistent {name} shapes")
+            if D > 1 and (st[3] != 1 or so[3] != 1):
+                raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"{name}: head_dim must be contiguous")
+            if t.dtype is not dt or out.dtype is not dt or (w is not None and w.dtype is not dt):
                 raise _capi.SfbError(_capi.SFB_ERR_DTYPE, "q, k, outputs and weights share one dtype")
-            if w is not None and (tuple(w.shape) != (D,) or not w.is_contiguous()):
-                raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"{n}_weight must be contiguous [head_dim]")
-        if q is not None:
-            a.q, a.q_out, a.heads, a.q_weight = q.data_ptr(), q_out.data_ptr(), q.shape[order[1]], _ptr(q_weight)
-            a.q_stride, a.q_out_stride = _strides3(q, order), _strides3(q_out, order)
-        if k is not None:
-            a.k, a.k_out, a.heads_kv, a.k_weight = k.data_ptr(), k_out.data_ptr(), k.shape[order[1]], _ptr(k_weight)
-            a.k_stride, a.k_out_stride = _strides3(k, order), _strides3(k_out, order)
-        a.batch, a.seq, a.head_dim, a.dtype = x.shape[0], x.shape[order[2]], D, _DTYPE_CODE[dt]
+            if w is not None and (w.shape != (D,) or not w.is_contiguous()):
+                raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"{name}_weight must be contiguous [head_dim]")
+            return (t.data_ptr(), out.data_ptr(), _ptr(w), sh[o[1]], (st[o[0]], st[o[1]], st[o[2]]),
+                    (so[o[0]], so[o[1]], so[o[2]]))
+
+        qp, qop, qw, H, qs, qos = side(q, q_out, q_weight, "q")
+        kp, kop, kw, Hkv, ks, kos = side(k, k_out, k_weight, "k")
+        table = rot = pos = pos_sb = 0
         if (cos is None) != (sin is None):
             raise _capi.SfbError(_capi.SFB_ERR_INVALID, "cos and sin come together")
         if cos is not None:
             if cos.dim() != 2 or cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous():
                 raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "cos / sin must be contiguous [positions, rot / 2]")
-            if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
                 raise _capi.SfbError(_capi.SFB_ERR_DTYPE, "cos / sin must be fp32")
-            a.cos_table, a.sin_table = cos.data_ptr(), sin.data_ptr()
-            a.table_len, a.rotary_dim = cos.shape[0], 2 * cos.shape[1]
+            table, rot = cos.shape
+            rot *= 2
             if positions is not None:
-                if positions.dtype != torch.int32:
+                if positions.dtype is not torch.int32:
                     raise _capi.SfbError(_capi.SFB_ERR_DTYPE, "positions must be int32")
-                if tuple(positions.shape) != (a.batch, a.seq) or (a.seq > 1 and positions.stride(1) != 1):
+                if positions.shape != (B, S) or (S > 1 and positions.stride(1) != 1):
                     raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "positions must be [B, S], row-contiguous")
-                a.positions, a.pos_stride_b = positions.data_ptr(), positions.stride(0)
-        a.interleaved, a.norm, a.eps = 1 if interleaved else 0, 1 if norm else 0, float(eps)
-        with _on_device(dev):
-            _capi.check(self._lib.sfb_qk_norm_rope(ctypes.byref(a), _stream_handle(stream)), "qk_norm_rope")
+                pos, pos_sb = positions.data_ptr(), positions.stride(0)
+        args = _capi.NORM_ROPE_ARGS.pack(
+            qp, kp, qop, kop, *qs, *ks, *qos, *kos, qw, kw, _ptr(cos), _ptr(sin), pos, pos_sb, table, B, S, H, Hkv, D,
+            rot, 1 if interleaved else 0, 1 if norm else 0, _DTYPE_CODE[dt], eps)
+        _call(self._lib.sfb_qk_norm_rope, "qk_norm_rope", dev, stream, args)
+
+    @staticmethod
+    def _not_4d(name):
+        raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"{name} must be 4-D")
 
     # The K/V cache held in 4 bits (quant4.KV4Cache)
-    def _kv4_side(self, cache, c, t, name, order, dt):
-        if t.dim() != 4 or t.shape[0] != c.batch or t.shape[order[1]] != c.heads_kv or t.shape[3] != c.head_dim:
+    @staticmethod
+    def _kv4_side(t, name, o, B, Hkv, D):
+        """Packed strides (batch, head, seq) of a 16- or 32-bit K or V that fits the cache."""
+        sh, st = t.shape, t.stride()
+        if len(sh) != 4 or sh[0] != B or sh[o[1]] != Hkv or sh[3] != D:
             raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"{name} does not fit the cache")
-        if t.stride(3) != 1:
+        if st[3] != 1:
             raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"{name}: head_dim must be contiguous")
-        if t.dtype != dt or dt not in _FLOATS:
-            raise _capi.SfbError(_capi.SFB_ERR_DTYPE, f"{name} dtype {t.dtype}")
-        return ctypes.byref(_strides3(t, order))
+        return _capi.I64X3.pack(st[0], st[o[1]], st[o[2]])
 
     def kv4_append(self, cache, K, V, start=0, lens=None, layout: str = "bhsd", stream=None) -> None:
         """Quantises K and V ([B, Hkv, S, D] or, layout "bshd", [B, S, Hkv, D])
@@ -324,40 +321,38 @@ class B200Backend:
         int, or int32 [B]), only the first lens[b] tokens where lens (int32 [B])
         is given. With tensor starts, tokens outside the cache are not written
         and record SFB_ERR_RANGE (device_error)."""
-        order = _layout(layout)
-        c = cache.struct()
+        o = _order(layout)
+        c, B, Hkv, _, D, _ = cache.pack()
         start_t = start if isinstance(start, torch.Tensor) else None
-        dev = _one_device(cache.k_codes, "cache", (K, "K"), (V, "V"), (start_t, "start"), (lens, "lens"))
+        dev = _device_index("cache", cache.k_codes, K, V, start_t, lens)
         if K.shape != V.shape:
             raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "K and V shapes differ")
-        ks = self._kv4_side(cache, c, K, "K", order, K.dtype)
-        vs = self._kv4_side(cache, c, V, "V", order, K.dtype)
+        if K.dtype not in _FLOATS or V.dtype is not K.dtype:
+            raise _capi.SfbError(_capi.SFB_ERR_DTYPE, "K and V share one float dtype")
+        ks, vs = self._kv4_side(K, "K", o, B, Hkv, D), self._kv4_side(V, "V", o, B, Hkv, D)
         for t, n in ((start_t, "start"), (lens, "lens")):
-            if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (c.batch,) or not t.is_contiguous()):
+            if t is not None and (t.dtype is not torch.int32 or t.shape != (B,) or not t.is_contiguous()):
                 raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"{n} must be contiguous int32 [B]")
-        with _on_device(dev):
-            _capi.check(self._lib.sfb_kv4_append(
-                ctypes.byref(c), K.data_ptr(), ks, V.data_ptr(), vs, _DTYPE_CODE[K.dtype], K.shape[order[2]],
-                _ptr(start_t), 0 if start_t is not None else int(start), _ptr(lens), _stream_handle(stream)),
-                "kv4_append")
+        _call(self._lib.sfb_kv4_append, "kv4_append", dev, stream, c, K.data_ptr(), ks, V.data_ptr(), vs,
+              _DTYPE_CODE[K.dtype], K.shape[o[2]], _ptr(start_t), 0 if start_t is not None else int(start), _ptr(lens))
 
     def kv4_read(self, cache, K=None, V=None, slot0: int = 0, layout: str = "bhsd", stream=None) -> None:
         """Writes the values of slots [slot0, slot0 + S) into K and V ([B, Hkv,
         S, D] or bshd; fp16 and fp32 exactly, bf16 rounded); either may be None."""
-        order = _layout(layout)
-        c = cache.struct()
+        o = _order(layout)
+        c, B, Hkv, _, D, _ = cache.pack()
         x = K if K is not None else V
         if x is None:
             raise _capi.SfbError(_capi.SFB_ERR_INVALID, "K or V expected")
-        dev = _one_device(cache.k_codes, "cache", (K, "K"), (V, "V"))
-        if K is not None and V is not None and K.shape != V.shape:
-            raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "K and V shapes differ")
-        ks = None if K is None else self._kv4_side(cache, c, K, "K", order, x.dtype)
-        vs = None if V is None else self._kv4_side(cache, c, V, "V", order, x.dtype)
-        with _on_device(dev):
-            _capi.check(self._lib.sfb_kv4_read(
-                ctypes.byref(c), _ptr(K), ks, _ptr(V), vs, _DTYPE_CODE[x.dtype], int(slot0), x.shape[order[2]],
-                _stream_handle(stream)), "kv4_read")
+        dev = _device_index("cache", cache.k_codes, K, V)
+        if K is not None and V is not None and (K.shape != V.shape or K.dtype is not V.dtype):
+            raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "K and V differ in shape or dtype")
+        if x.dtype not in _FLOATS:
+            raise _capi.SfbError(_capi.SFB_ERR_DTYPE, f"dtype {x.dtype}")
+        ks = None if K is None else self._kv4_side(K, "K", o, B, Hkv, D)
+        vs = None if V is None else self._kv4_side(V, "V", o, B, Hkv, D)
+        _call(self._lib.sfb_kv4_read, "kv4_read", dev, stream, c, _ptr(K), ks, _ptr(V), vs, _DTYPE_CODE[x.dtype],
+              int(slot0), x.shape[o[2]])
 
     def kv4_attention(self, Q, cache, out, seq_k: Optional[int] = None, kv_len=None, mask=None,
                       scale: float = 0.0, is_causal: bool = False, num_splits: int = 0,
@@ -367,35 +362,33 @@ class B200Backend:
         cache's heads. kv_len: int32 [B] valid slots; mask: bool/uint8 [B,
         seq_k] (True = keep); is_causal: the queries are the last Sq tokens of
         the valid slots. A query that sees no slot gives zeros."""
-        order = _layout(layout)
-        c = cache.struct()
-        dev = _one_device(cache.k_codes, "cache", (Q, "Q"), (out, "out"), (kv_len, "kv_len"), (mask, "mask"))
-        if Q.dtype not in _HALVES or out.dtype != Q.dtype:
+        o = _order(layout)
+        c, B, _, cap, D, _ = cache.pack()
+        dev = _device_index("cache", cache.k_codes, Q, out, kv_len, mask)
+        dt, sh, st, so = Q.dtype, Q.shape, Q.stride(), out.stride()
+        if dt not in _HALVES or out.dtype is not dt:
             raise _capi.SfbError(_capi.SFB_ERR_DTYPE, "Q and out must be bf16 or fp16, alike")
-        shape = Q.shape
-        if len(shape) != 4 or out.shape != shape or shape[0] != c.batch or shape[3] != c.head_dim:
+        if len(sh) != 4 or out.shape != sh or sh[0] != B or sh[3] != D:
             raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "Q and out must be 4-D and fit the cache")
-        if Q.stride(3) != 1 or out.stride(3) != 1:
+        if st[3] != 1 or so[3] != 1:
             raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "head_dim must be contiguous")
-        a = _capi.Kv4AttnArgs()
-        a.cache = ctypes.addressof(c)
-        a.q, a.out = Q.data_ptr(), out.data_ptr()
-        a.q_stride, a.out_stride = _strides3(Q, order), _strides3(out, order)
-        a.heads, a.seq_q = shape[order[1]], shape[order[2]]
-        sk = a.seq_k = c.capacity if seq_k is None else int(seq_k)
-        a.dtype, a.is_causal, a.num_splits, a.scale = _DTYPE_CODE[Q.dtype], 1 if is_causal else 0, num_splits, scale
+        sk = cap if seq_k is None else int(seq_k)
+        lens = keep = keep_sb = 0
         if kv_len is not None:
-            if kv_len.dtype != torch.int32 or tuple(kv_len.shape) != (c.batch,) or not kv_len.is_contiguous():
+            if kv_len.dtype is not torch.int32 or kv_len.shape != (B,) or not kv_len.is_contiguous():
                 raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "kv_len must be contiguous int32 [B]")
-            a.kv_len = kv_len.data_ptr()
+            lens = kv_len.data_ptr()
         if mask is not None:
             if mask.dtype not in (torch.bool, torch.uint8):
                 raise _capi.SfbError(_capi.SFB_ERR_DTYPE, "mask must be bool or uint8")
-            if tuple(mask.shape) != (c.batch, sk) or (sk > 1 and mask.stride(1) != 1):
+            if mask.shape != (B, sk) or (sk > 1 and mask.stride(1) != 1):
                 raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "mask must be [B, seq_k], row-contiguous")
-            a.key_mask, a.key_mask_stride_b = mask.data_ptr(), mask.stride(0)
-        with _on_device(dev):
-            _capi.check(self._lib.sfb_kv4_attention(ctypes.byref(a), _stream_handle(stream)), "kv4_attention")
+            keep, keep_sb = mask.data_ptr(), mask.stride(0)
+        h, s = o[1], o[2]
+        args = _capi.KV4_ATTN_ARGS.pack(
+            Q.data_ptr(), out.data_ptr(), st[0], st[h], st[s], so[0], so[h], so[s], lens, keep, keep_sb, sh[h], sh[s],
+            sk, _DTYPE_CODE[dt], 1 if is_causal else 0, int(num_splits), scale)
+        _call(self._lib.sfb_kv4_attention, "kv4_attention", dev, stream, c, args)
 
     # Linear layer with 4-bit weights and group scales (quant4.pack_w4)
     def w4a16_linear(self, x, w_q, w_scale, out, bias=None, residual=None, act: str = "none",
@@ -404,8 +397,7 @@ class B200Backend:
         c[n, k] · w_scale[n, k / group]: w_q uint8 [N, K / 2] packed codes,
         w_scale [N, K / group] fp16, bf16 or fp32 (group 32, 64 or 128 follows
         from its shape). x and bias bf16 or fp16; out x's dtype or fp32."""
-        dev = _one_device(x, "x", (w_q, "w_q"), (w_scale, "w_scale"), (out, "out"), (bias, "bias"),
-                          (residual, "residual"))
+        dev = _device_index("x", x, w_q, w_scale, out, bias, residual)
         if x.dtype not in _HALVES or w_q.dtype != torch.uint8 or w_scale.dtype not in _FLOATS:
             raise _capi.SfbError(_capi.SFB_ERR_DTYPE, "x bf16 or fp16, w_q uint8, w_scale float expected")
         if out.dtype != x.dtype and out.dtype != torch.float32:
@@ -427,13 +419,14 @@ class B200Backend:
         if act not in _ACTS:
             raise ValueError(f"unknown act {act!r}")
         # a single row's stride is never used: pass one that fits
-        ld = lambda t, n: t.stride(0) if M > 1 else n
-        with _on_device(dev):
-            _capi.check(self._lib.sfb_w4a16_linear(
-                x.data_ptr(), ld(x, (K + 7) // 8 * 8), _DTYPE_CODE[x.dtype], w_q.data_ptr(), w_scale.data_ptr(),
-                _DTYPE_CODE[w_scale.dtype], K // groups, _ptr(bias), _ptr(residual),
-                ld(residual, N) if residual is not None else 0, out.data_ptr(), ld(out, N), _DTYPE_CODE[out.dtype],
-                M, N, K, _ACTS[act], _stream_handle(stream)), "w4a16_linear")
+        ldx, ldr, ldy = (K + 7) // 8 * 8, N, N
+        if M > 1:
+            ldx, ldy = x.stride(0), out.stride(0)
+            if residual is not None:
+                ldr = residual.stride(0)
+        _call(self._lib.sfb_w4a16_linear, "w4a16_linear", dev, stream, x.data_ptr(), ldx, _DTYPE_CODE[x.dtype],
+              w_q.data_ptr(), w_scale.data_ptr(), _DTYPE_CODE[w_scale.dtype], K // groups, _ptr(bias),
+              _ptr(residual), ldr, out.data_ptr(), ldy, _DTYPE_CODE[out.dtype], M, N, K, _ACTS[act])
 
     # Graph hooks (backend.h:227-229; CUDABackend keeps one graph per stream,
     # cuda_backend.cu:592-608).

@@ -24,7 +24,7 @@ int kv4_append_launch(const sfb_kv4_cache* cache, const void* k, const int64_t* 
                       const int32_t* len, cudaStream_t s);
 int kv4_read_launch(const sfb_kv4_cache* cache, void* k, const int64_t* k_st, void* v, const int64_t* v_st,
                     int32_t dtype, int32_t slot0, int32_t seq, cudaStream_t s);
-int kv4_attention_launch(const sfb_kv4_attn_args& a, cudaStream_t s);
+int kv4_attention_launch(const sfb_kv4_cache* cache, const sfb_kv4_attn_args& a, cudaStream_t s);
 int w4a16_linear_launch(const void* x, int64_t ldx, int32_t x_dtype, const void* w, const void* w_scale,
                         int32_t scale_dtype, int32_t group, const void* bias, const void* residual, int64_t ldr,
                         void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t N, int32_t K, int32_t act,
@@ -184,9 +184,9 @@ int sfb_kv4_read(const sfb_kv4_cache* cache, void* k, const int64_t* k_stride, v
     return sfb::kv4_read_launch(cache, k, k_stride, v, v_stride, dtype, slot0, seq, static_cast<cudaStream_t>(stream));
 }
 
-int sfb_kv4_attention(const sfb_kv4_attn_args* a, void* stream) {
+int sfb_kv4_attention(const sfb_kv4_cache* cache, const sfb_kv4_attn_args* a, void* stream) {
     if (a == nullptr) return SFB_ERR_INVALID;
-    return sfb::kv4_attention_launch(*a, static_cast<cudaStream_t>(stream));
+    return sfb::kv4_attention_launch(cache, *a, static_cast<cudaStream_t>(stream));
 }
 
 int sfb_w4a16_linear(const void* x, int64_t ldx, int32_t x_dtype, const void* w, const void* w_scale,

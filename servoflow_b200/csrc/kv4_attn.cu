@@ -417,9 +417,9 @@ int pick_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
 
 }  // namespace kv4
 
-int kv4_attention_launch(const sfb_kv4_attn_args& a, cudaStream_t s) {
+int kv4_attention_launch(const sfb_kv4_cache* cache, const sfb_kv4_attn_args& a, cudaStream_t s) {
     Kv4AttnParams p{};
-    SFB_TRY(kv4_cache_check(a.cache, p.c));
+    SFB_TRY(kv4_cache_check(cache, p.c));
     if (a.dtype != SFB_F16 && a.dtype != SFB_BF16) return SFB_ERR_DTYPE;
     if (a.heads < 1 || a.heads % p.c.Hkv != 0 || a.seq_q < 0 || a.seq_k < 0 || a.seq_k > p.c.cap) return SFB_ERR_SHAPE;
     if (a.num_splits < 0 || a.num_splits > 16) return SFB_ERR_INVALID;

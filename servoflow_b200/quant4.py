@@ -87,26 +87,24 @@ class KV4Cache:
             out.append((unpack_codes(c).float().unflatten(-1, (-1, GROUP)) * s.float().unsqueeze(-1)).flatten(-2))
         return tuple(out)
 
-    def struct(self) -> "_capi.Kv4Cache":
-        """The C struct of this cache (sfb_kv4_cache); raises where the tensors do not fit it."""
+    def pack(self):
+        """(sfb_kv4_cache as bytes, batch, heads_kv, capacity, head_dim, device
+        index); raises where the tensors do not fit it."""
         kc, vc, ks, vs = self.k_codes, self.v_codes, self.k_scale, self.v_scale
-        st, ss = kc.stride(), ks.stride()
-        shape = kc.shape
-        if len(shape) != 4 or vc.shape != shape or ks.shape != vs.shape or ks.dim() != 4 \
-                or ks.shape[:3] != shape[:3] or ks.shape[3] * 16 != shape[3]:
+        shape, sshape, st, ss = kc.shape, ks.shape, kc.stride(), ks.stride()
+        if len(shape) != 4 or len(sshape) != 4 or vc.shape != shape or vs.shape != sshape \
+                or sshape[:3] != shape[:3] or sshape[3] * 16 != shape[3]:
             raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "inconsistent cache shapes")
-        if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or ks.dtype != torch.float16 \
-                or vs.dtype != torch.float16:
+        if kc.dtype is not torch.uint8 or vc.dtype is not torch.uint8 or ks.dtype is not torch.float16 \
+                or vs.dtype is not torch.float16:
             raise _capi.SfbError(_capi.SFB_ERR_DTYPE, "cache codes are uint8, scales fp16")
         if vc.stride() != st or vs.stride() != ss:
             raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "K and V of a cache share their strides")
-        if st[3] != 1 or ss[3] != 1 or (shape[2] > 1 and (st[2] != shape[3] or ss[2] != ks.shape[3])):
+        B, H, C, D2 = shape
+        if st[3] != 1 or ss[3] != 1 or (C > 1 and (st[2] != D2 or ss[2] != sshape[3])):
             raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "the last two dimensions of a cache are contiguous")
-        dev = kc.device
-        if not kc.is_cuda or vc.device != dev or ks.device != dev or vs.device != dev:
+        dev = kc.get_device()
+        if dev < 0 or vc.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev:
             raise ValueError("the cache's tensors must be on one CUDA device")
-        c = _capi.Kv4Cache()
-        c.k_codes, c.v_codes, c.k_scale, c.v_scale = kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr()
-        c.code_stride0, c.code_stride1, c.scale_stride0, c.scale_stride1 = st[0], st[1], ss[0], ss[1]
-        c.batch, c.heads_kv, c.capacity, c.head_dim = shape[0], shape[1], shape[2], 2 * shape[3]
-        return c
+        return (_capi.KV4_CACHE.pack(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), st[0], st[1],
+                                     ss[0], ss[1], B, H, C, 2 * D2), B, H, C, 2 * D2, dev)

@@ -1,6 +1,6 @@
 """CPU tests of the 4-bit formats (servoflow_b200.quant4) and of the refusals of
 the 4-bit and norm-rotation entry points that need no device."""
-import ctypes
+import re
 import struct
 
 import pytest
@@ -58,7 +58,7 @@ def test_cache_allocation_is_zero_and_rounded():
     k, v = c.dequantize()
     assert (k == 0).all() and (v == 0).all() and k.shape == (2, 3, 64, 64)
     with pytest.raises(ValueError):                    # the struct needs a CUDA cache
-        c.struct()
+        c.pack()
 
 
 def _offsets(struct_name, fields):
@@ -79,55 +79,70 @@ def _offsets(struct_name, fields):
         return list(map(int, subprocess.run([exe], capture_output=True, text=True).stdout.split()))
 
 
-def test_struct_mirrors_have_the_c_layout():
-    for name, py, rename in (("sfb_kv4_cache", _capi.Kv4Cache,
-                              {"code_stride0": "code_stride[0]", "code_stride1": "code_stride[1]",
-                               "scale_stride0": "scale_stride[0]", "scale_stride1": "scale_stride[1]"}),
-                             ("sfb_kv4_attn_args", _capi.Kv4AttnArgs, {}),
-                             ("sfb_norm_rope_args", _capi.NormRopeArgs, {})):
-        fields = [f for f, _ in py._fields_]
-        want = [getattr(py, f).offset for f in fields] + [ctypes.sizeof(py)]
-        assert _offsets(name, [rename.get(f, f) for f in fields]) == want, name
+CACHE = ("k_codes", "v_codes", "k_scale", "v_scale", "code_stride[0]", "code_stride[1]", "scale_stride[0]",
+         "scale_stride[1]", "batch", "heads_kv", "capacity", "head_dim")
+ATTN = ("q", "out", "q_stride[0]", "q_stride[1]", "q_stride[2]", "out_stride[0]", "out_stride[1]", "out_stride[2]",
+        "kv_len", "key_mask", "key_mask_stride_b", "heads", "seq_q", "seq_k", "dtype", "is_causal", "num_splits",
+        "scale")
+ROPE = ("q", "k", "q_out", "k_out") + tuple(
+    f"{n}[{i}]" for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride") for i in range(3)) + (
+    "q_weight", "k_weight", "cos_table", "sin_table", "positions", "pos_stride_b", "table_len", "batch", "seq", "heads",
+    "heads_kv", "head_dim", "rotary_dim", "interleaved", "norm", "dtype", "eps")
+
+
+def test_packed_structs_have_the_c_layout():
+    for name, fmt, fields in (("sfb_kv4_cache", _capi.KV4_CACHE, CACHE), ("sfb_kv4_attn_args", _capi.KV4_ATTN_ARGS, ATTN),
+                              ("sfb_norm_rope_args", _capi.NORM_ROPE_ARGS, ROPE)):
+        got = _offsets(name, fields)
+        codes = [ch for n, ch in re.findall(r"(\d*)([a-zA-Z])", fmt.format[:-2]) for _ in range(int(n or 1))]
+        assert len(codes) == len(fields) and got[-1] == fmt.size, name
+        want = [struct.calcsize("".join(codes[:i]) + "0" + codes[i]) for i in range(len(codes))]
+        assert got[:-1] == want, name
+
+
+def _packed(fmt, fields, values, over):
+    v = dict.fromkeys(fields, 0) | values | over
+    assert set(v) == set(fields), set(v) ^ set(fields)
+    return fmt.pack(*(v[f] for f in fields))
 
 
 def _cache(**over):
-    c = _capi.Kv4Cache()
-    c.k_codes = c.v_codes = c.k_scale = c.v_scale = 0x1000
-    c.code_stride0, c.code_stride1, c.scale_stride0, c.scale_stride1 = 8192, 2048, 512, 128
-    c.batch, c.heads_kv, c.capacity, c.head_dim = 2, 4, 64, 64
-    for k, v in over.items():
-        setattr(c, k, v)
-    return c
+    return _packed(_capi.KV4_CACHE, CACHE, {
+        "k_codes": 0x1000, "v_codes": 0x1000, "k_scale": 0x1000, "v_scale": 0x1000, "code_stride[0]": 8192,
+        "code_stride[1]": 2048, "scale_stride[0]": 512, "scale_stride[1]": 128, "batch": 2, "heads_kv": 4,
+        "capacity": 64, "head_dim": 64}, over)
 
 
 BAD_CACHES = [
-    (dict(k_codes=None), _capi.SFB_ERR_INVALID), (dict(v_scale=None), _capi.SFB_ERR_INVALID),
+    (dict(k_codes=0), _capi.SFB_ERR_INVALID), (dict(v_scale=0), _capi.SFB_ERR_INVALID),
     (dict(head_dim=96), _capi.SFB_ERR_SHAPE), (dict(head_dim=0), _capi.SFB_ERR_SHAPE),
     (dict(heads_kv=0), _capi.SFB_ERR_SHAPE), (dict(capacity=-1), _capi.SFB_ERR_SHAPE),
     (dict(k_codes=0x1008), _capi.SFB_ERR_ALIGN), (dict(v_scale=0x1002), _capi.SFB_ERR_ALIGN),
-    (dict(code_stride1=2056), _capi.SFB_ERR_ALIGN), (dict(scale_stride0=514), _capi.SFB_ERR_ALIGN),
+    ({"code_stride[1]": 2056}, _capi.SFB_ERR_ALIGN), ({"scale_stride[0]": 514}, _capi.SFB_ERR_ALIGN),
 ]
+
+
+def _attn(**over):
+    strides = {f: 64 for f in ATTN if "_stride[" in f}
+    return _packed(_capi.KV4_ATTN_ARGS, ATTN, strides | {
+        "q": 0x2000, "out": 0x3000, "heads": 8, "seq_q": 3, "seq_k": 64, "dtype": _capi.SFB_BF16}, over)
+
+
+I3 = _capi.I64X3.pack
 
 
 @pytest.mark.parametrize("over,status", BAD_CACHES)
 def test_bad_caches_are_refused_by_every_entry_point(over, status):
     lib = _capi.lib()
-    c = _cache(**over)
-    st = (ctypes.c_int64 * 3)(8192, 64, 256)
-    assert lib.sfb_kv4_append(ctypes.byref(c), 0x2000, st, 0x2000, st, _capi.SFB_BF16, 1, None, 0, None, None) == status
-    assert lib.sfb_kv4_read(ctypes.byref(c), 0x2000, st, 0x2000, st, _capi.SFB_F16, 0, 1, None) == status
-    a = _capi.Kv4AttnArgs()
-    a.cache, a.q, a.out = ctypes.addressof(c), 0x2000, 0x3000
-    a.heads, a.seq_q, a.seq_k, a.dtype = 4, 1, 32, _capi.SFB_BF16
-    assert lib.sfb_kv4_attention(ctypes.byref(a), None) == status
+    c, st = _cache(**over), I3(8192, 64, 256)
+    assert lib.sfb_kv4_append(c, 0x2000, st, 0x2000, st, _capi.SFB_BF16, 1, None, 0, None, None) == status
+    assert lib.sfb_kv4_read(c, 0x2000, st, 0x2000, st, _capi.SFB_F16, 0, 1, None) == status
+    assert lib.sfb_kv4_attention(c, _attn(seq_k=0), None) == status
 
 
 def test_append_and_read_refusals():
-    lib = _capi.lib()
-    c = ctypes.byref(_cache())
-    st = (ctypes.c_int64 * 3)(8192, 64, 256)
-    odd = (ctypes.c_int64 * 3)(8192, 64, 255)
-    E = _capi
+    lib, E = _capi.lib(), _capi
+    c, st, odd = _cache(), I3(8192, 64, 256), I3(8192, 64, 255)
     append = lambda cc, k, ks, v, vs, dt, seq, slot: lib.sfb_kv4_append(cc, k, ks, v, vs, dt, seq, None, slot, None, None)
     assert append(None, 0x2000, st, 0x2000, st, E.SFB_BF16, 1, 0) == E.SFB_ERR_INVALID
     assert append(c, None, st, 0x2000, st, E.SFB_BF16, 1, 0) == E.SFB_ERR_INVALID
@@ -152,23 +167,10 @@ def test_append_and_read_refusals():
 
 def test_attention_refusals():
     lib, E = _capi.lib(), _capi
-    c = _cache()
-
-    def call(**over):
-        a = _capi.Kv4AttnArgs()
-        a.cache, a.q, a.out = ctypes.addressof(c), 0x2000, 0x3000
-        a.heads, a.seq_q, a.seq_k, a.dtype = 8, 3, 64, E.SFB_BF16
-        a.q_stride[0] = a.q_stride[1] = a.q_stride[2] = a.out_stride[0] = a.out_stride[1] = a.out_stride[2] = 64
-        for k, v in over.items():
-            if k in ("q_stride", "out_stride"):
-                getattr(a, k)[2] = v
-            else:
-                setattr(a, k, v)
-        return lib.sfb_kv4_attention(ctypes.byref(a), None)
-
-    assert lib.sfb_kv4_attention(None, None) == E.SFB_ERR_INVALID
-    assert call(cache=None) == E.SFB_ERR_INVALID
-    assert call(q=None) == E.SFB_ERR_INVALID
+    call = lambda **over: lib.sfb_kv4_attention(_cache(), _attn(**over), None)
+    assert lib.sfb_kv4_attention(_cache(), None, None) == E.SFB_ERR_INVALID
+    assert lib.sfb_kv4_attention(None, _attn(), None) == E.SFB_ERR_INVALID
+    assert call(q=0) == E.SFB_ERR_INVALID
     assert call(dtype=E.SFB_F32) == E.SFB_ERR_DTYPE
     assert call(heads=6) == E.SFB_ERR_SHAPE
     assert call(heads=0) == E.SFB_ERR_SHAPE
@@ -178,34 +180,22 @@ def test_attention_refusals():
     assert call(seq_q=2 ** 31 - 1) == E.SFB_ERR_SHAPE
     assert call(num_splits=17) == E.SFB_ERR_INVALID
     assert call(q=0x2002) == E.SFB_ERR_ALIGN
-    assert call(q_stride=67) == E.SFB_ERR_ALIGN
-    assert call(out_stride=68) == E.SFB_ERR_ALIGN
+    assert call(**{"q_stride[2]": 67}) == E.SFB_ERR_ALIGN
+    assert call(**{"out_stride[2]": 68}) == E.SFB_ERR_ALIGN
     assert call(seq_q=0) == E.SFB_OK
 
 
 def test_norm_rope_refusals():
     lib, E = _capi.lib(), _capi
-
-    def call(**over):
-        a = _capi.NormRopeArgs()
-        a.q = a.q_out = a.k = a.k_out = 0x1000
-        for f in ("q_stride", "k_stride", "q_out_stride", "k_out_stride"):
-            for i in range(3):
-                getattr(a, f)[i] = 64
-        a.cos_table = a.sin_table = 0x4000
-        a.table_len, a.batch, a.seq, a.heads, a.heads_kv, a.head_dim = 10, 2, 3, 4, 2, 64
-        a.rotary_dim, a.norm, a.dtype, a.eps = 64, 1, E.SFB_BF16, 1e-6
-        for k, v in over.items():
-            if k.endswith("_stride"):
-                getattr(a, k)[1] = v
-            else:
-                setattr(a, k, v)
-        return lib.sfb_qk_norm_rope(ctypes.byref(a), None)
-
+    base = {f: 64 for f in ROPE if "stride[" in f} | {
+        "q": 0x1000, "k": 0x1000, "q_out": 0x1000, "k_out": 0x1000, "cos_table": 0x4000, "sin_table": 0x4000,
+        "table_len": 10, "batch": 2, "seq": 3, "heads": 4, "heads_kv": 2, "head_dim": 64, "rotary_dim": 64, "norm": 1,
+        "dtype": E.SFB_BF16, "eps": 1e-6}
+    call = lambda **over: lib.sfb_qk_norm_rope(_packed(_capi.NORM_ROPE_ARGS, ROPE, base, over), None)
     assert lib.sfb_qk_norm_rope(None, None) == E.SFB_ERR_INVALID
-    assert call(q=None) == E.SFB_ERR_INVALID                      # an output without its input
-    assert call(q=None, q_out=None, k=None, k_out=None) == E.SFB_ERR_INVALID
-    assert call(cos_table=None) == E.SFB_ERR_INVALID
+    assert call(q=0) == E.SFB_ERR_INVALID                         # an output without its input
+    assert call(q=0, q_out=0, k=0, k_out=0) == E.SFB_ERR_INVALID
+    assert call(cos_table=0) == E.SFB_ERR_INVALID
     assert call(dtype=E.SFB_I8) == E.SFB_ERR_DTYPE
     assert call(head_dim=60) == E.SFB_ERR_SHAPE
     assert call(head_dim=264, rotary_dim=0) == E.SFB_ERR_SHAPE
@@ -213,7 +203,7 @@ def test_norm_rope_refusals():
     assert call(rotary_dim=80) == E.SFB_ERR_SHAPE
     assert call(batch=-1) == E.SFB_ERR_SHAPE
     assert call(q=0x1004, q_out=0x1004) == E.SFB_ERR_ALIGN
-    assert call(k_out_stride=65) == E.SFB_ERR_ALIGN
+    assert call(**{"k_out_stride[1]": 65}) == E.SFB_ERR_ALIGN
     assert call(sin_table=0x4004) == E.SFB_ERR_ALIGN
     assert call(batch=0) == E.SFB_OK
     assert call(seq=0) == E.SFB_OK
