@@ -32,7 +32,7 @@ struct Kv4MoveParams {
     int64_t k_st[3], v_st[3];      // element strides: batch, head, seq
     int32_t seq, slot0;
     const int32_t *start, *len;
-    int64_t warps;
+    uint32_t warps;
     int32_t tgroups;               // token groups per session
 };
 
@@ -50,14 +50,14 @@ struct Where { int b, hh, tok; bool ok; };       // hh: K heads, then V heads
 template <int D>
 __device__ __forceinline__ Where where(const Kv4MoveParams& p) {
     constexpr int kLanes = D / 8, kTok = 32 / kLanes;
-    const int64_t w = (blockIdx.x * static_cast<int64_t>(kMoveThreads) + threadIdx.x) >> 5;
+    const uint32_t w = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5);
     Where r;
     r.ok = w < p.warps;
-    const int heads2 = 2 * p.c.Hkv;
-    const int64_t wt = w / heads2;
+    const uint32_t heads2 = 2 * p.c.Hkv;
+    const uint32_t wt = w / heads2;
     r.hh = static_cast<int>(w - wt * heads2);
-    r.b = static_cast<int>(wt / p.tgroups);
-    r.tok = static_cast<int>(wt - static_cast<int64_t>(r.b) * p.tgroups) * kTok + (threadIdx.x & 31) / kLanes;
+    r.b = static_cast<int>(wt / static_cast<uint32_t>(p.tgroups));
+    r.tok = static_cast<int>(wt - r.b * p.tgroups) * kTok + (threadIdx.x & 31) / kLanes;
     r.ok = r.ok && r.tok < p.seq;
     return r;
 }
@@ -96,10 +96,16 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(const Kv4MoveP
     const bool fits = mx < 0x7f800000u && s <= kMaxScale;
     uint32_t word = 0x88888888u;
     if (fits && s > 0.f) {
+        // x / s correctly rounded, as the division would give it, for eight x and
+        // one reciprocal: q = x·y and one residual step q + (x − q·s)·y with y =
+        // 1 / s correctly rounded (Markstein, 1990)
+        const float y = 1.f / s;
         word = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float c = fminf(7.f, fmaxf(-7.f, rintf(x[i] / s)));
+            float q = x[i] * y;
+            q = fmaf(fmaf(-q, s, x[i]), y, q);
+            const float c = fminf(7.f, fmaxf(-7.f, rintf(q)));
             word |= static_cast<uint32_t>(static_cast<int>(c) + 8) << nibble_shift(i);
         }
     }
@@ -141,10 +147,11 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(const Kv4MovePar
 template <typename T>
 int launch_move(Kv4MoveParams& p, bool append, cudaStream_t s) {
     const int tok = 32 / (p.c.D / 8);
-    p.tgroups = (p.seq + tok - 1) / tok;
-    p.warps = static_cast<int64_t>(p.c.B) * p.tgroups * 2 * p.c.Hkv;
-    const int64_t blocks = (p.warps * 32 + kMoveThreads - 1) / kMoveThreads;
-    if (blocks > 0x7fffffff) return SFB_ERR_SHAPE;
+    p.tgroups = static_cast<int32_t>((static_cast<int64_t>(p.seq) + tok - 1) / tok);
+    const int64_t warps = static_cast<int64_t>(p.c.B) * p.tgroups * 2 * p.c.Hkv;
+    if (static_cast<int64_t>(p.c.B) * p.tgroups > 0x7fffffff || warps > 0xffffff00ll) return SFB_ERR_SHAPE;
+    p.warps = static_cast<uint32_t>(warps);
+    const int64_t blocks = (warps * 32 + kMoveThreads - 1) / kMoveThreads;
     auto kern = p.c.D == 64 ? (append ? kv4_append_kernel<T, 64> : kv4_read_kernel<T, 64>)
                             : (append ? kv4_append_kernel<T, 128> : kv4_read_kernel<T, 128>);
     prefer_max_shared(kern);

@@ -44,11 +44,13 @@ struct Kv4AttnParams {
     int64_t mask_sb;
 };
 
+namespace kv4tc { template <typename T> int pick(Kv4AttnParams& p, int num_splits, cudaStream_t s); }
+
 namespace kv4 {
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                  "{%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -104,7 +106,7 @@ __host__ __device__ constexpr int attn_smem(int D, int NT, int W) {
 }
 
 template <typename T, int D, int NT, int W>
-__global__ void __launch_bounds__(W * 32) kv4_attn_kernel(const Kv4AttnParams p) {
+__global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const Kv4AttnParams p) {
     constexpr int kRows = NT * 8, kPad = attn_pad(D), kSteps = D / 16, kMT = D / 16;
     extern __shared__ __align__(16) uint8_t smem[];
     __half* sQ = reinterpret_cast<__half*>(smem);
@@ -153,33 +155,55 @@ __global__ void __launch_bounds__(W * 32) kv4_attn_kernel(const Kv4AttnParams p)
     }
     __syncthreads();
 
-    const uint8_t* kc = p.c.kc + b * p.c.code_sb + hk * p.c.code_sh + (D / 8) * t;
-    const uint8_t* vc = p.c.vc + b * p.c.code_sb + hk * p.c.code_sh + (D / 16) * g;
-    const uint16_t* ks = reinterpret_cast<const uint16_t*>(p.c.ks + b * p.c.sc_sb + hk * p.c.sc_sh) + (D / 4 * t) / kGroup;
-    const uint16_t* vs = reinterpret_cast<const uint16_t*>(p.c.vs + b * p.c.sc_sb + hk * p.c.sc_sh) + (D / 8 * g) / kGroup;
     const uint8_t* mask = p.key_mask != nullptr ? p.key_mask + b * p.mask_sb : nullptr;
     auto seen = [&](int key) { return key < kend && (mask == nullptr || mask[key] != 0); };
-    // a tile's codes and scales; a masked slot is not read and its scale is 0
+    // this lane's codes and scales of tile `warp` of the CTA, advanced by W tiles
+    const int64_t first = static_cast<int64_t>(t_begin + warp) * 16;
+    const uint8_t* kp = p.c.kc + b * p.c.code_sb + hk * p.c.code_sh + (first + g) * (D / 2) + (D / 8) * t;
+    const uint8_t* vp = p.c.vc + b * p.c.code_sb + hk * p.c.code_sh + (first + 2 * t) * (D / 2) + (D / 16) * g;
+    const uint16_t* ksp = reinterpret_cast<const uint16_t*>(p.c.ks + b * p.c.sc_sb + hk * p.c.sc_sh) +
+                          (first + g) * (D / kGroup) + (D / 4 * t) / kGroup;
+    const uint16_t* vsp = reinterpret_cast<const uint16_t*>(p.c.vs + b * p.c.sc_sb + hk * p.c.sc_sh) +
+                          (first + 2 * t) * (D / kGroup) + (D / 8 * g) / kGroup;
+    // In a tile with slots that are not seen, those are not read (nor trusted:
+    // they may hold anything) and their scale is 0.
     auto load = [&](Raw<D>& r, int tile) {
         const int k0 = tile * 16;
+        using KT = typename KWords<D>::T;
+        using VT = typename VWords<D>::T;
+        if (k0 + 16 <= kend && mask == nullptr) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int64_t key = k0 + g + 8 * i;
-            r.k[i] = {}; r.ks[i] = 0;
-            if (key < kend) {
-                r.k[i] = *reinterpret_cast<const typename KWords<D>::T*>(kc + key * (D / 2));
-                r.ks[i] = ks[key * (D / kGroup)];
+            for (int i = 0; i < 2; ++i) {
+                r.k[i] = *reinterpret_cast<const KT*>(kp + 8 * i * (D / 2));
+                r.ks[i] = ksp[8 * i * (D / kGroup)];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = (i & 1) + 8 * (i >> 1);
+                r.v[i] = *reinterpret_cast<const VT*>(vp + row * (D / 2));
+                r.vs[i] = vsp[row * (D / kGroup)];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                r.k[i] = {}; r.ks[i] = 0;
+                if (k0 + g + 8 * i < kend) {
+                    r.k[i] = *reinterpret_cast<const KT*>(kp + 8 * i * (D / 2));
+                    r.ks[i] = ksp[8 * i * (D / kGroup)];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = (i & 1) + 8 * (i >> 1);
+                r.v[i] = {}; r.vs[i] = 0;
+                if (seen(k0 + 2 * t + row)) {
+                    r.v[i] = *reinterpret_cast<const VT*>(vp + row * (D / 2));
+                    r.vs[i] = vsp[row * (D / kGroup)];
+                }
             }
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t key = k0 + 2 * t + (i & 1) + 8 * (i >> 1);
-            r.v[i] = {}; r.vs[i] = 0;
-            if (seen(static_cast<int>(key))) {
-                r.v[i] = *reinterpret_cast<const typename VWords<D>::T*>(vc + key * (D / 2));
-                r.vs[i] = vs[key * (D / kGroup)];
-            }
-        }
+        kp += 16 * W * (D / 2); vp += 16 * W * (D / 2);
+        ksp += 16 * W * (D / kGroup); vsp += 16 * W * (D / kGroup);
     };
 
     float o[kMT][NT][4], m[NT][2], l[NT][2];
@@ -190,12 +214,16 @@ __global__ void __launch_bounds__(W * 32) kv4_attn_kernel(const Kv4AttnParams p)
 #pragma unroll
         for (int i = 0; i < kMT; ++i) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
     }
-    Raw<D> nxt;
-    int tile = t_begin + warp;
-    if (tile < t_end) load(nxt, tile);
-    for (; tile < t_end; tile += W) {
-        const Raw<D> cur = nxt;
-        if (tile + W < t_end) load(nxt, tile + W);
+    constexpr bool kQReg = NT <= 2;                // Q fragments held in registers
+    uint4 qr[kQReg ? NT : 1][kQReg ? kSteps / 2 : 1];
+    if constexpr (kQReg) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int s = 0; s < kSteps / 2; ++s)
+                qr[j][s] = reinterpret_cast<const uint4*>(sQ + (j * 8 + g) * kPad + (D / 4) * t)[s];
+    }
+    auto step = [&](const Raw<D>& cur, int tile) {
         const int k0 = tile * 16;
         // K fragments: half2 2s and 2s+1 of a key's words are step s
         uint32_t ka[2][kSteps * 2];
@@ -226,20 +254,22 @@ __global__ void __launch_bounds__(W * 32) kv4_attn_kernel(const Kv4AttnParams p)
             }
         }
         const bool edge = k0 + 16 > kfull || mask != nullptr;
-        const bool vis0 = seen(k0 + g), vis1 = seen(k0 + g + 8);
+        bool vis0 = true, vis1 = true;
+        if (edge) { vis0 = seen(k0 + g); vis1 = seen(k0 + g + 8); }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-            const uint4* qf = reinterpret_cast<const uint4*>(sQ + (j * 8 + g) * kPad + (D / 4) * t);
+            float c[4] = {0.f, 0.f, 0.f, 0.f}, c2[4] = {0.f, 0.f, 0.f, 0.f};      // two chains
 #pragma unroll
             for (int s = 0; s < kSteps; s += 2) {
-                const uint4 q4 = qf[s / 2];
+                uint4 q4;
+                if constexpr (kQReg) q4 = qr[j][s / 2];
+                else q4 = reinterpret_cast<const uint4*>(sQ + (j * 8 + g) * kPad + (D / 4) * t)[s / 2];
                 mma16816(c, ka[0][2 * s], ka[1][2 * s], ka[0][2 * s + 1], ka[1][2 * s + 1], q4.x, q4.y);
-                mma16816(c, ka[0][2 * s + 2], ka[1][2 * s + 2], ka[0][2 * s + 3], ka[1][2 * s + 3], q4.z, q4.w);
+                mma16816(c2, ka[0][2 * s + 2], ka[1][2 * s + 2], ka[0][2 * s + 3], ka[1][2 * s + 3], q4.z, q4.w);
             }
             float x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = c[e] * p.sl2;
+            for (int e = 0; e < 4; ++e) x[e] = (c[e] + c2[e]) * p.sl2;
             if (edge) {
                 const int ra = min(r0 + j * 8 + 2 * t, p.R - 1), rb = min(r0 + j * 8 + 2 * t + 1, p.R - 1);
                 const int la = limit(ra), lb = limit(rb);
@@ -275,6 +305,23 @@ __global__ void __launch_bounds__(W * 32) kv4_attn_kernel(const Kv4AttnParams p)
             for (int i = 0; i < kMT; ++i)
                 mma16816(o[i][j], va[0][i / 4][0][i % 4], va[0][i / 4][1][i % 4], va[1][i / 4][0][i % 4],
                          va[1][i / 4][1][i % 4], b0, b1);
+        }
+    };
+    // tiles in flight per warp: two where the registers allow two CTAs per SM all the same
+    constexpr int kDepth = (NT == 1 && D == 64) ? 2 : 1;
+    Raw<D> ring[kDepth];
+    int tile = t_begin + warp;
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i)
+        if (tile + i * W < t_end) load(ring[i], tile + i * W);
+    for (; tile < t_end; tile += kDepth * W) {
+#pragma unroll
+        for (int i = 0; i < kDepth; ++i) {
+            const int cur_tile = tile + i * W;
+            if (i > 0 && cur_tile >= t_end) break;
+            const Raw<D> cur = ring[i];
+            if (cur_tile + kDepth * W < t_end) load(ring[i], cur_tile + kDepth * W);
+            step(cur, cur_tile);
         }
     }
 
@@ -407,8 +454,7 @@ int pick_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     if (p.c.D == 64) {
         if (p.R <= 8) return launch_attn<T, 64, 1, 8>(p, num_splits, s);
         if (p.R <= 16) return launch_attn<T, 64, 2, 8>(p, num_splits, s);
-        if (p.R <= 32) return launch_attn<T, 64, 4, 8>(p, num_splits, s);
-        return launch_attn<T, 64, 9, 8>(p, num_splits, s);
+        return kv4tc::pick<T>(p, num_splits, s);
     }
     if (p.R <= 8) return launch_attn<T, 128, 1, 8>(p, num_splits, s);
     if (p.R <= 16) return launch_attn<T, 128, 2, 8>(p, num_splits, s);

@@ -1,0 +1,636 @@
+// kv4_attn_tc.cu — attention over the 4-bit K/V cache on the 5th-generation
+// tensor cores, for more than 16 rows per K/V head (head_dim 64): an action
+// chunk's cross-attention, a prompt chunk, grouped heads. kv4_attn.cu holds the
+// form for few rows and the definitions (rows, masks, cache).
+//
+// As there, the keys are the MMA's M side. A tile is 128 keys by NQ rows:
+//   Sᵀ[128 keys, NQ] = K · Qᵀ      A = K (fp16) in TMEM, B = Q in shared memory
+//   Oᵀ[64, NQ]      += Vᵀ · Pᵀ     A = Vᵀ, B = Pᵀ, both in shared memory as the
+//                                  rows of V and P lie (MN-major)
+// 67 rows of an action chunk then cost 80 columns of exponentials (the bound: 16
+// a clock per SM, 640 clocks a tile) instead of the 128 or 96 lanes that the
+// rows cost as M. A thread of the softmax owns one key, so masks by length or
+// key are one predicate per thread; a thread of the dequantisation owns one
+// key's codes, 32 bytes of K and of V loaded two tiles ahead, and writes K to
+// its TMEM lane and V to its row of shared memory. K in TMEM rather than shared
+// memory: the shared-memory port, at 128 B/clk, is the second bound (dequantised
+// V 16 KB in and out, P 20 KB in and out, Q 10 KB out: 600 clocks a tile).
+//
+// 16 warps: two softmax groups of four (alternate tiles, own reference, own
+// accumulator, so that one computes while the other waits for its Sᵀ), four that
+// dequantise, one that issues the MMAs; registers are moved from the last two
+// warpgroups to the first two, which hold a row sum per column and thread.
+// The reference of a row (the m of exp2(x − m)) is shared by a group's 128
+// threads through shared memory and raised only when a logit passes it by more
+// than 8: one pass over Sᵀ finds that out (a comparison a value, with a vote of
+// the group), the second makes P.
+//
+// TMEM columns: Sᵀ at 96·g, Oᵀ at 192 + 96·g, K at 384 + 32·stage. With M = 64
+// the accumulator's row d is in lane 32·(d / 16) + d % 16.
+// Every wait is bounded; an expired one records SFB_ERR_DEVICE_TIMEOUT.
+#include "common.cuh"
+#include "sm100_ptx.cuh"
+
+namespace sfb {
+namespace kv4tc {
+
+constexpr int kThreads = 512;
+constexpr int kStages = 4;                        // dequantised K / V tiles
+constexpr int kKeys = 128;
+constexpr int kVBytes = kKeys * 128;              // fp16 V tile
+constexpr int kPBlock = kKeys * 128;              // 64 columns of P
+constexpr int kMaxQ = 96;
+constexpr int kTmemS = 0, kTmemO = 192, kTmemK = 384;
+constexpr int kOffQ = 0;                                      // [96 rows] × 128 B
+constexpr int kOffV = kOffQ + kMaxQ * 128;
+constexpr int kOffP = kOffV + kStages * kVBytes;              // [2 groups][2 blocks]
+constexpr int kOffCol = kOffP + 2 * 2 * kPBlock;              // per column, see Cols
+constexpr int kColBytes = kMaxQ * 4 * (2 * 5 + 1 + 8);
+constexpr int kOffBar = kOffCol + kColBytes;
+constexpr int kNumBars = 2 * kStages + 2 * 3 + 1;
+constexpr int kOffTmem = kOffBar + 8 * kNumBars;
+constexpr int kSmemBytes = kOffTmem + 16 + 1024;              // + alignment slack
+static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
+static_assert(kOffV % 1024 == 0 && kOffP % 1024 == 0 && kOffCol % 16 == 0 && kOffBar % 8 == 0, "alignment");
+// the partial result of a CTA, over P once every MMA is done: [NQ][64] O, [NQ] m, l
+static_assert(kMaxQ * 64 * 4 + 2 * kMaxQ * 4 <= 4 * kPBlock, "partial fits over P");
+
+__host__ __device__ constexpr int bar_ready(int s) { return s; }              // K, V of a stage written
+__host__ __device__ constexpr int bar_free(int s) { return kStages + s; }     // both MMAs of a stage done
+__host__ __device__ constexpr int bar_s(int g) { return 2 * kStages + g; }    // Sᵀ of the group's tile
+__host__ __device__ constexpr int bar_p(int g) { return 2 * kStages + 2 + g; }
+__host__ __device__ constexpr int bar_o(int g) { return 2 * kStages + 4 + g; } // the group's P·V done
+constexpr int kBarDrain = 2 * kStages + 6;
+constexpr uint64_t kWaitNs = 1000000000ull, kDrainNs = 100000000ull;
+
+struct Cols {                                     // shared memory, kMaxQ values each
+    float* negm;      // −m, 0 where no key was seen yet
+    float* thr;       // raw logit beyond which m is raised
+    float* m;
+    float* alpha;
+    int* cmax;        // ordered-integer maximum of the raw logits of a tile
+};
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+          "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+        : "r"(taddr));
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+// Barrier `id` of 128 threads with the OR of a predicate.
+__device__ __forceinline__ bool bar_or(uint32_t id, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+        "barrier.red.or.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r) : "r"(x ? 1u : 0u), "r"(id) : "memory");
+    return r != 0;
+}
+// fp32 ordering as signed integers (a positive NaN is above infinity).
+__device__ __forceinline__ int ordered(float x) {
+    const int i = __float_as_int(x);
+    return i ^ ((i >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+
+template <typename T, int NQ>
+__global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnParams p) {
+    using namespace ptx;
+    constexpr int D = 64;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + kOffTmem);
+    float* colbase = reinterpret_cast<float*>(smem + kOffCol);
+    auto cols = [&](int grp) {
+        float* c = colbase + grp * 5 * kMaxQ;
+        return Cols{c, c + kMaxQ, c + 2 * kMaxQ, c + 3 * kMaxQ, reinterpret_cast<int*>(c + 4 * kMaxQ)};
+    };
+    int* lim = reinterpret_cast<int*>(colbase + 10 * kMaxQ);       // slots below lim[c] are visible to row c
+    float* lsum = colbase + 11 * kMaxQ;                            // [8 warps][kMaxQ]
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = blockIdx.x, hk = blockIdx.y / p.rtiles, rt = blockIdx.y - hk * p.rtiles, b = blockIdx.z;
+    // rows in equal tiles of at most NQ
+    const int r0 = static_cast<int>(static_cast<int64_t>(p.R) * rt / p.rtiles);
+    const int rows = static_cast<int>(static_cast<int64_t>(p.R) * (rt + 1) / p.rtiles) - r0;
+
+    if (tid == 384) {
+        for (int s = 0; s < kStages; ++s) { mbar_init(&bars[bar_ready(s)], 4); mbar_init(&bars[bar_free(s)], 1); }
+        for (int g = 0; g < 2; ++g) {
+            mbar_init(&bars[bar_s(g)], 1);
+            mbar_init(&bars[bar_p(g)], 4);
+            mbar_init(&bars[bar_o(g)], 1);
+        }
+        mbar_init(&bars[kBarDrain], 1);
+        fence_mbarrier_init();
+    }
+    if (warp == 0) { tmem_alloc(tmem_holder, 512); tmem_relinquish(); }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_holder;
+    pdl_trigger();                                 // TMEM is held: the next kernel may start
+    pdl_wait();
+
+    int n = p.Sk;
+    if (p.kv_len != nullptr) n = min(n, max(0, p.kv_len[b]));
+    auto limit = [&](int r) { return p.causal ? min(n, max(0, n - p.Sq + r / p.g + 1)) : n; };
+    const int kend = limit(r0 + rows - 1), kfull = limit(r0);
+    const int tiles = (kend + kKeys - 1) / kKeys;
+    const int per = tiles / p.splits, rem = tiles - per * p.splits;
+    const int t_begin = split * per + min(split, rem), ntl = per + (split < rem ? 1 : 0);
+    const uint8_t* mask = p.key_mask != nullptr ? p.key_mask + b * p.mask_sb : nullptr;
+
+    // ── Q (fp16, 128-byte-swizzled rows; zeros past the last row), columns ──
+    bool bad = false;
+    for (int i = tid; i < NQ * 8; i += kThreads) {
+        const int r = i >> 3, c = i & 7;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (r < rows) {
+            const int rr = r0 + r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
+            u = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_st[0] + h * p.q_st[1] +
+                                                qi * p.q_st[2] + c * 8);
+            uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                    const float lo = __uint_as_float(w[e] << 16), hi = __uint_as_float(w[e] & 0xffff0000u);
+                    bad |= (fabsf(lo) > 65504.f && !isinf(lo)) | (fabsf(hi) > 65504.f && !isinf(hi));
+                    w[e] = kv4::h2u(__floats2half2_rn(lo, hi));
+                }
+                if (p.sl2 < 0.f) w[e] ^= 0x80008000u;      // the kernel's scale is |scale|
+            }
+        }
+        *reinterpret_cast<uint4*>(smem + kOffQ + r * 128 + ((c ^ (r & 7)) << 4)) = u;
+    }
+    if (tid < kMaxQ) {
+        lim[tid] = tid < rows ? limit(r0 + tid) : kend;
+        for (int g = 0; g < 2; ++g) {
+            const Cols c = cols(g);
+            c.negm[tid] = 0.f; c.thr[tid] = -INFINITY; c.m[tid] = -INFINITY;
+            c.cmax[tid] = static_cast<int>(0x80000000u);
+        }
+    }
+    fence_proxy_async_smem();
+    __syncthreads();
+
+    bool ok = true;
+    auto wait = [&](int bar, uint32_t parity) {
+        if (!mbar_wait(&bars[bar], parity, ok ? kWaitNs : 0ull)) ok = false;
+    };
+    float* pO = reinterpret_cast<float*>(smem + kOffP);            // [NQ][64]
+    float* pM = pO + kMaxQ * D;
+    float* pL = pM + kMaxQ;
+
+    if (warp >= 8 && warp < 12) {
+        // ── dequantisation: thread = key ────────────────────────────────────
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        const int key_in = (warp - 8) * 32 + lane;
+        const uint32_t lane_off = static_cast<uint32_t>((warp - 8) * 32) << 16;
+        const int64_t first = static_cast<int64_t>(t_begin) * kKeys + key_in;
+        const uint8_t* kp = p.c.kc + b * p.c.code_sb + hk * p.c.code_sh + first * (D / 2);
+        const uint8_t* vp = p.c.vc + b * p.c.code_sb + hk * p.c.code_sh + first * (D / 2);
+        const __half2* ksp = reinterpret_cast<const __half2*>(p.c.ks + b * p.c.sc_sb + hk * p.c.sc_sh) + first;
+        const __half2* vsp = reinterpret_cast<const __half2*>(p.c.vs + b * p.c.sc_sb + hk * p.c.sc_sh) + first;
+        struct RawRow { uint4 k0, k1, v0, v1; __half2 ks, vs; };
+        // a slot that is not seen is not read; its codes stand for 0 · 0
+        auto load = [&](RawRow& r, int j) {
+            const int key = (t_begin + j) * kKeys + key_in;
+            r.k0 = r.k1 = r.v0 = r.v1 = make_uint4(0, 0, 0, 0);
+            r.ks = r.vs = __float2half2_rn(0.f);
+            if (key < kend && (mask == nullptr || mask[key] != 0)) {
+                const int64_t o = static_cast<int64_t>(j) * kKeys;
+                const uint4* k4 = reinterpret_cast<const uint4*>(kp + o * (D / 2));
+                const uint4* v4 = reinterpret_cast<const uint4*>(vp + o * (D / 2));
+                r.k0 = k4[0]; r.k1 = k4[1]; r.v0 = v4[0]; r.v1 = v4[1];
+                r.ks = ksp[o]; r.vs = vsp[o];
+            }
+        };
+        RawRow ring[2];
+        if (ntl > 0) load(ring[0], 0);
+        if (ntl > 1) load(ring[1], 1);
+        for (int j0 = 0; j0 < ntl; j0 += 2) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int j = j0 + e;
+                if (j >= ntl) break;
+                const RawRow r = ring[e];
+                if (j + 2 < ntl) load(ring[e], j + 2);
+                const int s = j % kStages;
+                if (j >= kStages) { wait(bar_free(s), ((j / kStages) - 1) & 1); tc_fence_after_sync(); }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint4 w = h ? r.k1 : r.k0;
+                    const __half2 sc = h ? __high2half2(r.ks) : __low2half2(r.ks);
+                    const uint32_t* wp = reinterpret_cast<const uint32_t*>(&w);
+                    uint32_t kf[16];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t d4[4];
+                        kv4::dequant_word(wp[x], sc, d4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) kf[4 * x + i] = d4[i];
+                    }
+                    tmem_st16(tmem + kTmemK + 32 * s + 16 * h + lane_off, kf);
+                }
+                uint8_t* vrow = smem + kOffV + s * kVBytes + key_in * 128;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint4 w = h ? r.v1 : r.v0;
+                    const __half2 sc = h ? __high2half2(r.vs) : __low2half2(r.vs);
+                    const uint32_t* wp = reinterpret_cast<const uint32_t*>(&w);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t d4[4];
+                        kv4::dequant_word(wp[x], sc, d4);
+                        *reinterpret_cast<uint4*>(vrow + (((4 * h + x) ^ (key_in & 7)) << 4)) =
+                            make_uint4(d4[0], d4[1], d4[2], d4[3]);
+                    }
+                }
+                tmem_st_wait();
+                fence_proxy_async_smem();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars[bar_ready(s)]);
+            }
+        }
+    } else if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 12 && ntl > 0) {
+            // ── MMA issue ───────────────────────────────────────────────────
+            constexpr uint32_t idS = idesc_f16(128, NQ, 0, 0, 0);       // K(tmem) · Qᵀ, both K-major
+            constexpr uint32_t idO = idesc_f16(64, NQ, 0, 1, 1);        // Vᵀ · Pᵀ, both MN-major
+            const uint32_t aq = smem_u32(smem + kOffQ);
+            auto issue_s = [&](int j) {
+                const int s = j % kStages, g = j & 1;
+                tc_fence_after_sync();
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        mma_f16_ts(tmem + kTmemS + 96 * g, tmem + kTmemK + 32 * s + 8 * kk,
+                                   smem_desc_sw128(aq + kk * 32, 16, 1024), idS, kk > 0 ? 1u : 0u);
+                    mma_commit(&bars[bar_s(g)]);
+                }
+                __syncwarp();
+            };
+            auto issue_o = [&](int j) {
+                const int s = j % kStages, g = j & 1;
+                tc_fence_after_sync();
+                const uint32_t av = smem_u32(smem + kOffV + s * kVBytes), ap = smem_u32(smem + kOffP + g * 2 * kPBlock);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        mma_f16_ss(tmem + kTmemO + 96 * g, smem_desc_sw128(av + k * 2048, kVBytes, 1024),
+                                   smem_desc_sw128(ap + k * 2048, kPBlock, 1024), idO, (j >= 2 || k > 0) ? 1u : 0u);
+                    mma_commit(&bars[bar_free(s)]);
+                    mma_commit(&bars[bar_o(g)]);
+                }
+                __syncwarp();
+            };
+            // (decisions are the whole warp's: a lane alone never leaves the loop)
+            auto wait_all = [&](int bar, uint32_t parity) {
+                wait(bar, parity);
+                ok = __all_sync(0xffffffffu, ok) != 0;
+                return ok;
+            };
+            for (int j = 0; j < min(2, ntl) && ok; ++j)
+                if (wait_all(bar_ready(j), 0)) issue_s(j);
+            for (int j = 0; j < ntl && ok; ++j) {
+                if (!wait_all(bar_p(j & 1), (j / 2) & 1)) break;
+                // the group's next Sᵀ first, when its operands are there already
+                const int nx = j + 2, sn = nx % kStages;
+                const bool now = nx < ntl && __all_sync(0xffffffffu, mbar_test(&bars[bar_ready(sn)], (nx / kStages) & 1));
+                if (now) issue_s(nx);
+                issue_o(j);
+                if (nx < ntl && !now && wait_all(bar_ready(sn), (nx / kStages) & 1)) issue_s(nx);
+            }
+            // every MMA is done before TMEM and shared memory are let go
+            if (elect_one()) mma_commit(&bars[kBarDrain]);
+            __syncwarp();
+            if (!mbar_wait(&bars[kBarDrain], 0, kDrainNs)) ok = false;
+        }
+    } else {
+        // ── softmax group: thread = key of the group's tiles ────────────────
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        const int grp = warp >> 2, win = warp & 3, row = win * 32 + lane;
+        const uint32_t lane_off = static_cast<uint32_t>(win * 32) << 16;
+        const uint32_t tS = tmem + kTmemS + 96 * grp + lane_off, tO = tmem + kTmemO + 96 * grp + lane_off;
+        const Cols col = cols(grp);
+        const float sl2 = fabsf(p.sl2);
+        uint8_t* prow = smem + kOffP + grp * 2 * kPBlock + row * 128;
+        float2 l[NQ / 2];
+#pragma unroll
+        for (int i = 0; i < NQ / 2; ++i) l[i] = make_float2(0.f, 0.f);
+        int uses = 0;
+        for (int j = grp; j < ntl; j += 2, ++uses) {
+            const int k0 = (t_begin + j) * kKeys, key = k0 + row;
+            const bool edge = k0 + kKeys > kfull || mask != nullptr;
+            const bool vis = !edge || (key < kend && (mask == nullptr || mask[key] != 0));
+            wait(bar_s(grp), uses & 1);
+            tc_fence_after_sync();
+            // pass 1: does any visible logit pass its row's reference by more than 8?
+            bool over = false;
+            {
+                float a[2][16];
+                tmem_ld16(tS, a[0]);
+#pragma unroll
+                for (int ch = 0; ch < NQ / 16; ++ch) {
+                    tmem_ld_wait();
+                    if (ch + 1 < NQ / 16) tmem_ld16(tS + 16 * (ch + 1), a[(ch + 1) & 1]);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 t4 = *reinterpret_cast<const float4*>(col.thr + 16 * ch + i);
+                        const float (&x)[16] = a[ch & 1];
+                        if (!edge) {
+                            over |= (x[i] > t4.x) | (x[i + 1] > t4.y) | (x[i + 2] > t4.z) | (x[i + 3] > t4.w);
+                        } else if (vis) {
+                            const int4 l4 = *reinterpret_cast<const int4*>(lim + 16 * ch + i);
+                            over |= (x[i] > t4.x && key < l4.x) | (x[i + 1] > t4.y && key < l4.y) |
+                                    (x[i + 2] > t4.z && key < l4.z) | (x[i + 3] > t4.w && key < l4.w);
+                        }
+                    }
+                }
+            }
+            if (bar_or(1 + grp, over)) {
+                // raise the references: column maxima of the tile over the group
+#pragma unroll 1
+                for (int ch = 0; ch < NQ / 16; ++ch) {
+                    float a[16];
+                    tmem_ld16(tS + 16 * ch, a);
+                    tmem_ld_wait();
+                    int mine = static_cast<int>(0x80000000u);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const bool see = vis && (!edge || key < lim[16 * ch + i]);
+                        const int v = __reduce_max_sync(0xffffffffu, see ? ordered(a[i]) : static_cast<int>(0x80000000u));
+                        if (lane == i) mine = v;
+                    }
+                    if (lane < 16) atomicMax(col.cmax + 16 * ch + lane, mine);
+                }
+                named_bar_sync(1 + grp, 128);
+                if (row < NQ) {
+                    const int cm = col.cmax[row];
+                    const float x = cm == static_cast<int>(0x80000000u) ? -INFINITY : unordered(cm) * sl2;
+                    const float old = col.m[row];
+                    float alpha = 1.f;
+                    if (!(x <= old + 8.f) && x != -INFINITY) {      // a NaN raises it too
+                        alpha = old == -INFINITY ? 0.f : ex2(old - x);
+                        col.m[row] = x;
+                        col.negm[row] = -x;
+                        col.thr[row] = (x + 8.f) / sl2;
+                    }
+                    col.alpha[row] = alpha;
+                    col.cmax[row] = static_cast<int>(0x80000000u);
+                }
+                named_bar_sync(1 + grp, 128);
+#pragma unroll
+                for (int i = 0; i < NQ / 2; ++i) {
+                    const float2 al = *reinterpret_cast<const float2*>(col.alpha + 2 * i);
+                    l[i].x *= al.x; l[i].y *= al.y;
+                }
+                if (uses > 0) {
+                    wait(bar_o(grp), (uses - 1) & 1);               // the accumulator is at rest
+                    tc_fence_after_sync();
+#pragma unroll 1
+                    for (int ch = 0; ch < NQ / 16; ++ch) {
+                        float a[16];
+                        tmem_ld16(tO + 16 * ch, a);
+                        tmem_ld_wait();
+                        uint32_t u[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(a[i] * col.alpha[16 * ch + i]);
+                        tmem_st16(tO + 16 * ch, u);
+                    }
+                    tmem_st_wait();
+                }
+                named_bar_sync(1 + grp, 128);                       // alpha is read before it is written again
+            }
+            // pass 2: P = 2^(x·sl2 − m), row sums, fp16 P into this key's row
+            if (uses > 0) wait(bar_o(grp), (uses - 1) & 1);         // P's buffer is free
+            {
+                float a[2][16];
+                tmem_ld16(tS, a[0]);
+                const float2 s2 = make_float2(sl2, sl2);
+#pragma unroll
+                for (int ch = 0; ch < NQ / 16; ++ch) {
+                    tmem_ld_wait();
+                    if (ch + 1 < NQ / 16) tmem_ld16(tS + 16 * (ch + 1), a[(ch + 1) & 1]);
+                    const float (&x)[16] = a[ch & 1];
+                    uint32_t h[8];
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 m4 = *reinterpret_cast<const float4*>(col.negm + 16 * ch + i);
+                        float2 t0 = fma2(make_float2(x[i], x[i + 1]), s2, make_float2(m4.x, m4.y));
+                        float2 t1 = fma2(make_float2(x[i + 2], x[i + 3]), s2, make_float2(m4.z, m4.w));
+                        if (edge) {
+                            const int4 l4 = *reinterpret_cast<const int4*>(lim + 16 * ch + i);
+                            if (!vis || key >= l4.x) t0.x = -INFINITY;
+                            if (!vis || key >= l4.y) t0.y = -INFINITY;
+                            if (!vis || key >= l4.z) t1.x = -INFINITY;
+                            if (!vis || key >= l4.w) t1.y = -INFINITY;
+                        }
+                        const float2 p0 = make_float2(ex2(t0.x), ex2(t0.y)), p1 = make_float2(ex2(t1.x), ex2(t1.y));
+                        l[8 * ch + i / 2] = add2(l[8 * ch + i / 2], p0);
+                        l[8 * ch + i / 2 + 1] = add2(l[8 * ch + i / 2 + 1], p1);
+                        h[i / 2] = kv4::h2u(__floats2half2_rn(p0.x, p0.y));
+                        h[i / 2 + 1] = kv4::h2u(__floats2half2_rn(p1.x, p1.y));
+                    }
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int c = 2 * ch + q;                   // 16-byte chunk: 8 columns
+                        *reinterpret_cast<uint4*>(prow + (c >> 3) * kPBlock + (((c & 7) ^ (row & 7)) << 4)) =
+                            make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[bar_p(grp)]);
+        }
+        // row sums over the warp's keys: a butterfly that halves the columns each
+        // lane holds leaves column base + lane in lane
+#pragma unroll
+        for (int base = 0; base < NQ; base += 32) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const int c = base + i;
+                v[i] = c < NQ ? ((c & 1) ? l[c < NQ ? c / 2 : 0].y : l[c < NQ ? c / 2 : 0].x) : 0.f;
+            }
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) {
+                const bool up = (lane & w) != 0;
+#pragma unroll
+                for (int i = 0; i < w; ++i) {
+                    const float send = up ? v[i] : v[i + w], keep = up ? v[i + w] : v[i];
+                    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+                }
+            }
+            if (base + lane < NQ) lsum[warp * kMaxQ + base + lane] = v[0];
+        }
+        // every P·V of both groups is done: P's memory becomes the partial result
+        if (ntl >= 1) wait(bar_o(0), ((ntl + 1) / 2 - 1) & 1);
+        if (ntl >= 2) wait(bar_o(1), (ntl / 2 - 1) & 1);
+        tc_fence_after_sync();
+        named_bar_sync(3, 256);
+        const Cols ca = cols(0), cb = cols(1);
+        {
+            // group g joins the columns of its half; lanes 0..15 hold row d of Oᵀ
+            const int d = 16 * win + (lane & 15);
+            const uint32_t oa = tmem + kTmemO + lane_off, ob = oa + 96;
+            constexpr int kHalf = (NQ / 16 + 1) / 2;
+#pragma unroll 1
+            for (int ch = grp * kHalf; ch < min(NQ / 16, (grp + 1) * kHalf); ++ch) {
+                float a[16], c[16];
+                tmem_ld16(oa + 16 * ch, a);
+                tmem_ld16(ob + 16 * ch, c);
+                tmem_ld_wait();
+                if (lane < 16) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int q = 16 * ch + i;
+                        const float ma = ca.m[q], mb = cb.m[q], M = fmaxf(ma, mb);
+                        const float x = ma == -INFINITY ? 0.f : ex2(ma - M) * a[i];
+                        const float y = mb == -INFINITY ? 0.f : ex2(mb - M) * c[i];
+                        pO[q * D + d] = x + y;
+                    }
+                }
+            }
+            if (tid < NQ) {
+                const float ma = ca.m[tid], mb = cb.m[tid], M = fmaxf(ma, mb);
+                float la = 0.f, lb = 0.f;
+                for (int w = 0; w < 4; ++w) { la += lsum[w * kMaxQ + tid]; lb += lsum[(4 + w) * kMaxQ + tid]; }
+                pM[tid] = M;
+                pL[tid] = (ma == -INFINITY ? la : ex2(ma - M) * la) + (mb == -INFINITY ? lb : ex2(mb - M) * lb);
+            }
+        }
+        named_bar_sync(3, 256);
+        T* out = static_cast<T*>(p.out);
+        auto store = [&](int r, int d, float4 a, float inv) {
+            const int rr = r0 + r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
+            T* dst = out + b * p.o_st[0] + h * p.o_st[1] + qi * p.o_st[2] + d;
+            uint2 u;
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
+                u.x = *reinterpret_cast<const uint32_t*>(&x); u.y = *reinterpret_cast<const uint32_t*>(&y);
+            } else {
+                u.x = kv4::h2u(__floats2half2_rn(a.x * inv, a.y * inv)); u.y = kv4::h2u(__floats2half2_rn(a.z * inv, a.w * inv));
+            }
+            *reinterpret_cast<uint2*>(dst) = u;
+        };
+        if (p.splits == 1) {
+            if (ok)
+                for (int i = tid; i < rows * (D / 4); i += 256) {
+                    const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+                    const float L = pL[r];
+                    store(r, d, *reinterpret_cast<const float4*>(pO + r * D + d), L != 0.f ? 1.f / L : 0.f);
+                }
+        } else {
+            cluster_sync();                        // every CTA's partial is written
+            const uint32_t aO = smem_u32(pO), aM = smem_u32(pM), aL = smem_u32(pL);
+            const int mine = split < rows ? (rows - split + p.splits - 1) / p.splits : 0;
+            for (int i = tid; i < mine * (D / 4); i += 256) {
+                const int r = split + (i / (D / 4)) * p.splits, d = (i % (D / 4)) * 4;
+                float M = -INFINITY, L = 0.f;
+                for (int k = 0; k < p.splits; ++k) M = fmaxf(M, dsmem_ld_f32(dsmem_map(aM + 4 * r, k)));
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < p.splits; ++k) {
+                    const float mk = dsmem_ld_f32(dsmem_map(aM + 4 * r, k)), lk = dsmem_ld_f32(dsmem_map(aL + 4 * r, k));
+                    if (mk == -INFINITY) { L += lk; continue; }
+                    const float f = ex2(mk - M);
+                    L += f * lk;
+                    const float4 v = dsmem_ld_f32x4(dsmem_map(aO + 4 * (r * D + d), k));
+                    a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
+                }
+                if (ok) store(r, d, a, L != 0.f ? 1.f / L : 0.f);
+            }
+            cluster_sync();                        // nobody leaves while its partial may be read
+        }
+    }
+    if (warp >= 8 && p.splits > 1) { cluster_sync(); cluster_sync(); }
+    if (bad) atomicExch(&g_sfb_device_error, SFB_ERR_RANGE);
+    if (!ok) atomicExch(&g_sfb_device_error, SFB_ERR_DEVICE_TIMEOUT);
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <typename T, int NQ>
+int launch(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
+    const DeviceInfo& dev = device_info();
+    auto kern = kv4_attn_tc_kernel<T, NQ>;
+    static std::atomic<bool> done[64];             // kernel attributes, once per device (idempotent)
+    if (!done[dev.ordinal & 63].load(std::memory_order_acquire)) {
+        const cudaError_t e1 = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        const cudaError_t e2 = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e1 != cudaSuccess || e2 != cudaSuccess) {
+            record_cuda_error(e1 != cudaSuccess ? e1 : e2, "kv4 attention attributes");
+            return SFB_ERR_CUDA;
+        }
+        prefer_max_shared(kern);
+        done[dev.ordinal & 63].store(true, std::memory_order_release);
+    }
+    p.rtiles = (p.R + NQ - 1) / NQ;
+    const int64_t units = static_cast<int64_t>(p.c.B) * p.c.Hkv * p.rtiles;
+    const int tiles = (p.Sk + kKeys - 1) / kKeys;
+    int sp = num_splits;
+    if (sp == 0) {
+        // as many as keep every CTA in one wave (one per SM), two tiles each at least
+        sp = static_cast<int>(std::min<int64_t>(16, std::max<int64_t>(1, dev.num_sms / units)));
+        sp = std::min(sp, std::max(1, tiles / 2));
+    }
+    p.splits = std::min(sp, std::max(1, tiles));
+    if (static_cast<int64_t>(p.c.Hkv) * p.rtiles > 65535 || p.c.B > 65535) return SFB_ERR_SHAPE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.splits, p.c.Hkv * p.rtiles, p.c.B);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1 + pdl_attr(&attr[1], true);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+    if (e != cudaSuccess) { record_cuda_error(e, "kv4 attention (tcgen05) launch"); return SFB_ERR_LAUNCH; }
+    return SFB_OK;
+}
+
+// The column count that pads the equal row tiles least.
+template <typename T>
+int pick(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
+    auto cost = [&](int nq) { return static_cast<int64_t>((p.R + nq - 1) / nq) * (nq + 16); };
+    const int64_t c48 = cost(48), c80 = cost(80), c96 = cost(96);
+    if (c96 <= c80 && c96 <= c48) return launch<T, 96>(p, num_splits, s);
+    if (c80 <= c48) return launch<T, 80>(p, num_splits, s);
+    return launch<T, 48>(p, num_splits, s);
+}
+
+}  // namespace kv4tc
+}  // namespace sfb

@@ -30,7 +30,7 @@ struct NormRopeParams {
     int64_t pos_sb;
     int32_t table_len, S, H, Hkv, D, rot, norm;
     int32_t chunks;                                   // threads (of a head's lane) per token
-    int64_t tokens;
+    uint32_t tokens;
     float eps;
 };
 
@@ -80,13 +80,14 @@ __global__ void __launch_bounds__(kThreads)
 norm_rope_kernel(const NormRopeParams p) {
     pdl_trigger();
     pdl_wait();
-    const int64_t unit = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) / kLanes;
+    const uint32_t unit = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
     const int sub = threadIdx.x % kLanes;
-    const int64_t tok = unit / p.chunks;
+    const uint32_t tok = unit / static_cast<uint32_t>(p.chunks);
     const int chunk = static_cast<int>(unit - tok * p.chunks);
     const bool in_range = tok < p.tokens;             // whole warps take the shuffles below
-    const int64_t b = in_range ? tok / p.S : 0;
-    const int64_t s = in_range ? tok - b * p.S : 0;
+    const uint32_t bi = in_range ? tok / static_cast<uint32_t>(p.S) : 0;
+    const int64_t b = bi, s = in_range ? tok - bi * p.S : 0;
+    const int64_t pos = in_range && p.rot > 0 && p.pos != nullptr ? p.pos[b * p.pos_sb + s] : s;
     const int d0 = sub * 8;
     const bool act = in_range && d0 < p.D;
     const int heads = p.H + p.Hkv;
@@ -104,12 +105,19 @@ norm_rope_kernel(const NormRopeParams p) {
             load8(src + d0, x[j]);
         }
     }
+    // the weights of this lane's channels (q's and k's differ only by head)
+    float gq[8], gk[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) gq[i] = gk[i] = 1.f;
+    if (p.norm && act) {
+        if (p.q_w != nullptr && chunk < p.H) load8(static_cast<const T*>(p.q_w) + d0, gq);
+        if (p.k_w != nullptr && chunk + (kHeads - 1) * p.chunks >= p.H) load8(static_cast<const T*>(p.k_w) + d0, gk);
+    }
     // the token's angles: 8 (half-split) or 4 (interleaved) pairs for this lane
     float c[8], sn[8];
     bool bad = false;
     const bool rotates = p.rot > 0 && d0 < p.rot;
     if (p.rot > 0 && in_range) {
-        const int64_t pos = p.pos != nullptr ? p.pos[b * p.pos_sb + s] : s;
         bad = pos < 0 || pos >= p.table_len;
         if (rotates && !bad) {
             const int64_t base = pos * (p.rot / 2);
@@ -137,13 +145,9 @@ norm_rope_kernel(const NormRopeParams p) {
 #pragma unroll
             for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             const float inv = 1.f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
-            const void* w = h < p.H ? p.q_w : p.k_w;
-            float g[8];
+            const bool is_q = h < p.H;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] = 1.f;
-            if (have && w != nullptr) load8(static_cast<const T*>(w) + d0, g);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * g[i];
+            for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * (is_q ? gq[i] : gk[i]);
         }
         if (p.rot > 0) {
             if constexpr (kInter) {
@@ -178,16 +182,16 @@ norm_rope_kernel(const NormRopeParams p) {
 
 template <typename T, int kLanes, bool kInter>
 int launch(NormRopeParams& p, cudaStream_t s) {
-    // Four heads per thread once the grid fills the GPU without it (the shared
-    // angles then cost a quarter); one head per thread below that, where the
-    // launch is latency and every lane should hold one load.
+    // Four heads per thread once that still leaves half the GPU's threads busy:
+    // four loads in flight each, the angles' loads a quarter. One head per
+    // thread below that, where a call is latency.
     const int heads = p.H + p.Hkv;
-    const int64_t one = p.tokens * heads * kLanes;
-    const bool many = one >= static_cast<int64_t>(std::max(device_info().num_sms, 1)) * 2048 * 4;
+    const int64_t one = static_cast<int64_t>(p.tokens) * heads * kLanes;
+    const bool many = one >= static_cast<int64_t>(std::max(device_info().num_sms, 1)) * 1024 * 4;
     const int per = many ? 4 : 1;
     p.chunks = (heads + per - 1) / per;
-    const int64_t blocks = (p.tokens * p.chunks * kLanes + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffff) return SFB_ERR_SHAPE;
+    const int64_t units = static_cast<int64_t>(p.tokens) * p.chunks, blocks = (units * kLanes + kThreads - 1) / kThreads;
+    if (units > 0xffffff00ll || blocks > 0x7fffffff) return SFB_ERR_SHAPE;
     auto kern = many ? norm_rope_kernel<T, kLanes, 4, kInter> : norm_rope_kernel<T, kLanes, 1, kInter>;
     prefer_max_shared(kern);
     return launch_kernel(kern, static_cast<unsigned>(blocks), kThreads, 0, s, true, p);
@@ -235,7 +239,9 @@ int qk_norm_rope_launch(const sfb_norm_rope_args& a, cudaStream_t s) {
     p.table_len = a.table_len;
     p.S = a.seq; p.H = H; p.Hkv = Hkv; p.D = a.head_dim; p.rot = a.rotary_dim;
     p.norm = a.norm ? 1 : 0; p.eps = a.eps;
-    p.tokens = static_cast<int64_t>(a.batch) * a.seq;
+    const int64_t tokens = static_cast<int64_t>(a.batch) * a.seq;
+    if (tokens > 0x7fffffff) return SFB_ERR_SHAPE;
+    p.tokens = static_cast<uint32_t>(tokens);
     const bool inter = a.interleaved != 0;
     if (a.dtype == SFB_BF16) return nrope::pick<__nv_bfloat16>(p, inter, s);
     if (a.dtype == SFB_F16) return nrope::pick<__half>(p, inter, s);
