@@ -16,16 +16,16 @@
 // memory: the shared-memory port, at 128 B/clk, is the second bound (dequantised
 // V 16 KB in and out, P 20 KB in and out, Q 10 KB out: 600 clocks a tile).
 //
-// 16 warps: two softmax groups of four (alternate tiles, own reference, own
-// accumulator, so that one computes while the other waits for its Sᵀ), four that
-// dequantise, one that issues the MMAs; registers are moved from the last two
-// warpgroups to the first two, which hold a row sum per column and thread.
+// 13 warps: two softmax groups of four, each with half of the columns of every
+// tile (a thread then holds its key's logits and its row sums in registers, S is
+// read once and no column has two owners), four that dequantise, one that issues
+// the MMAs. Sᵀ is double-buffered and given back as soon as it is read, so the
+// next tile's is there when a group gets to it.
 // The reference of a row (the m of exp2(x − m)) is shared by a group's 128
 // threads through shared memory and raised only when a logit passes it by more
-// than 8: one pass over Sᵀ finds that out (a comparison a value, with a vote of
-// the group), the second makes P.
+// than 8: a comparison a value with one vote of the group finds that out.
 //
-// TMEM columns: Sᵀ at 96·g, Oᵀ at 192 + 96·g, K at 384 + 32·stage. With M = 64
+// TMEM columns: Sᵀ at 96·(tile & 1), Oᵀ at 192, K at 384 + 32·stage. With M = 64
 // the accumulator's row d is in lane 32·(d / 16) + d % 16.
 // Every wait is bounded; an expired one records SFB_ERR_DEVICE_TIMEOUT.
 #include "common.cuh"
@@ -34,7 +34,7 @@
 namespace sfb {
 namespace kv4tc {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 13 * 32;
 constexpr int kStages = 4;                        // dequantised K / V tiles
 constexpr int kKeys = 128;
 constexpr int kVBytes = kKeys * 128;              // fp16 V tile
@@ -43,42 +43,57 @@ constexpr int kMaxQ = 96;
 constexpr int kTmemS = 0, kTmemO = 192, kTmemK = 384;
 constexpr int kOffQ = 0;                                      // [96 rows] × 128 B
 constexpr int kOffV = kOffQ + kMaxQ * 128;
-constexpr int kOffP = kOffV + kStages * kVBytes;              // [2 groups][2 blocks]
-constexpr int kOffCol = kOffP + 2 * 2 * kPBlock;              // per column, see Cols
-constexpr int kColBytes = kMaxQ * 4 * (2 * 5 + 1 + 8);
+constexpr int kOffP = kOffV + kStages * kVBytes;              // [tile & 1][2 blocks]
+constexpr int kOffCol = kOffP + 2 * 2 * kPBlock;              // per column: −m, −threshold, m, alpha, limit
+constexpr int kColBytes = kMaxQ * 4 * (5 + 8);                // and [8 warps] maxima, then row sums
 constexpr int kOffBar = kOffCol + kColBytes;
-constexpr int kNumBars = 2 * kStages + 2 * 3 + 1;
+constexpr int kNumBars = 2 * kStages + 8 + 1;
 constexpr int kOffTmem = kOffBar + 8 * kNumBars;
 constexpr int kSmemBytes = kOffTmem + 16 + 1024;              // + alignment slack
 static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
-static_assert(kOffV % 1024 == 0 && kOffP % 1024 == 0 && kOffCol % 16 == 0 && kOffBar % 8 == 0, "alignment");
+static_assert(kMaxQ <= 128 && kOffV % 1024 == 0 && kOffP % 1024 == 0 && kOffCol % 16 == 0 && kOffBar % 8 == 0, "alignment");
 // the partial result of a CTA, over P once every MMA is done: [NQ][64] O, [NQ] m, l
 static_assert(kMaxQ * 64 * 4 + 2 * kMaxQ * 4 <= 4 * kPBlock, "partial fits over P");
 
-__host__ __device__ constexpr int bar_ready(int s) { return s; }              // K, V of a stage written
-__host__ __device__ constexpr int bar_free(int s) { return kStages + s; }     // both MMAs of a stage done
-__host__ __device__ constexpr int bar_s(int g) { return 2 * kStages + g; }    // Sᵀ of the group's tile
-__host__ __device__ constexpr int bar_p(int g) { return 2 * kStages + 2 + g; }
-__host__ __device__ constexpr int bar_o(int g) { return 2 * kStages + 4 + g; } // the group's P·V done
-constexpr int kBarDrain = 2 * kStages + 6;
+__host__ __device__ constexpr int bar_ready(int s) { return s; }                // K, V of a stage written
+__host__ __device__ constexpr int bar_free(int s) { return kStages + s; }       // both MMAs of a stage done
+__host__ __device__ constexpr int bar_s(int u) { return 2 * kStages + u; }      // Sᵀ of a tile, u = tile & 1
+__host__ __device__ constexpr int bar_read(int u) { return 2 * kStages + 2 + u; }   // Sᵀ read
+__host__ __device__ constexpr int bar_p(int u) { return 2 * kStages + 4 + u; }  // Pᵀ written
+__host__ __device__ constexpr int bar_o(int u) { return 2 * kStages + 6 + u; }  // P·V done
+constexpr int kBarDrain = 2 * kStages + 8;
 constexpr uint64_t kWaitNs = 1000000000ull, kDrainNs = 100000000ull;
 
-struct Cols {                                     // shared memory, kMaxQ values each
-    float* negm;      // −m, 0 where no key was seen yet
-    float* thr;       // raw logit beyond which m is raised
-    float* m;
-    float* alpha;
-    int* cmax;        // ordered-integer maximum of the raw logits of a tile
-};
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
+// 8 columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* r) {
     uint32_t* u = reinterpret_cast<uint32_t*>(r);
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
-          "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
-        : "r"(taddr));
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&u)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                 : "memory");
+}
+// Reduces 8 values per lane over the warp: lane 4·(i / 4) ... holds, in lanes with
+// lane % 8 == i, the result of value i.
+template <typename Op>
+__device__ __forceinline__ float reduce8(float (&v)[8], int lane, Op op) {
+#pragma unroll
+    for (int w = 16; w >= 8; w >>= 1)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = op(v[i], __shfl_xor_sync(0xffffffffu, v[i], w));
+#pragma unroll
+    for (int w = 4; w > 0; w >>= 1) {
+        const bool up = (lane & w) != 0;
+#pragma unroll
+        for (int i = 0; i < w; ++i) {
+            const float send = up ? v[i] : v[i + w], keep = up ? v[i + w] : v[i];
+            v[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, w));
+        }
+    }
+    return v[0];
 }
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -104,13 +119,6 @@ __device__ __forceinline__ bool bar_or(uint32_t id, bool x) {
         : "=r"(r) : "r"(x ? 1u : 0u), "r"(id) : "memory");
     return r != 0;
 }
-// fp32 ordering as signed integers (a positive NaN is above infinity).
-__device__ __forceinline__ int ordered(float x) {
-    const int i = __float_as_int(x);
-    return i ^ ((i >> 31) & 0x7fffffff);
-}
-__device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
-
 template <typename T, int NQ>
 __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnParams p) {
     using namespace ptx;
@@ -120,13 +128,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + kOffTmem);
-    float* colbase = reinterpret_cast<float*>(smem + kOffCol);
-    auto cols = [&](int grp) {
-        float* c = colbase + grp * 5 * kMaxQ;
-        return Cols{c, c + kMaxQ, c + 2 * kMaxQ, c + 3 * kMaxQ, reinterpret_cast<int*>(c + 4 * kMaxQ)};
-    };
-    int* lim = reinterpret_cast<int*>(colbase + 10 * kMaxQ);       // slots below lim[c] are visible to row c
-    float* lsum = colbase + 11 * kMaxQ;                            // [8 warps][kMaxQ]
+    float* negm = reinterpret_cast<float*>(smem + kOffCol);        // −m, 0 where no key was seen yet
+    float* nthr = negm + kMaxQ;                                    // −(raw logit beyond which m is raised)
+    float* colm = nthr + kMaxQ;
+    float* alpha = colm + kMaxQ;
+    int* lim = reinterpret_cast<int*>(alpha + kMaxQ);              // slots below lim[c] are visible to row c
+    float* wred = alpha + 2 * kMaxQ;                               // [8 warps][kMaxQ]
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, hk = blockIdx.y / p.rtiles, rt = blockIdx.y - hk * p.rtiles, b = blockIdx.z;
@@ -134,12 +141,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
     const int r0 = static_cast<int>(static_cast<int64_t>(p.R) * rt / p.rtiles);
     const int rows = static_cast<int>(static_cast<int64_t>(p.R) * (rt + 1) / p.rtiles) - r0;
 
-    if (tid == 384) {
+    if (tid == 12 * 32) {
         for (int s = 0; s < kStages; ++s) { mbar_init(&bars[bar_ready(s)], 4); mbar_init(&bars[bar_free(s)], 1); }
-        for (int g = 0; g < 2; ++g) {
-            mbar_init(&bars[bar_s(g)], 1);
-            mbar_init(&bars[bar_p(g)], 4);
-            mbar_init(&bars[bar_o(g)], 1);
+        for (int u = 0; u < 2; ++u) {
+            mbar_init(&bars[bar_s(u)], 1);
+            mbar_init(&bars[bar_read(u)], 8);
+            mbar_init(&bars[bar_p(u)], 8);
+            mbar_init(&bars[bar_o(u)], 1);
         }
         mbar_init(&bars[kBarDrain], 1);
         fence_mbarrier_init();
@@ -185,11 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
     }
     if (tid < kMaxQ) {
         lim[tid] = tid < rows ? limit(r0 + tid) : kend;
-        for (int g = 0; g < 2; ++g) {
-            const Cols c = cols(g);
-            c.negm[tid] = 0.f; c.thr[tid] = -INFINITY; c.m[tid] = -INFINITY;
-            c.cmax[tid] = static_cast<int>(0x80000000u);
-        }
+        negm[tid] = 0.f; nthr[tid] = INFINITY; colm[tid] = -INFINITY;
     }
     fence_proxy_async_smem();
     __syncthreads();
@@ -204,7 +208,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
 
     if (warp >= 8 && warp < 12) {
         // ── dequantisation: thread = key ────────────────────────────────────
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         const int key_in = (warp - 8) * 32 + lane;
         const uint32_t lane_off = static_cast<uint32_t>((warp - 8) * 32) << 16;
         const int64_t first = static_cast<int64_t>(t_begin) * kKeys + key_in;
@@ -275,35 +278,35 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             }
         }
     } else if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 12 && ntl > 0) {
             // ── MMA issue ───────────────────────────────────────────────────
             constexpr uint32_t idS = idesc_f16(128, NQ, 0, 0, 0);       // K(tmem) · Qᵀ, both K-major
             constexpr uint32_t idO = idesc_f16(64, NQ, 0, 1, 1);        // Vᵀ · Pᵀ, both MN-major
             const uint32_t aq = smem_u32(smem + kOffQ);
             auto issue_s = [&](int j) {
-                const int s = j % kStages, g = j & 1;
+                const int s = j % kStages;
                 tc_fence_after_sync();
                 if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        mma_f16_ts(tmem + kTmemS + 96 * g, tmem + kTmemK + 32 * s + 8 * kk,
+                        mma_f16_ts(tmem + kTmemS + 96 * (j & 1), tmem + kTmemK + 32 * s + 8 * kk,
                                    smem_desc_sw128(aq + kk * 32, 16, 1024), idS, kk > 0 ? 1u : 0u);
-                    mma_commit(&bars[bar_s(g)]);
+                    mma_commit(&bars[bar_s(j & 1)]);
                 }
                 __syncwarp();
             };
             auto issue_o = [&](int j) {
-                const int s = j % kStages, g = j & 1;
+                const int s = j % kStages;
                 tc_fence_after_sync();
-                const uint32_t av = smem_u32(smem + kOffV + s * kVBytes), ap = smem_u32(smem + kOffP + g * 2 * kPBlock);
+                const uint32_t av = smem_u32(smem + kOffV + s * kVBytes);
+                const uint32_t ap = smem_u32(smem + kOffP + (j & 1) * 2 * kPBlock);
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        mma_f16_ss(tmem + kTmemO + 96 * g, smem_desc_sw128(av + k * 2048, kVBytes, 1024),
-                                   smem_desc_sw128(ap + k * 2048, kPBlock, 1024), idO, (j >= 2 || k > 0) ? 1u : 0u);
+                        mma_f16_ss(tmem + kTmemO, smem_desc_sw128(av + k * 2048, kVBytes, 1024),
+                                   smem_desc_sw128(ap + k * 2048, kPBlock, 1024), idO, (j > 0 || k > 0) ? 1u : 0u);
                     mma_commit(&bars[bar_free(s)]);
-                    mma_commit(&bars[bar_o(g)]);
+                    mma_commit(&bars[bar_o(j & 1)]);
                 }
                 __syncwarp();
             };
@@ -316,13 +319,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             for (int j = 0; j < min(2, ntl) && ok; ++j)
                 if (wait_all(bar_ready(j), 0)) issue_s(j);
             for (int j = 0; j < ntl && ok; ++j) {
+                const int nx = j + 2;
+                if (nx < ntl) {
+                    if (!wait_all(bar_read(j & 1), (j / 2) & 1)) break;
+                    if (!wait_all(bar_ready(nx % kStages), (nx / kStages) & 1)) break;
+                    issue_s(nx);
+                }
                 if (!wait_all(bar_p(j & 1), (j / 2) & 1)) break;
-                // the group's next Sᵀ first, when its operands are there already
-                const int nx = j + 2, sn = nx % kStages;
-                const bool now = nx < ntl && __all_sync(0xffffffffu, mbar_test(&bars[bar_ready(sn)], (nx / kStages) & 1));
-                if (now) issue_s(nx);
                 issue_o(j);
-                if (nx < ntl && !now && wait_all(bar_ready(sn), (nx / kStages) & 1)) issue_s(nx);
             }
             // every MMA is done before TMEM and shared memory are let go
             if (elect_one()) mma_commit(&bars[kBarDrain]);
@@ -330,199 +334,146 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             if (!mbar_wait(&bars[kBarDrain], 0, kDrainNs)) ok = false;
         }
     } else {
-        // ── softmax group: thread = key of the group's tiles ────────────────
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-        const int grp = warp >> 2, win = warp & 3, row = win * 32 + lane;
+        // ── softmax: thread = key; group g has the columns [g·kC, (g+1)·kC) ──
+        constexpr int kC = NQ / 2;
+        const int grp = warp >> 2, win = warp & 3, row = win * 32 + lane, c0 = grp * kC;
         const uint32_t lane_off = static_cast<uint32_t>(win * 32) << 16;
-        const uint32_t tS = tmem + kTmemS + 96 * grp + lane_off, tO = tmem + kTmemO + 96 * grp + lane_off;
-        const Cols col = cols(grp);
+        const uint32_t tS = tmem + kTmemS + c0 + lane_off, tO = tmem + kTmemO + c0 + lane_off;
         const float sl2 = fabsf(p.sl2);
-        uint8_t* prow = smem + kOffP + grp * 2 * kPBlock + row * 128;
-        float2 l[NQ / 2];
+        const float2 s2 = make_float2(sl2, sl2);
+        uint8_t* const prow = smem + kOffP + row * 128;
+        float2 l[kC / 2];
 #pragma unroll
-        for (int i = 0; i < NQ / 2; ++i) l[i] = make_float2(0.f, 0.f);
-        int uses = 0;
-        for (int j = grp; j < ntl; j += 2, ++uses) {
-            const int k0 = (t_begin + j) * kKeys, key = k0 + row;
+        for (int i = 0; i < kC / 2; ++i) l[i] = make_float2(0.f, 0.f);
+        for (int j = 0; j < ntl; ++j) {
+            const int k0 = (t_begin + j) * kKeys, key = k0 + row, u = j & 1;
             const bool edge = k0 + kKeys > kfull || mask != nullptr;
-            const bool vis = !edge || (key < kend && (mask == nullptr || mask[key] != 0));
-            wait(bar_s(grp), uses & 1);
+            wait(bar_s(u), (j / 2) & 1);
             tc_fence_after_sync();
-            // pass 1: does any visible logit pass its row's reference by more than 8?
-            bool over = false;
-            {
-                float a[2][16];
-                tmem_ld16(tS, a[0]);
+            float x[kC];
 #pragma unroll
-                for (int ch = 0; ch < NQ / 16; ++ch) {
-                    tmem_ld_wait();
-                    if (ch + 1 < NQ / 16) tmem_ld16(tS + 16 * (ch + 1), a[(ch + 1) & 1]);
+            for (int i = 0; i < kC; i += 8) tmem_ld8(tS + 96 * u + i, x + i);
+            tmem_ld_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[bar_read(u)]);
+            if (edge) {                            // keys that some row does not see
+                const bool vis = key < kend && (mask == nullptr || mask[key] != 0);
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const float4 t4 = *reinterpret_cast<const float4*>(col.thr + 16 * ch + i);
-                        const float (&x)[16] = a[ch & 1];
-                        if (!edge) {
-                            over |= (x[i] > t4.x) | (x[i + 1] > t4.y) | (x[i + 2] > t4.z) | (x[i + 3] > t4.w);
-                        } else if (vis) {
-                            const int4 l4 = *reinterpret_cast<const int4*>(lim + 16 * ch + i);
-                            over |= (x[i] > t4.x && key < l4.x) | (x[i + 1] > t4.y && key < l4.y) |
-                                    (x[i + 2] > t4.z && key < l4.z) | (x[i + 3] > t4.w && key < l4.w);
-                        }
-                    }
-                }
+                for (int i = 0; i < kC; ++i) x[i] = vis && key < lim[c0 + i] ? x[i] : -INFINITY;
             }
-            if (bar_or(1 + grp, over)) {
-                // raise the references: column maxima of the tile over the group
-#pragma unroll 1
-                for (int ch = 0; ch < NQ / 16; ++ch) {
-                    float a[16];
-                    tmem_ld16(tS + 16 * ch, a);
-                    tmem_ld_wait();
-                    int mine = static_cast<int>(0x80000000u);
+            // does any logit pass its row's reference by more than 8?
+            float over[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const bool see = vis && (!edge || key < lim[16 * ch + i]);
-                        const int v = __reduce_max_sync(0xffffffffu, see ? ordered(a[i]) : static_cast<int>(0x80000000u));
-                        if (lane == i) mine = v;
-                    }
-                    if (lane < 16) atomicMax(col.cmax + 16 * ch + lane, mine);
+            for (int i = 0; i < kC; i += 4) {
+                const float4 t4 = *reinterpret_cast<const float4*>(nthr + c0 + i);
+                const float2 d0 = add2(make_float2(x[i], x[i + 1]), make_float2(t4.x, t4.y));
+                const float2 d1 = add2(make_float2(x[i + 2], x[i + 3]), make_float2(t4.z, t4.w));
+                over[(i / 4) & 3] = fmaxf(fmaxf(over[(i / 4) & 3], d0.x), d0.y);
+                over[(i / 4 + 2) & 3] = fmaxf(fmaxf(over[(i / 4 + 2) & 3], d1.x), d1.y);
+            }
+            if (bar_or(1 + grp, fmaxf(fmaxf(over[0], over[1]), fmaxf(over[2], over[3])) > 0.f)) {
+                // raise the references: column maxima of the tile, over a warp's keys, then its group's warps
+#pragma unroll
+                for (int i = 0; i < kC; i += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = x[i + e];
+                    const float mx = reduce8(v, lane, [](float a, float c) { return fmaxf(a, c); });
+                    if (lane < 8) wred[warp * kMaxQ + c0 + i + lane] = mx;
                 }
                 named_bar_sync(1 + grp, 128);
-                if (row < NQ) {
-                    const int cm = col.cmax[row];
-                    const float x = cm == static_cast<int>(0x80000000u) ? -INFINITY : unordered(cm) * sl2;
-                    const float old = col.m[row];
-                    float alpha = 1.f;
-                    if (!(x <= old + 8.f) && x != -INFINITY) {      // a NaN raises it too
-                        alpha = old == -INFINITY ? 0.f : ex2(old - x);
-                        col.m[row] = x;
-                        col.negm[row] = -x;
-                        col.thr[row] = (x + 8.f) / sl2;
+                if (row < kC) {
+                    const float* cm = wred + grp * 4 * kMaxQ + c0 + row;
+                    const float t = fmaxf(fmaxf(cm[0], cm[kMaxQ]), fmaxf(cm[2 * kMaxQ], cm[3 * kMaxQ])) * sl2;
+                    const float old = colm[c0 + row];
+                    float al = 1.f;
+                    if (t > old + 8.f) {
+                        al = old == -INFINITY ? 0.f : ex2(old - t);
+                        colm[c0 + row] = t;
+                        negm[c0 + row] = -t;
+                        nthr[c0 + row] = -(t + 8.f) / sl2;
                     }
-                    col.alpha[row] = alpha;
-                    col.cmax[row] = static_cast<int>(0x80000000u);
+                    alpha[c0 + row] = al;
                 }
                 named_bar_sync(1 + grp, 128);
 #pragma unroll
-                for (int i = 0; i < NQ / 2; ++i) {
-                    const float2 al = *reinterpret_cast<const float2*>(col.alpha + 2 * i);
+                for (int i = 0; i < kC / 2; ++i) {
+                    const float2 al = *reinterpret_cast<const float2*>(alpha + c0 + 2 * i);
                     l[i].x *= al.x; l[i].y *= al.y;
                 }
-                if (uses > 0) {
-                    wait(bar_o(grp), (uses - 1) & 1);               // the accumulator is at rest
+                if (j > 0) {
+                    wait(bar_o(u ^ 1), ((j - 1) / 2) & 1);          // the accumulator is at rest
                     tc_fence_after_sync();
 #pragma unroll 1
-                    for (int ch = 0; ch < NQ / 16; ++ch) {
-                        float a[16];
-                        tmem_ld16(tO + 16 * ch, a);
+                    for (int i = 0; i < kC; i += 8) {
+                        float a[8];
+                        tmem_ld8(tO + i, a);
                         tmem_ld_wait();
-                        uint32_t u[16];
+                        uint32_t w[8];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(a[i] * col.alpha[16 * ch + i]);
-                        tmem_st16(tO + 16 * ch, u);
+                        for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(a[e] * alpha[c0 + i + e]);
+                        tmem_st8(tO + i, w);
                     }
                     tmem_st_wait();
                 }
                 named_bar_sync(1 + grp, 128);                       // alpha is read before it is written again
             }
-            // pass 2: P = 2^(x·sl2 − m), row sums, fp16 P into this key's row
-            if (uses > 0) wait(bar_o(grp), (uses - 1) & 1);         // P's buffer is free
-            {
-                float a[2][16];
-                tmem_ld16(tS, a[0]);
-                const float2 s2 = make_float2(sl2, sl2);
+            // P = 2^(x·sl2 − m), row sums, fp16 P into this key's row
+            if (j > 1) wait(bar_o(u), ((j - 2) / 2) & 1);           // P's buffer is free
 #pragma unroll
-                for (int ch = 0; ch < NQ / 16; ++ch) {
-                    tmem_ld_wait();
-                    if (ch + 1 < NQ / 16) tmem_ld16(tS + 16 * (ch + 1), a[(ch + 1) & 1]);
-                    const float (&x)[16] = a[ch & 1];
-                    uint32_t h[8];
+            for (int i = 0; i < kC; i += 8) {
+                uint32_t h[4];
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const float4 m4 = *reinterpret_cast<const float4*>(col.negm + 16 * ch + i);
-                        float2 t0 = fma2(make_float2(x[i], x[i + 1]), s2, make_float2(m4.x, m4.y));
-                        float2 t1 = fma2(make_float2(x[i + 2], x[i + 3]), s2, make_float2(m4.z, m4.w));
-                        if (edge) {
-                            const int4 l4 = *reinterpret_cast<const int4*>(lim + 16 * ch + i);
-                            if (!vis || key >= l4.x) t0.x = -INFINITY;
-                            if (!vis || key >= l4.y) t0.y = -INFINITY;
-                            if (!vis || key >= l4.z) t1.x = -INFINITY;
-                            if (!vis || key >= l4.w) t1.y = -INFINITY;
-                        }
-                        const float2 p0 = make_float2(ex2(t0.x), ex2(t0.y)), p1 = make_float2(ex2(t1.x), ex2(t1.y));
-                        l[8 * ch + i / 2] = add2(l[8 * ch + i / 2], p0);
-                        l[8 * ch + i / 2 + 1] = add2(l[8 * ch + i / 2 + 1], p1);
-                        h[i / 2] = kv4::h2u(__floats2half2_rn(p0.x, p0.y));
-                        h[i / 2 + 1] = kv4::h2u(__floats2half2_rn(p1.x, p1.y));
-                    }
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int c = 2 * ch + q;                   // 16-byte chunk: 8 columns
-                        *reinterpret_cast<uint4*>(prow + (c >> 3) * kPBlock + (((c & 7) ^ (row & 7)) << 4)) =
-                            make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
-                    }
+                for (int e = 0; e < 8; e += 4) {
+                    const float4 m4 = *reinterpret_cast<const float4*>(negm + c0 + i + e);
+                    const float2 t0 = fma2(make_float2(x[i + e], x[i + e + 1]), s2, make_float2(m4.x, m4.y));
+                    const float2 t1 = fma2(make_float2(x[i + e + 2], x[i + e + 3]), s2, make_float2(m4.z, m4.w));
+                    const float2 p0 = make_float2(ex2(t0.x), ex2(t0.y)), p1 = make_float2(ex2(t1.x), ex2(t1.y));
+                    l[(i + e) / 2] = add2(l[(i + e) / 2], p0);
+                    l[(i + e) / 2 + 1] = add2(l[(i + e) / 2 + 1], p1);
+                    h[e / 2] = kv4::h2u(__floats2half2_rn(p0.x, p0.y));
+                    h[e / 2 + 1] = kv4::h2u(__floats2half2_rn(p1.x, p1.y));
                 }
+                const int c = (c0 + i) >> 3;                        // 16-byte chunk: 8 columns
+                *reinterpret_cast<uint4*>(prow + (2 * u + (c >> 3)) * kPBlock + (((c & 7) ^ (row & 7)) << 4)) =
+                    make_uint4(h[0], h[1], h[2], h[3]);
             }
             fence_proxy_async_smem();
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars[bar_p(grp)]);
+            if (lane == 0) mbar_arrive(&bars[bar_p(u)]);
         }
-        // row sums over the warp's keys: a butterfly that halves the columns each
-        // lane holds leaves column base + lane in lane
+        // row sums over the warp's keys
 #pragma unroll
-        for (int base = 0; base < NQ; base += 32) {
-            float v[32];
+        for (int i = 0; i < kC; i += 8) {
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const int c = base + i;
-                v[i] = c < NQ ? ((c & 1) ? l[c < NQ ? c / 2 : 0].y : l[c < NQ ? c / 2 : 0].x) : 0.f;
-            }
-#pragma unroll
-            for (int w = 16; w > 0; w >>= 1) {
-                const bool up = (lane & w) != 0;
-#pragma unroll
-                for (int i = 0; i < w; ++i) {
-                    const float send = up ? v[i] : v[i + w], keep = up ? v[i + w] : v[i];
-                    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
-                }
-            }
-            if (base + lane < NQ) lsum[warp * kMaxQ + base + lane] = v[0];
+            for (int e = 0; e < 8; ++e) v[e] = (e & 1) ? l[(i + e) / 2].y : l[(i + e) / 2].x;
+            const float t = reduce8(v, lane, [](float a, float c) { return a + c; });
+            if (lane < 8) wred[warp * kMaxQ + c0 + i + lane] = t;
         }
-        // every P·V of both groups is done: P's memory becomes the partial result
-        if (ntl >= 1) wait(bar_o(0), ((ntl + 1) / 2 - 1) & 1);
-        if (ntl >= 2) wait(bar_o(1), (ntl / 2 - 1) & 1);
+        // every P·V is done: P's memory becomes the partial result
+        if (ntl >= 1) wait(bar_o((ntl - 1) & 1), ((ntl - 1) / 2) & 1);
         tc_fence_after_sync();
         named_bar_sync(3, 256);
-        const Cols ca = cols(0), cb = cols(1);
         {
-            // group g joins the columns of its half; lanes 0..15 hold row d of Oᵀ
+            // lanes 0..15 hold row d of Oᵀ
             const int d = 16 * win + (lane & 15);
-            const uint32_t oa = tmem + kTmemO + lane_off, ob = oa + 96;
-            constexpr int kHalf = (NQ / 16 + 1) / 2;
 #pragma unroll 1
-            for (int ch = grp * kHalf; ch < min(NQ / 16, (grp + 1) * kHalf); ++ch) {
-                float a[16], c[16];
-                tmem_ld16(oa + 16 * ch, a);
-                tmem_ld16(ob + 16 * ch, c);
+            for (int i = 0; i < kC; i += 8) {
+                float a[8];
+                tmem_ld8(tO + i, a);
                 tmem_ld_wait();
                 if (lane < 16) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int q = 16 * ch + i;
-                        const float ma = ca.m[q], mb = cb.m[q], M = fmaxf(ma, mb);
-                        const float x = ma == -INFINITY ? 0.f : ex2(ma - M) * a[i];
-                        const float y = mb == -INFINITY ? 0.f : ex2(mb - M) * c[i];
-                        pO[q * D + d] = x + y;
-                    }
+                    for (int e = 0; e < 8; ++e) pO[(c0 + i + e) * D + d] = ntl > 0 ? a[e] : 0.f;
                 }
             }
-            if (tid < NQ) {
-                const float ma = ca.m[tid], mb = cb.m[tid], M = fmaxf(ma, mb);
-                float la = 0.f, lb = 0.f;
-                for (int w = 0; w < 4; ++w) { la += lsum[w * kMaxQ + tid]; lb += lsum[(4 + w) * kMaxQ + tid]; }
-                pM[tid] = M;
-                pL[tid] = (ma == -INFINITY ? la : ex2(ma - M) * la) + (mb == -INFINITY ? lb : ex2(mb - M) * lb);
+            if (row < kC) {
+                const float* ls = wred + grp * 4 * kMaxQ + c0 + row;
+                pM[c0 + row] = colm[c0 + row];
+                pL[c0 + row] = (ls[0] + ls[kMaxQ]) + (ls[2 * kMaxQ] + ls[3 * kMaxQ]);
             }
         }
         named_bar_sync(3, 256);
@@ -540,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             *reinterpret_cast<uint2*>(dst) = u;
         };
         if (p.splits == 1) {
+            // (with every logit of a row NaN its sum is, and so is the row)
             if (ok)
                 for (int i = tid; i < rows * (D / 4); i += 256) {
                     const int r = i / (D / 4), d = (i % (D / 4)) * 4;
