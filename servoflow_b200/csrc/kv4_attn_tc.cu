@@ -16,10 +16,10 @@
 // memory: the shared-memory port, at 128 B/clk, is the second bound (dequantised
 // V 16 KB in and out, P 20 KB in and out, Q 10 KB out: 600 clocks a tile).
 //
-// 13 warps: two softmax groups of four, each with half of the columns of every
-// tile (a thread then holds its key's logits and its row sums in registers, S is
-// read once and no column has two owners), four that dequantise, one that issues
-// the MMAs. Sᵀ is double-buffered and given back as soon as it is read, so the
+// 21 warps: four softmax groups of four, each with a quarter of the columns of
+// every tile (a thread then holds its key's logits and its row sums in registers,
+// S is read once and no column has two owners), four that dequantise, one that
+// issues the MMAs. Sᵀ is double-buffered and given back as soon as it is read, so the
 // next tile's is there when a group gets to it.
 // The reference of a row (the m of exp2(x − m)) is shared by a group's 128
 // threads through shared memory and raised only when a logit passes it by more
@@ -34,7 +34,9 @@
 namespace sfb {
 namespace kv4tc {
 
-constexpr int kThreads = 13 * 32;
+constexpr int kSoftWarps = 16, kSoftThreads = kSoftWarps * 32;   // 4 column groups of 4 warps
+constexpr int kDeqWarp0 = 16, kCtrlWarp = 20;
+constexpr int kThreads = 21 * 32;
 constexpr int kStages = 4;                        // dequantised K / V tiles
 constexpr int kKeys = 128;
 constexpr int kVBytes = kKeys * 128;              // fp16 V tile
@@ -45,7 +47,7 @@ constexpr int kOffQ = 0;                                      // [96 rows] × 12
 constexpr int kOffV = kOffQ + kMaxQ * 128;
 constexpr int kOffP = kOffV + kStages * kVBytes;              // [tile & 1][2 blocks]
 constexpr int kOffCol = kOffP + 2 * 2 * kPBlock;              // per column: −m, −threshold, m, alpha, limit
-constexpr int kColBytes = kMaxQ * 4 * (5 + 8);                // and [8 warps] maxima, then row sums
+constexpr int kColBytes = kMaxQ * 4 * (5 + 4);                // and [4 windows] maxima, then row sums
 constexpr int kOffBar = kOffCol + kColBytes;
 constexpr int kNumBars = 2 * kStages + 8 + 1;
 constexpr int kOffTmem = kOffBar + 8 * kNumBars;
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
     float* colm = nthr + kMaxQ;
     float* alpha = colm + kMaxQ;
     int* lim = reinterpret_cast<int*>(alpha + kMaxQ);              // slots below lim[c] are visible to row c
-    float* wred = alpha + 2 * kMaxQ;                               // [8 warps][kMaxQ]
+    float* wred = alpha + 2 * kMaxQ;                               // [4 windows][kMaxQ]
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, hk = blockIdx.y / p.rtiles, rt = blockIdx.y - hk * p.rtiles, b = blockIdx.z;
@@ -141,12 +143,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
     const int r0 = static_cast<int>(static_cast<int64_t>(p.R) * rt / p.rtiles);
     const int rows = static_cast<int>(static_cast<int64_t>(p.R) * (rt + 1) / p.rtiles) - r0;
 
-    if (tid == 12 * 32) {
+    if (tid == kCtrlWarp * 32) {
         for (int s = 0; s < kStages; ++s) { mbar_init(&bars[bar_ready(s)], 4); mbar_init(&bars[bar_free(s)], 1); }
         for (int u = 0; u < 2; ++u) {
             mbar_init(&bars[bar_s(u)], 1);
-            mbar_init(&bars[bar_read(u)], 8);
-            mbar_init(&bars[bar_p(u)], 8);
+            mbar_init(&bars[bar_read(u)], kSoftWarps);
+            mbar_init(&bars[bar_p(u)], kSoftWarps);
             mbar_init(&bars[bar_o(u)], 1);
         }
         mbar_init(&bars[kBarDrain], 1);
@@ -206,10 +208,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
     float* pM = pO + kMaxQ * D;
     float* pL = pM + kMaxQ;
 
-    if (warp >= 8 && warp < 12) {
+    if (warp >= kDeqWarp0 && warp < kCtrlWarp) {
         // ── dequantisation: thread = key ────────────────────────────────────
-        const int key_in = (warp - 8) * 32 + lane;
-        const uint32_t lane_off = static_cast<uint32_t>((warp - 8) * 32) << 16;
+        const int key_in = (warp - kDeqWarp0) * 32 + lane;
+        const uint32_t lane_off = static_cast<uint32_t>((warp - kDeqWarp0) * 32) << 16;
         const int64_t first = static_cast<int64_t>(t_begin) * kKeys + key_in;
         const uint8_t* kp = p.c.kc + b * p.c.code_sb + hk * p.c.code_sh + first * (D / 2);
         const uint8_t* vp = p.c.vc + b * p.c.code_sb + hk * p.c.code_sh + first * (D / 2);
@@ -237,8 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             for (int e = 0; e < 2; ++e) {
                 const int j = j0 + e;
                 if (j >= ntl) break;
-                const RawRow r = ring[e];
-                if (j + 2 < ntl) load(ring[e], j + 2);
+                const RawRow& r = ring[e];
                 const int s = j % kStages;
                 if (j >= kStages) { wait(bar_free(s), ((j / kStages) - 1) & 1); tc_fence_after_sync(); }
 #pragma unroll
@@ -275,10 +276,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars[bar_ready(s)]);
+                if (j + 2 < ntl) load(ring[e], j + 2);
             }
         }
-    } else if (warp >= 12) {
-        if (warp == 12 && ntl > 0) {
+    } else if (warp == kCtrlWarp) {
+        if (ntl > 0) {
             // ── MMA issue ───────────────────────────────────────────────────
             constexpr uint32_t idS = idesc_f16(128, NQ, 0, 0, 0);       // K(tmem) · Qᵀ, both K-major
             constexpr uint32_t idO = idesc_f16(64, NQ, 0, 1, 1);        // Vᵀ · Pᵀ, both MN-major
@@ -334,14 +336,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             if (!mbar_wait(&bars[kBarDrain], 0, kDrainNs)) ok = false;
         }
     } else {
-        // ── softmax: thread = key; group g has the columns [g·kC, (g+1)·kC) ──
-        constexpr int kC = NQ / 2;
-        const int grp = warp >> 2, win = warp & 3, row = win * 32 + lane, c0 = grp * kC;
+        // ── softmax: thread = key; group g has 8·nch columns from c0 ────────
+        constexpr int kCh = NQ / 8, kMaxCh = (kCh + 3) / 4, kC = kMaxCh * 8;
+        const int grp = warp >> 2, win = warp & 3, row = win * 32 + lane;
+        const int nch = kCh / 4 + (grp < kCh % 4 ? 1 : 0);             // kMaxCh or one less
+        const int c0 = 8 * (grp * (kCh / 4) + min(grp, kCh % 4));
         const uint32_t lane_off = static_cast<uint32_t>(win * 32) << 16;
         const uint32_t tS = tmem + kTmemS + c0 + lane_off, tO = tmem + kTmemO + c0 + lane_off;
         const float sl2 = fabsf(p.sl2);
         const float2 s2 = make_float2(sl2, sl2);
         uint8_t* const prow = smem + kOffP + row * 128;
+        auto has = [&](int i) { return i + 8 < kC || nch == kMaxCh; };   // is chunk i / 8 this group's?
         float2 l[kC / 2];
 #pragma unroll
         for (int i = 0; i < kC / 2; ++i) l[i] = make_float2(0.f, 0.f);
@@ -352,7 +357,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             tc_fence_after_sync();
             float x[kC];
 #pragma unroll
-            for (int i = 0; i < kC; i += 8) tmem_ld8(tS + 96 * u + i, x + i);
+            for (int i = 0; i < kC; i += 8)
+                if (has(i)) tmem_ld8(tS + 96 * u + i, x + i);
             tmem_ld_wait();
             tc_fence_before_sync();
             __syncwarp();
@@ -360,12 +366,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             if (edge) {                            // keys that some row does not see
                 const bool vis = key < kend && (mask == nullptr || mask[key] != 0);
 #pragma unroll
-                for (int i = 0; i < kC; ++i) x[i] = vis && key < lim[c0 + i] ? x[i] : -INFINITY;
+                for (int i = 0; i < kC; ++i)
+                    if (has(i)) x[i] = vis && key < lim[c0 + i] ? x[i] : -INFINITY;
             }
             // does any logit pass its row's reference by more than 8?
             float over[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int i = 0; i < kC; i += 4) {
+                if (!has(i)) continue;
                 const float4 t4 = *reinterpret_cast<const float4*>(nthr + c0 + i);
                 const float2 d0 = add2(make_float2(x[i], x[i + 1]), make_float2(t4.x, t4.y));
                 const float2 d1 = add2(make_float2(x[i + 2], x[i + 3]), make_float2(t4.z, t4.w));
@@ -376,15 +384,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
                 // raise the references: column maxima of the tile, over a warp's keys, then its group's warps
 #pragma unroll
                 for (int i = 0; i < kC; i += 8) {
+                    if (!has(i)) continue;
                     float v[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] = x[i + e];
                     const float mx = reduce8(v, lane, [](float a, float c) { return fmaxf(a, c); });
-                    if (lane < 8) wred[warp * kMaxQ + c0 + i + lane] = mx;
+                    if (lane < 8) wred[win * kMaxQ + c0 + i + lane] = mx;
                 }
                 named_bar_sync(1 + grp, 128);
-                if (row < kC) {
-                    const float* cm = wred + grp * 4 * kMaxQ + c0 + row;
+                if (row < 8 * nch) {
+                    const float* cm = wred + c0 + row;
                     const float t = fmaxf(fmaxf(cm[0], cm[kMaxQ]), fmaxf(cm[2 * kMaxQ], cm[3 * kMaxQ])) * sl2;
                     const float old = colm[c0 + row];
                     float al = 1.f;
@@ -399,6 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
                 named_bar_sync(1 + grp, 128);
 #pragma unroll
                 for (int i = 0; i < kC / 2; ++i) {
+                    if (!has(2 * i)) continue;
                     const float2 al = *reinterpret_cast<const float2*>(alpha + c0 + 2 * i);
                     l[i].x *= al.x; l[i].y *= al.y;
                 }
@@ -406,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
                     wait(bar_o(u ^ 1), ((j - 1) / 2) & 1);          // the accumulator is at rest
                     tc_fence_after_sync();
 #pragma unroll 1
-                    for (int i = 0; i < kC; i += 8) {
+                    for (int i = 0; i < 8 * nch; i += 8) {
                         float a[8];
                         tmem_ld8(tO + i, a);
                         tmem_ld_wait();
@@ -423,6 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             if (j > 1) wait(bar_o(u), ((j - 2) / 2) & 1);           // P's buffer is free
 #pragma unroll
             for (int i = 0; i < kC; i += 8) {
+                if (!has(i)) continue;
                 uint32_t h[4];
 #pragma unroll
                 for (int e = 0; e < 8; e += 4) {
@@ -447,21 +458,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
         // row sums over the warp's keys
 #pragma unroll
         for (int i = 0; i < kC; i += 8) {
+            if (!has(i)) continue;
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = (e & 1) ? l[(i + e) / 2].y : l[(i + e) / 2].x;
             const float t = reduce8(v, lane, [](float a, float c) { return a + c; });
-            if (lane < 8) wred[warp * kMaxQ + c0 + i + lane] = t;
+            if (lane < 8) wred[win * kMaxQ + c0 + i + lane] = t;
         }
         // every P·V is done: P's memory becomes the partial result
         if (ntl >= 1) wait(bar_o((ntl - 1) & 1), ((ntl - 1) / 2) & 1);
         tc_fence_after_sync();
-        named_bar_sync(3, 256);
+        named_bar_sync(5, kSoftThreads);
         {
             // lanes 0..15 hold row d of Oᵀ
             const int d = 16 * win + (lane & 15);
 #pragma unroll 1
-            for (int i = 0; i < kC; i += 8) {
+            for (int i = 0; i < 8 * nch; i += 8) {
                 float a[8];
                 tmem_ld8(tO + i, a);
                 tmem_ld_wait();
@@ -470,13 +482,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
                     for (int e = 0; e < 8; ++e) pO[(c0 + i + e) * D + d] = ntl > 0 ? a[e] : 0.f;
                 }
             }
-            if (row < kC) {
-                const float* ls = wred + grp * 4 * kMaxQ + c0 + row;
+            if (row < 8 * nch) {
+                const float* ls = wred + c0 + row;
                 pM[c0 + row] = colm[c0 + row];
                 pL[c0 + row] = (ls[0] + ls[kMaxQ]) + (ls[2 * kMaxQ] + ls[3 * kMaxQ]);
             }
         }
-        named_bar_sync(3, 256);
+        named_bar_sync(5, kSoftThreads);
         T* out = static_cast<T*>(p.out);
         auto store = [&](int r, int d, float4 a, float inv) {
             const int rr = r0 + r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
@@ -493,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
         if (p.splits == 1) {
             // (with every logit of a row NaN its sum is, and so is the row)
             if (ok)
-                for (int i = tid; i < rows * (D / 4); i += 256) {
+                for (int i = tid; i < rows * (D / 4); i += kSoftThreads) {
                     const int r = i / (D / 4), d = (i % (D / 4)) * 4;
                     const float L = pL[r];
                     store(r, d, *reinterpret_cast<const float4*>(pO + r * D + d), L != 0.f ? 1.f / L : 0.f);
@@ -502,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             cluster_sync();                        // every CTA's partial is written
             const uint32_t aO = smem_u32(pO), aM = smem_u32(pM), aL = smem_u32(pL);
             const int mine = split < rows ? (rows - split + p.splits - 1) / p.splits : 0;
-            for (int i = tid; i < mine * (D / 4); i += 256) {
+            for (int i = tid; i < mine * (D / 4); i += kSoftThreads) {
                 const int r = split + (i / (D / 4)) * p.splits, d = (i % (D / 4)) * 4;
                 float M = -INFINITY, L = 0.f;
                 for (int k = 0; k < p.splits; ++k) M = fmaxf(M, dsmem_ld_f32(dsmem_map(aM + 4 * r, k)));
@@ -520,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             cluster_sync();                        // nobody leaves while its partial may be read
         }
     }
-    if (warp >= 8 && p.splits > 1) { cluster_sync(); cluster_sync(); }
+    if (warp >= kSoftWarps && p.splits > 1) { cluster_sync(); cluster_sync(); }
     if (bad) atomicExch(&g_sfb_device_error, SFB_ERR_RANGE);
     if (!ok) atomicExch(&g_sfb_device_error, SFB_ERR_DEVICE_TIMEOUT);
     tc_fence_before_sync();
