@@ -126,8 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
     using namespace ptx;
     constexpr int D = 64;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>(
-        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // (stays a shared-memory address)
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + kOffTmem);
     float* negm = reinterpret_cast<float*>(smem + kOffCol);        // −m, 0 where no key was seen yet
@@ -137,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
     int* lim = reinterpret_cast<int*>(alpha + kMaxQ);              // slots below lim[c] are visible to row c
     float* wred = alpha + 2 * kMaxQ;                               // [4 windows][kMaxQ]
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int split = blockIdx.x, hk = blockIdx.y / p.rtiles, rt = blockIdx.y - hk * p.rtiles, b = blockIdx.z;
     // rows in equal tiles of at most NQ
     const int r0 = static_cast<int>(static_cast<int64_t>(p.R) * rt / p.rtiles);
@@ -202,7 +201,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
 
     bool ok = true;
     auto wait = [&](int bar, uint32_t parity) {
-        if (!mbar_wait(&bars[bar], parity, ok ? kWaitNs : 0ull)) ok = false;
+        if (mbar_try_wait(smem_u32(&bars[bar]), parity)) return;
+        if (!ok || !mbar_wait(&bars[bar], parity, kWaitNs)) ok = false;
     };
     float* pO = reinterpret_cast<float*>(smem + kOffP);            // [NQ][64]
     float* pM = pO + kMaxQ * D;
@@ -241,7 +241,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
                 if (j >= ntl) break;
                 const RawRow& r = ring[e];
                 const int s = j % kStages;
-                if (j >= kStages) { wait(bar_free(s), ((j / kStages) - 1) & 1); tc_fence_after_sync(); }
+                if (j >= kStages) {
+                    // (stages ahead of the MMAs: this wait is the long one, and not urgent)
+                    if (!ok || !mbar_wait_sleep(&bars[bar_free(s)], ((j / kStages) - 1) & 1, 200, kWaitNs)) ok = false;
+                    tc_fence_after_sync();
+                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint4 w = h ? r.k1 : r.k0;
@@ -345,7 +349,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
         const uint32_t tS = tmem + kTmemS + c0 + lane_off, tO = tmem + kTmemO + c0 + lane_off;
         const float sl2 = fabsf(p.sl2);
         const float2 s2 = make_float2(sl2, sl2);
-        uint8_t* const prow = smem + kOffP + row * 128;
+        uint32_t poff[kMaxCh];                     // this key's 16-byte chunks (8 columns) in P's buffer
+#pragma unroll
+        for (int i = 0; i < kMaxCh; ++i) {
+            const int c = (c0 >> 3) + i;
+            poff[i] = kOffP + (c >> 3) * kPBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+        }
         auto has = [&](int i) { return i + 8 < kC || nch == kMaxCh; };   // is chunk i / 8 this group's?
         float2 l[kC / 2];
 #pragma unroll
@@ -446,9 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
                     h[e / 2] = kv4::h2u(__floats2half2_rn(p0.x, p0.y));
                     h[e / 2 + 1] = kv4::h2u(__floats2half2_rn(p1.x, p1.y));
                 }
-                const int c = (c0 + i) >> 3;                        // 16-byte chunk: 8 columns
-                *reinterpret_cast<uint4*>(prow + (2 * u + (c >> 3)) * kPBlock + (((c & 7) ^ (row & 7)) << 4)) =
-                    make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4*>(smem + poff[i / 8] + u * 2 * kPBlock) = make_uint4(h[0], h[1], h[2], h[3]);
             }
             fence_proxy_async_smem();
             tc_fence_before_sync();

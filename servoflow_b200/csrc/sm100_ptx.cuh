@@ -103,6 +103,20 @@ __device__ __forceinline__ bool mbar_wait_spin(uint64_t* bar, uint32_t parity,
     }
 }
 
+// Same contract as mbar_wait for waits that may be late by some hundred
+// nanoseconds: sleeps between the tries, so that the warp takes few issue slots.
+__device__ __forceinline__ bool mbar_wait_sleep(uint64_t* bar, uint32_t parity, uint32_t sleep_ns,
+                                                uint64_t timeout_ns = 1000000000ull) {
+    const uint32_t a = smem_u32(bar);
+    if (mbar_try_wait(a, parity)) return true;
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t it = 0;; ++it) {
+        __nanosleep(sleep_ns);
+        if (mbar_try_wait(a, parity)) return true;
+        if ((it & 63u) == 63u && global_timer_ns() - t0 > timeout_ns) return false;
+    }
+}
+
 // ── TMA (tensor tile loads, this CTA only) ───────────────────────────────────
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
