@@ -16,11 +16,11 @@
 // memory: the shared-memory port, at 128 B/clk, is the second bound (dequantised
 // V 16 KB in and out, P 20 KB in and out, Q 10 KB out: 600 clocks a tile).
 //
-// 21 warps: four softmax groups of four, each with a quarter of the columns of
-// every tile (a thread then holds its key's logits and its row sums in registers,
-// S is read once and no column has two owners), four that dequantise, one that
-// issues the MMAs. Sᵀ is double-buffered and given back as soon as it is read, so the
-// next tile's is there when a group gets to it.
+// Warps: a softmax group of four for every 16 columns (a thread then holds its
+// key's logits and row sums in registers, S is read once and no column has two
+// owners), four that dequantise, one that issues the MMAs. Sᵀ and Pᵀ are double-
+// buffered; Sᵀ of tile j + 2 is issued behind P·V of tile j, so that one barrier
+// tells a group both that its logits are there and that its P buffer is free.
 // The reference of a row (the m of exp2(x − m)) is shared by a group's 128
 // threads through shared memory and raised only when a logit passes it by more
 // than 8: a comparison a value with one vote of the group finds that out.
@@ -34,9 +34,9 @@
 namespace sfb {
 namespace kv4tc {
 
-constexpr int kSoftWarps = 16, kSoftThreads = kSoftWarps * 32;   // 4 column groups of 4 warps
-constexpr int kDeqWarp0 = 16, kCtrlWarp = 20;
-constexpr int kThreads = 21 * 32;
+constexpr int kC = 16;                            // columns of a softmax group
+__host__ __device__ constexpr int soft_warps(int nq) { return nq / kC * 4; }
+__host__ __device__ constexpr int threads(int nq) { return (soft_warps(nq) + 5) * 32; }   // + 4 dequantising, 1 issuing
 constexpr int kStages = 4;                        // dequantised K / V tiles
 constexpr int kKeys = 128;
 constexpr int kVBytes = kKeys * 128;              // fp16 V tile
@@ -46,10 +46,10 @@ constexpr int kTmemS = 0, kTmemO = 192, kTmemK = 384;
 constexpr int kOffQ = 0;                                      // [96 rows] × 128 B
 constexpr int kOffV = kOffQ + kMaxQ * 128;
 constexpr int kOffP = kOffV + kStages * kVBytes;              // [tile & 1][2 blocks]
-constexpr int kOffCol = kOffP + 2 * 2 * kPBlock;              // per column: −m, −threshold, m, alpha, limit
-constexpr int kColBytes = kMaxQ * 4 * (5 + 4);                // and [4 windows] maxima, then row sums
+constexpr int kOffCol = kOffP + 2 * 2 * kPBlock;              // per column: −m, m, alpha, limit
+constexpr int kColBytes = kMaxQ * 4 * (4 + 4);                // and [4 windows] maxima, then row sums
 constexpr int kOffBar = kOffCol + kColBytes;
-constexpr int kNumBars = 2 * kStages + 8 + 1;
+constexpr int kNumBars = 2 * kStages + 2 + 2 + 1 + 1;
 constexpr int kOffTmem = kOffBar + 8 * kNumBars;
 constexpr int kSmemBytes = kOffTmem + 16 + 1024;              // + alignment slack
 static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
@@ -60,34 +60,30 @@ static_assert(kMaxQ * 64 * 4 + 2 * kMaxQ * 4 <= 4 * kPBlock, "partial fits over 
 __host__ __device__ constexpr int bar_ready(int s) { return s; }                // K, V of a stage written
 __host__ __device__ constexpr int bar_free(int s) { return kStages + s; }       // both MMAs of a stage done
 __host__ __device__ constexpr int bar_s(int u) { return 2 * kStages + u; }      // Sᵀ of a tile, u = tile & 1
-__host__ __device__ constexpr int bar_read(int u) { return 2 * kStages + 2 + u; }   // Sᵀ read
-__host__ __device__ constexpr int bar_p(int u) { return 2 * kStages + 4 + u; }  // Pᵀ written
-__host__ __device__ constexpr int bar_o(int u) { return 2 * kStages + 6 + u; }  // P·V done
-constexpr int kBarDrain = 2 * kStages + 8;
+__host__ __device__ constexpr int bar_p(int u) { return 2 * kStages + 2 + u; }  // Sᵀ read and Pᵀ written
+constexpr int kBarO = 2 * kStages + 4;                                          // P·V of a tile done
+constexpr int kBarDrain = kBarO + 1;
+constexpr float kUnseen = 1e30f;
 constexpr uint64_t kWaitNs = 1000000000ull, kDrainNs = 100000000ull;
 
-// 8 columns of this thread's lane.
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* r) {
+// 16 columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
     uint32_t* u = reinterpret_cast<uint32_t*>(r);
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
-                 : "r"(taddr));
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+          "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+        : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&u)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
-                 : "memory");
-}
-// Reduces 8 values per lane over the warp: lane 4·(i / 4) ... holds, in lanes with
-// lane % 8 == i, the result of value i.
+// Reduces 16 values per lane over the warp; the result of value i is left in the
+// lanes with lane % 16 == i.
 template <typename Op>
-__device__ __forceinline__ float reduce8(float (&v)[8], int lane, Op op) {
+__device__ __forceinline__ float reduce16(float (&v)[16], int lane, Op op) {
 #pragma unroll
-    for (int w = 16; w >= 8; w >>= 1)
+    for (int i = 0; i < 16; ++i) v[i] = op(v[i], __shfl_xor_sync(0xffffffffu, v[i], 16));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = op(v[i], __shfl_xor_sync(0xffffffffu, v[i], w));
-#pragma unroll
-    for (int w = 4; w > 0; w >>= 1) {
+    for (int w = 8; w > 0; w >>= 1) {
         const bool up = (lane & w) != 0;
 #pragma unroll
         for (int i = 0; i < w; ++i) {
@@ -122,16 +118,16 @@ __device__ __forceinline__ bool bar_or(uint32_t id, bool x) {
     return r != 0;
 }
 template <typename T, int NQ>
-__global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnParams p) {
+__global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4AttnParams p) {
     using namespace ptx;
-    constexpr int D = 64;
+    constexpr int D = 64, kSoftWarps = soft_warps(NQ), kSoftThreads = kSoftWarps * 32, kThreads = threads(NQ);
+    constexpr int kDeqWarp0 = kSoftWarps, kCtrlWarp = kSoftWarps + 4;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // (stays a shared-memory address)
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + kOffTmem);
-    float* negm = reinterpret_cast<float*>(smem + kOffCol);        // −m, 0 where no key was seen yet
-    float* nthr = negm + kMaxQ;                                    // −(raw logit beyond which m is raised)
-    float* colm = nthr + kMaxQ;
+    float* negm = reinterpret_cast<float*>(smem + kOffCol);        // −m, kUnseen where no key was seen yet
+    float* colm = negm + kMaxQ;
     float* alpha = colm + kMaxQ;
     int* lim = reinterpret_cast<int*>(alpha + kMaxQ);              // slots below lim[c] are visible to row c
     float* wred = alpha + 2 * kMaxQ;                               // [4 windows][kMaxQ]
@@ -146,10 +142,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
         for (int s = 0; s < kStages; ++s) { mbar_init(&bars[bar_ready(s)], 4); mbar_init(&bars[bar_free(s)], 1); }
         for (int u = 0; u < 2; ++u) {
             mbar_init(&bars[bar_s(u)], 1);
-            mbar_init(&bars[bar_read(u)], kSoftWarps);
             mbar_init(&bars[bar_p(u)], kSoftWarps);
-            mbar_init(&bars[bar_o(u)], 1);
         }
+        mbar_init(&bars[kBarO], 1);
         mbar_init(&bars[kBarDrain], 1);
         fence_mbarrier_init();
     }
@@ -192,9 +187,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
         }
         *reinterpret_cast<uint4*>(smem + kOffQ + r * 128 + ((c ^ (r & 7)) << 4)) = u;
     }
-    if (tid < kMaxQ) {
+    if (tid < NQ) {
         lim[tid] = tid < rows ? limit(r0 + tid) : kend;
-        negm[tid] = 0.f; nthr[tid] = INFINITY; colm[tid] = -INFINITY;
+        negm[tid] = kUnseen; colm[tid] = -INFINITY;
     }
     fence_proxy_async_smem();
     __syncthreads();
@@ -231,15 +226,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
                 r.ks = ksp[o]; r.vs = vsp[o];
             }
         };
-        RawRow ring[2];
-        if (ntl > 0) load(ring[0], 0);
-        if (ntl > 1) load(ring[1], 1);
-        for (int j0 = 0; j0 < ntl; j0 += 2) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int j = j0 + e;
-                if (j >= ntl) break;
-                const RawRow& r = ring[e];
+        RawRow nxt;
+        if (ntl > 0) load(nxt, 0);
+        for (int j = 0; j < ntl; ++j) {
+                const RawRow r = nxt;
+                if (j + 1 < ntl) load(nxt, j + 1);
                 const int s = j % kStages;
                 if (j >= kStages) {
                     // (stages ahead of the MMAs: this wait is the long one, and not urgent)
@@ -280,8 +271,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars[bar_ready(s)]);
-                if (j + 2 < ntl) load(ring[e], j + 2);
-            }
         }
     } else if (warp == kCtrlWarp) {
         if (ntl > 0) {
@@ -312,27 +301,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
                         mma_f16_ss(tmem + kTmemO, smem_desc_sw128(av + k * 2048, kVBytes, 1024),
                                    smem_desc_sw128(ap + k * 2048, kPBlock, 1024), idO, (j > 0 || k > 0) ? 1u : 0u);
                     mma_commit(&bars[bar_free(s)]);
-                    mma_commit(&bars[bar_o(j & 1)]);
+                    mma_commit(&bars[kBarO]);
                 }
                 __syncwarp();
             };
             // (decisions are the whole warp's: a lane alone never leaves the loop)
             auto wait_all = [&](int bar, uint32_t parity) {
-                wait(bar, parity);
+                if (!ok || !mbar_wait_sleep(&bars[bar], parity, 32, kWaitNs)) ok = false;   // none of these is urgent
                 ok = __all_sync(0xffffffffu, ok) != 0;
                 return ok;
             };
             for (int j = 0; j < min(2, ntl) && ok; ++j)
                 if (wait_all(bar_ready(j), 0)) issue_s(j);
+            // P·V of tile j before Sᵀ of tile j + 2, whose commit then also says that
+            // tile j's buffer of P is free
             for (int j = 0; j < ntl && ok; ++j) {
                 const int nx = j + 2;
-                if (nx < ntl) {
-                    if (!wait_all(bar_read(j & 1), (j / 2) & 1)) break;
-                    if (!wait_all(bar_ready(nx % kStages), (nx / kStages) & 1)) break;
-                    issue_s(nx);
-                }
                 if (!wait_all(bar_p(j & 1), (j / 2) & 1)) break;
                 issue_o(j);
+                if (nx < ntl && wait_all(bar_ready(nx % kStages), (nx / kStages) & 1)) issue_s(nx);
             }
             // every MMA is done before TMEM and shared memory are let go
             if (elect_one()) mma_commit(&bars[kBarDrain]);
@@ -340,68 +327,64 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             if (!mbar_wait(&bars[kBarDrain], 0, kDrainNs)) ok = false;
         }
     } else {
-        // ── softmax: thread = key; group g has 8·nch columns from c0 ────────
-        constexpr int kCh = NQ / 8, kMaxCh = (kCh + 3) / 4, kC = kMaxCh * 8;
-        const int grp = warp >> 2, win = warp & 3, row = win * 32 + lane;
-        const int nch = kCh / 4 + (grp < kCh % 4 ? 1 : 0);             // kMaxCh or one less
-        const int c0 = 8 * (grp * (kCh / 4) + min(grp, kCh % 4));
+        // ── softmax: thread = key; group g has the columns [16·g, 16·g + 16) ──
+        const int grp = warp >> 2, win = warp & 3, row = win * 32 + lane, c0 = kC * grp;
         const uint32_t lane_off = static_cast<uint32_t>(win * 32) << 16;
         const uint32_t tS = tmem + kTmemS + c0 + lane_off, tO = tmem + kTmemO + c0 + lane_off;
         const float sl2 = fabsf(p.sl2);
         const float2 s2 = make_float2(sl2, sl2);
-        uint32_t poff[kMaxCh];                     // this key's 16-byte chunks (8 columns) in P's buffer
+        uint32_t poff[2];                          // this key's two 16-byte chunks (8 columns) in P's buffer
 #pragma unroll
-        for (int i = 0; i < kMaxCh; ++i) {
-            const int c = (c0 >> 3) + i;
+        for (int i = 0; i < 2; ++i) {
+            const int c = 2 * grp + i;
             poff[i] = kOffP + (c >> 3) * kPBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4);
         }
-        auto has = [&](int i) { return i + 8 < kC || nch == kMaxCh; };   // is chunk i / 8 this group's?
         float2 l[kC / 2];
 #pragma unroll
         for (int i = 0; i < kC / 2; ++i) l[i] = make_float2(0.f, 0.f);
         for (int j = 0; j < ntl; ++j) {
             const int k0 = (t_begin + j) * kKeys, key = k0 + row, u = j & 1;
             const bool edge = k0 + kKeys > kfull || mask != nullptr;
-            wait(bar_s(u), (j / 2) & 1);
+            wait(bar_s(u), (j / 2) & 1);           // also: P·V of tile j − 2 is done, its P buffer free
             tc_fence_after_sync();
             float x[kC];
-#pragma unroll
-            for (int i = 0; i < kC; i += 8)
-                if (has(i)) tmem_ld8(tS + 96 * u + i, x + i);
+            tmem_ld16(tS + 96 * u, x);
             tmem_ld_wait();
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars[bar_read(u)]);
-            if (edge) {                            // keys that some row does not see
+            auto hide = [&]() {                    // keys that some row does not see
                 const bool vis = key < kend && (mask == nullptr || mask[key] != 0);
 #pragma unroll
-                for (int i = 0; i < kC; ++i)
-                    if (has(i)) x[i] = vis && key < lim[c0 + i] ? x[i] : -INFINITY;
-            }
-            // does any logit pass its row's reference by more than 8?
-            float over[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                for (int i = 0; i < kC; ++i) x[i] = vis && key < lim[c0 + i] ? x[i] : -INFINITY;
+            };
+            auto to_exponents = [&]() {            // x → x·sl2 − m
 #pragma unroll
-            for (int i = 0; i < kC; i += 4) {
-                if (!has(i)) continue;
-                const float4 t4 = *reinterpret_cast<const float4*>(nthr + c0 + i);
-                const float2 d0 = add2(make_float2(x[i], x[i + 1]), make_float2(t4.x, t4.y));
-                const float2 d1 = add2(make_float2(x[i + 2], x[i + 3]), make_float2(t4.z, t4.w));
-                over[(i / 4) & 3] = fmaxf(fmaxf(over[(i / 4) & 3], d0.x), d0.y);
-                over[(i / 4 + 2) & 3] = fmaxf(fmaxf(over[(i / 4 + 2) & 3], d1.x), d1.y);
-            }
-            if (bar_or(1 + grp, fmaxf(fmaxf(over[0], over[1]), fmaxf(over[2], over[3])) > 0.f)) {
+                for (int i = 0; i < kC; i += 4) {
+                    const float4 m4 = *reinterpret_cast<const float4*>(negm + c0 + i);
+                    const float2 t0 = fma2(make_float2(x[i], x[i + 1]), s2, make_float2(m4.x, m4.y));
+                    const float2 t1 = fma2(make_float2(x[i + 2], x[i + 3]), s2, make_float2(m4.z, m4.w));
+                    x[i] = t0.x; x[i + 1] = t0.y; x[i + 2] = t1.x; x[i + 3] = t1.y;
+                }
+            };
+            if (edge) hide();
+            to_exponents();
+            // does any logit pass its row's reference by more than 8? (a row that saw
+            // no key yet has the reference −kUnseen)
+            float over[2] = {x[0], x[1]};
+#pragma unroll
+            for (int i = 2; i < kC; i += 2) over[(i / 2) & 1] = fmaxf(fmaxf(over[(i / 2) & 1], x[i]), x[i + 1]);
+            if (bar_or(1 + grp, fmaxf(over[0], over[1]) > 8.f)) {
                 // raise the references: column maxima of the tile, over a warp's keys, then its group's warps
+                tmem_ld16(tS + 96 * u, x);
+                tmem_ld_wait();
+                if (edge) hide();
+                {
+                    float v[kC];
 #pragma unroll
-                for (int i = 0; i < kC; i += 8) {
-                    if (!has(i)) continue;
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = x[i + e];
-                    const float mx = reduce8(v, lane, [](float a, float c) { return fmaxf(a, c); });
-                    if (lane < 8) wred[win * kMaxQ + c0 + i + lane] = mx;
+                    for (int i = 0; i < kC; ++i) v[i] = x[i];
+                    const float mx = reduce16(v, lane, [](float a, float c) { return fmaxf(a, c); });
+                    if (lane < kC) wred[win * kMaxQ + c0 + lane] = mx;
                 }
                 named_bar_sync(1 + grp, 128);
-                if (row < 8 * nch) {
+                if (row < kC) {
                     const float* cm = wred + c0 + row;
                     const float t = fmaxf(fmaxf(cm[0], cm[kMaxQ]), fmaxf(cm[2 * kMaxQ], cm[3 * kMaxQ])) * sl2;
                     const float old = colm[c0 + row];
@@ -410,50 +393,39 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
                         al = old == -INFINITY ? 0.f : ex2(old - t);
                         colm[c0 + row] = t;
                         negm[c0 + row] = -t;
-                        nthr[c0 + row] = -(t + 8.f) / sl2;
                     }
                     alpha[c0 + row] = al;
                 }
                 named_bar_sync(1 + grp, 128);
 #pragma unroll
                 for (int i = 0; i < kC / 2; ++i) {
-                    if (!has(2 * i)) continue;
                     const float2 al = *reinterpret_cast<const float2*>(alpha + c0 + 2 * i);
                     l[i].x *= al.x; l[i].y *= al.y;
                 }
                 if (j > 0) {
-                    wait(bar_o(u ^ 1), ((j - 1) / 2) & 1);          // the accumulator is at rest
+                    wait(kBarO, (j - 1) & 1);                       // the accumulator is at rest
                     tc_fence_after_sync();
-#pragma unroll 1
-                    for (int i = 0; i < 8 * nch; i += 8) {
-                        float a[8];
-                        tmem_ld8(tO + i, a);
-                        tmem_ld_wait();
-                        uint32_t w[8];
+                    float a[kC];
+                    tmem_ld16(tO, a);
+                    tmem_ld_wait();
+                    uint32_t w[kC];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(a[e] * alpha[c0 + i + e]);
-                        tmem_st8(tO + i, w);
-                    }
+                    for (int i = 0; i < kC; ++i) w[i] = __float_as_uint(a[i] * alpha[c0 + i]);
+                    tmem_st16(tO, w);
                     tmem_st_wait();
                 }
                 named_bar_sync(1 + grp, 128);                       // alpha is read before it is written again
+                to_exponents();
             }
             // P = 2^(x·sl2 − m), row sums, fp16 P into this key's row
-            if (j > 1) wait(bar_o(u), ((j - 2) / 2) & 1);           // P's buffer is free
 #pragma unroll
             for (int i = 0; i < kC; i += 8) {
-                if (!has(i)) continue;
                 uint32_t h[4];
 #pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    const float4 m4 = *reinterpret_cast<const float4*>(negm + c0 + i + e);
-                    const float2 t0 = fma2(make_float2(x[i + e], x[i + e + 1]), s2, make_float2(m4.x, m4.y));
-                    const float2 t1 = fma2(make_float2(x[i + e + 2], x[i + e + 3]), s2, make_float2(m4.z, m4.w));
-                    const float2 p0 = make_float2(ex2(t0.x), ex2(t0.y)), p1 = make_float2(ex2(t1.x), ex2(t1.y));
+                for (int e = 0; e < 8; e += 2) {
+                    const float2 p0 = make_float2(ex2(x[i + e]), ex2(x[i + e + 1]));
                     l[(i + e) / 2] = add2(l[(i + e) / 2], p0);
-                    l[(i + e) / 2 + 1] = add2(l[(i + e) / 2 + 1], p1);
                     h[e / 2] = kv4::h2u(__floats2half2_rn(p0.x, p0.y));
-                    h[e / 2 + 1] = kv4::h2u(__floats2half2_rn(p1.x, p1.y));
                 }
                 *reinterpret_cast<uint4*>(smem + poff[i / 8] + u * 2 * kPBlock) = make_uint4(h[0], h[1], h[2], h[3]);
             }
@@ -463,39 +435,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_tc_kernel(const Kv4AttnP
             if (lane == 0) mbar_arrive(&bars[bar_p(u)]);
         }
         // row sums over the warp's keys
+        {
+            float v[kC];
 #pragma unroll
-        for (int i = 0; i < kC; i += 8) {
-            if (!has(i)) continue;
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (e & 1) ? l[(i + e) / 2].y : l[(i + e) / 2].x;
-            const float t = reduce8(v, lane, [](float a, float c) { return a + c; });
-            if (lane < 8) wred[win * kMaxQ + c0 + i + lane] = t;
+            for (int i = 0; i < kC; ++i) v[i] = (i & 1) ? l[i / 2].y : l[i / 2].x;
+            const float t = reduce16(v, lane, [](float a, float c) { return a + c; });
+            if (lane < kC) wred[win * kMaxQ + c0 + lane] = t;
         }
         // every P·V is done: P's memory becomes the partial result
-        if (ntl >= 1) wait(bar_o((ntl - 1) & 1), ((ntl - 1) / 2) & 1);
+        if (ntl >= 1) wait(kBarO, (ntl - 1) & 1);
         tc_fence_after_sync();
-        named_bar_sync(5, kSoftThreads);
+        named_bar_sync(7, kSoftThreads);
         {
             // lanes 0..15 hold row d of Oᵀ
             const int d = 16 * win + (lane & 15);
-#pragma unroll 1
-            for (int i = 0; i < 8 * nch; i += 8) {
-                float a[8];
-                tmem_ld8(tO + i, a);
-                tmem_ld_wait();
-                if (lane < 16) {
+            float a[kC];
+            tmem_ld16(tO, a);
+            tmem_ld_wait();
+            if (lane < 16) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) pO[(c0 + i + e) * D + d] = ntl > 0 ? a[e] : 0.f;
-                }
+                for (int i = 0; i < kC; ++i) pO[(c0 + i) * D + d] = ntl > 0 ? a[i] : 0.f;
             }
-            if (row < 8 * nch) {
+            if (row < kC) {
                 const float* ls = wred + c0 + row;
                 pM[c0 + row] = colm[c0 + row];
                 pL[c0 + row] = (ls[0] + ls[kMaxQ]) + (ls[2 * kMaxQ] + ls[3 * kMaxQ]);
             }
         }
-        named_bar_sync(5, kSoftThreads);
+        named_bar_sync(7, kSoftThreads);
         T* out = static_cast<T*>(p.out);
         auto store = [&](int r, int d, float4 a, float inv) {
             const int rr = r0 + r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
@@ -578,7 +545,7 @@ int launch(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     if (static_cast<int64_t>(p.c.Hkv) * p.rtiles > 65535 || p.c.B > 65535) return SFB_ERR_SHAPE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.splits, p.c.Hkv * p.rtiles, p.c.B);
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.blockDim = dim3(threads(NQ), 1, 1);
     cfg.dynamicSmemBytes = kSmemBytes;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
