@@ -12,8 +12,18 @@
 // turns them into MMA fragments in registers. The order of the contraction
 // index is free as long as both operands use the same, which is what makes the
 // loads whole: lane (g, t) = (lane / 4, lane % 4) holds for Sᵀ the channels
-// [D/4·t, D/4·(t+1)) of keys g and g + 8 and for Oᵀ the channels [D/8·g,
-// D/8·(g+1)) of keys 2t, 2t+1, 2t+8, 2t+9.
+// [D/4·t, D/4·(t+1)) of the keys of MMA rows g and g + 8 and for Oᵀ the channels
+// [D/8·g, D/8·(g+1)) of rows 2t, 2t+1, 2t+8, 2t+9. Row m of the MMA is key
+// key_of(m) of its tile, chosen so that either kind of load touches one
+// contiguous run of shared memory.
+// A tile is 16 keys; blocks of 128 give one to each of a CTA's eight warps. With
+// 64 channels a lane loads its codes of the next tile straight into registers
+// while it works on this one. With 128 those registers would cost the second CTA
+// per SM, so blocks go through a ring in shared memory, four untiled bulk copies
+// each (codes and scales of K and V), issued by a ninth warp (by warp 0 with 32
+// rows, whose warps need the ninth's registers). 32 sessions of 8 to 16 k slots
+// of 8 heads: 178 µs from registers, 153 through the ring; 32 sessions of 4374
+// slots of 32 64-channel heads: 105 µs from registers, 111 through the ring.
 // A nibble becomes fp16 exactly with one bit operation and one add or fma
 // (0x6400 | n = 1024 + n), the scale is one exact fp16 product (kv4.cu).
 // Pᵀ moves from the accumulator's layout to the B operand's by two movmatrix.
@@ -89,28 +99,45 @@ template <int D> struct VWords;
 template <> struct VWords<64>  { using T = uint32_t; };
 template <> struct VWords<128> { using T = uint2; };
 
-// Codes and scales of one 16-key tile as a lane holds them.
+constexpr float kUnseen = 1e30f;
+constexpr int kWarps = 8;                                        // computing
+__host__ __device__ constexpr bool uses_ring(int D) { return D == 128; }
+__host__ __device__ constexpr bool own_warp(int D, int NT) { return uses_ring(D) && NT < 4; }   // a ninth issues the copies
+__host__ __device__ constexpr int attn_threads(int D, int NT) { return (kWarps + (own_warp(D, NT) ? 1 : 0)) * 32; }
+constexpr int kBlock = 16 * kWarps;                              // keys per ring stage
+__host__ __device__ constexpr int code_bytes(int D) { return kBlock * D / 2; }
+__host__ __device__ constexpr int scale_bytes(int D) { return kBlock * (D / kGroup) * 2; }
+__host__ __device__ constexpr int stage_bytes(int D) { return 2 * (code_bytes(D) + scale_bytes(D)); }
+__host__ __device__ constexpr int ring_stages(int D) { return uses_ring(D) ? 4 : 0; }
+__host__ __device__ constexpr int attn_pad(int D) { return D + 8; }   // halves per row of Q in shared memory
+__host__ __device__ constexpr int join_bytes(int D, int NT) {         // per-warp O, m, l and the CTA's partial
+    return (kWarps + 1) * NT * 8 * (D + 2) * 4;
+}
+__host__ __device__ constexpr int attn_smem(int D, int NT) {
+    const int ring = stage_bytes(D) * ring_stages(D), join = join_bytes(D, NT);
+    return NT * 8 * attn_pad(D) * 2 + (ring > join ? ring : join) + 16 * ring_stages(D);
+}
+// Codes and scales of one 16-key tile as a lane holds them: K of MMA rows g and
+// g + 8 (channels [D/4·t, +D/4)), V of rows 2t, 2t+1, 2t+8, 2t+9 (channels [D/8·g, +D/8)).
 template <int D>
 struct Raw {
-    typename KWords<D>::T k[2];       // keys g, g + 8: channels [D/4·t, +D/4)
-    typename VWords<D>::T v[4];       // keys 2t, 2t+1, 2t+8, 2t+9: channels [D/8·g, +D/8)
+    typename KWords<D>::T k[2];
+    typename VWords<D>::T v[4];
     uint16_t ks[2], vs[4];
 };
 
-__host__ __device__ constexpr int attn_pad(int D) { return D + 8; }                  // halves per row of Q in shared memory
-__host__ __device__ constexpr int attn_smem(int D, int NT, int W) {
-    const int rows = NT * 8;
-    return rows * attn_pad(D) * 2                                // Q
-         + W * rows * D * 4 + W * rows * 2 * 4                   // per-warp O, m, l
-         + rows * D * 4 + rows * 2 * 4;                          // the CTA's partial
-}
+// The key of a 16-key tile that is row m of the MMAs.
+__device__ __forceinline__ int key_of(int m) { return ((m & 7) >> 1) + 4 * (m & 1) + 8 * (m >> 3); }
 
-template <typename T, int D, int NT, int W>
-__global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const Kv4AttnParams p) {
-    constexpr int kRows = NT * 8, kPad = attn_pad(D), kSteps = D / 16, kMT = D / 16;
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn_kernel(const Kv4AttnParams p) {
+    constexpr int kRows = NT * 8, kPad = attn_pad(D), kSteps = D / 16, kMT = D / 16, W = kWarps, kThreads = attn_threads(D, NT);
+    constexpr int kStages = ring_stages(D), kCode = code_bytes(D), kScale = scale_bytes(D), kStage = stage_bytes(D);
     extern __shared__ __align__(16) uint8_t smem[];
-    __half* sQ = reinterpret_cast<__half*>(smem);
-    float* sO = reinterpret_cast<float*>(smem + kRows * kPad * 2);        // [W][kRows][D]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem);                   // full, then empty
+    __half* sQ = reinterpret_cast<__half*>(smem + 16 * kStages);
+    uint8_t* ring = smem + 16 * kStages + kRows * kPad * 2;               // per stage: K codes, V codes, K, V scales
+    float* sO = reinterpret_cast<float*>(ring);                           // over the ring at the end: [W][kRows][D]
     float* sM = sO + W * kRows * D;                                       // [W][kRows]
     float* sL = sM + W * kRows;
     float* pO = sL + W * kRows;                                           // [kRows][D]
@@ -120,6 +147,10 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int split = blockIdx.x, hk = blockIdx.y / p.rtiles, rt = blockIdx.y - hk * p.rtiles, b = blockIdx.z;
     const int r0 = rt * kRows, rows = min(kRows, p.R - r0);
+    if (kStages > 0 && tid == 0) {
+        for (int i = 0; i < kStages; ++i) { ptx::mbar_init(&bars[i], 1); ptx::mbar_init(&bars[kStages + i], W); }
+        ptx::fence_mbarrier_init();
+    }
     pdl_trigger();
     pdl_wait();
 
@@ -128,13 +159,13 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const
     // a row sees the slots below limit(row)
     auto limit = [&](int r) { return p.causal ? min(n, max(0, n - p.Sq + r / p.g + 1)) : n; };
     const int kend = limit(r0 + rows - 1), kfull = limit(r0);             // limits grow with the row
-    const int tiles = (kend + 15) >> 4;
-    const int per = tiles / p.splits, rem = tiles - per * p.splits;
-    const int t_begin = split * per + min(split, rem), t_end = t_begin + per + (split < rem ? 1 : 0);
+    const int blocks = (kend + kBlock - 1) / kBlock;
+    const int per = blocks / p.splits, rem = blocks - per * p.splits;
+    const int b_begin = split * per + min(split, rem), nblk = per + (split < rem ? 1 : 0);
 
     // ── Q rows as fp16 in shared memory (zeros past the last row) ───────────
     bool bad = false;
-    for (int i = tid; i < kRows * (D / 8); i += W * 32) {
+    for (int i = tid; i < kRows * (D / 8); i += kThreads) {
         const int r = i / (D / 8), d = (i % (D / 8)) * 8;
         uint4 u = make_uint4(0, 0, 0, 0);
         if (r < rows) {
@@ -157,59 +188,13 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const
 
     const uint8_t* mask = p.key_mask != nullptr ? p.key_mask + b * p.mask_sb : nullptr;
     auto seen = [&](int key) { return key < kend && (mask == nullptr || mask[key] != 0); };
-    // this lane's codes and scales of tile `warp` of the CTA, advanced by W tiles
-    const int64_t first = static_cast<int64_t>(t_begin + warp) * 16;
-    const uint8_t* kp = p.c.kc + b * p.c.code_sb + hk * p.c.code_sh + (first + g) * (D / 2) + (D / 8) * t;
-    const uint8_t* vp = p.c.vc + b * p.c.code_sb + hk * p.c.code_sh + (first + 2 * t) * (D / 2) + (D / 16) * g;
-    const uint16_t* ksp = reinterpret_cast<const uint16_t*>(p.c.ks + b * p.c.sc_sb + hk * p.c.sc_sh) +
-                          (first + g) * (D / kGroup) + (D / 4 * t) / kGroup;
-    const uint16_t* vsp = reinterpret_cast<const uint16_t*>(p.c.vs + b * p.c.sc_sb + hk * p.c.sc_sh) +
-                          (first + 2 * t) * (D / kGroup) + (D / 8 * g) / kGroup;
-    // In a tile with slots that are not seen, those are not read (nor trusted:
-    // they may hold anything) and their scale is 0.
-    auto load = [&](Raw<D>& r, int tile) {
-        const int k0 = tile * 16;
-        using KT = typename KWords<D>::T;
-        using VT = typename VWords<D>::T;
-        if (k0 + 16 <= kend && mask == nullptr) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                r.k[i] = *reinterpret_cast<const KT*>(kp + 8 * i * (D / 2));
-                r.ks[i] = ksp[8 * i * (D / kGroup)];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = (i & 1) + 8 * (i >> 1);
-                r.v[i] = *reinterpret_cast<const VT*>(vp + row * (D / 2));
-                r.vs[i] = vsp[row * (D / kGroup)];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                r.k[i] = {}; r.ks[i] = 0;
-                if (k0 + g + 8 * i < kend) {
-                    r.k[i] = *reinterpret_cast<const KT*>(kp + 8 * i * (D / 2));
-                    r.ks[i] = ksp[8 * i * (D / kGroup)];
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = (i & 1) + 8 * (i >> 1);
-                r.v[i] = {}; r.vs[i] = 0;
-                if (seen(k0 + 2 * t + row)) {
-                    r.v[i] = *reinterpret_cast<const VT*>(vp + row * (D / 2));
-                    r.vs[i] = vsp[row * (D / kGroup)];
-                }
-            }
-        }
-        kp += 16 * W * (D / 2); vp += 16 * W * (D / 2);
-        ksp += 16 * W * (D / kGroup); vsp += 16 * W * (D / kGroup);
-    };
+    bool ok = true;
 
-    float o[kMT][NT][4], m[NT][2], l[NT][2];
+    const float sgn = p.sl2 < 0.f ? -1.f : 1.f;    // a masked logit is −∞ after the scaling
+    float o[kMT][NT][4], nm[NT][2], l[NT][2];      // nm: −reference
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        m[j][0] = m[j][1] = -INFINITY;
+        nm[j][0] = nm[j][1] = kUnseen;
         l[j][0] = l[j][1] = 0.f;
 #pragma unroll
         for (int i = 0; i < kMT; ++i) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
@@ -223,14 +208,14 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const
             for (int s = 0; s < kSteps / 2; ++s)
                 qr[j][s] = reinterpret_cast<const uint4*>(sQ + (j * 8 + g) * kPad + (D / 4) * t)[s];
     }
-    auto step = [&](const Raw<D>& cur, int tile) {
-        const int k0 = tile * 16;
+    auto step = [&](const Raw<D>& r, int k0) {
+        const bool edge = k0 + 16 > kfull || mask != nullptr;
         // K fragments: half2 2s and 2s+1 of a key's words are step s
         uint32_t ka[2][kSteps * 2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(&cur.k[i]);
-            const __half2 s = __half2half2(__ushort_as_half(cur.ks[i]));
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&r.k[i]);
+            const __half2 s = __half2half2(__ushort_as_half(r.ks[i]));
 #pragma unroll
             for (int x = 0; x < kSteps / 2; ++x) {
                 uint32_t d4[4];
@@ -239,95 +224,229 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const
                 for (int e = 0; e < 4; ++e) ka[i][4 * x + e] = d4[e];
             }
         }
-        // Vᵀ fragments: words of a key pair interleaved by halves, so that a
-        // nibble pair is one channel of both keys; [pair][word][low / high half]
-        uint32_t va[2][kMT / 4][2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&cur.v[2 * i]);
-            const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&cur.v[2 * i + 1]);
-            const __half2 s = __halves2half2(__ushort_as_half(cur.vs[2 * i]), __ushort_as_half(cur.vs[2 * i + 1]));
-#pragma unroll
-            for (int x = 0; x < kMT / 4; ++x) {
-                dequant_word(ptx::prmt(w0[x], w1[x], 0x5410u), s, va[i][x][0]);
-                dequant_word(ptx::prmt(w0[x], w1[x], 0x7632u), s, va[i][x][1]);
-            }
-        }
-        const bool edge = k0 + 16 > kfull || mask != nullptr;
-        bool vis0 = true, vis1 = true;
-        if (edge) { vis0 = seen(k0 + g); vis1 = seen(k0 + g + 8); }
+        uint32_t pb[NT][2];                        // Pᵀ fragments
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f}, c2[4] = {0.f, 0.f, 0.f, 0.f};      // two chains
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < kSteps; s += 2) {
                 uint4 q4;
                 if constexpr (kQReg) q4 = qr[j][s / 2];
                 else q4 = reinterpret_cast<const uint4*>(sQ + (j * 8 + g) * kPad + (D / 4) * t)[s / 2];
                 mma16816(c, ka[0][2 * s], ka[1][2 * s], ka[0][2 * s + 1], ka[1][2 * s + 1], q4.x, q4.y);
-                mma16816(c2, ka[0][2 * s + 2], ka[1][2 * s + 2], ka[0][2 * s + 3], ka[1][2 * s + 3], q4.z, q4.w);
+                mma16816(c, ka[0][2 * s + 2], ka[1][2 * s + 2], ka[0][2 * s + 3], ka[1][2 * s + 3], q4.z, q4.w);
             }
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = (c[e] + c2[e]) * p.sl2;
             if (edge) {
                 const int ra = min(r0 + j * 8 + 2 * t, p.R - 1), rb = min(r0 + j * 8 + 2 * t + 1, p.R - 1);
-                const int la = limit(ra), lb = limit(rb);
-                if (!vis0 || k0 + g >= la) x[0] = -INFINITY;
-                if (!vis0 || k0 + g >= lb) x[1] = -INFINITY;
-                if (!vis1 || k0 + g + 8 >= la) x[2] = -INFINITY;
-                if (!vis1 || k0 + g + 8 >= lb) x[3] = -INFINITY;
+                const int la = limit(ra), lb = limit(rb), ka_ = k0 + key_of(g), kb_ = ka_ + 8;
+                const bool v0 = seen(ka_), v1 = seen(kb_);
+                if (!v0 || ka_ >= la) c[0] = -INFINITY * sgn;
+                if (!v0 || ka_ >= lb) c[1] = -INFINITY * sgn;
+                if (!v1 || kb_ >= la) c[2] = -INFINITY * sgn;
+                if (!v1 || kb_ >= lb) c[3] = -INFINITY * sgn;
             }
-            float ma = fmaxf(x[0], x[2]), mb = fmaxf(x[1], x[3]);
-            if (__any_sync(0xffffffffu, ma > m[j][0] + 8.f || mb > m[j][1] + 8.f)) {
+            // exponents against the rows' references; a row that saw no key yet has
+            // the reference −kUnseen, so that its first key passes it
+            float x[4] = {fmaf(c[0], p.sl2, nm[j][0]), fmaf(c[1], p.sl2, nm[j][1]), fmaf(c[2], p.sl2, nm[j][0]),
+                          fmaf(c[3], p.sl2, nm[j][1])};
+            if (__any_sync(0xffffffffu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > 8.f)) {
+                float ma = fmaxf(c[0] * p.sl2, c[2] * p.sl2), mb = fmaxf(c[1] * p.sl2, c[3] * p.sl2);
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) {
                     ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, off));
                     mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, off));
                 }
                 float aa = 1.f, ab = 1.f;
-                if (ma > m[j][0] + 8.f) { aa = m[j][0] == -INFINITY ? 0.f : ptx::ex2(m[j][0] - ma); m[j][0] = ma; }
-                if (mb > m[j][1] + 8.f) { ab = m[j][1] == -INFINITY ? 0.f : ptx::ex2(m[j][1] - mb); m[j][1] = mb; }
+                if (ma + nm[j][0] > 8.f) { aa = nm[j][0] == kUnseen ? 0.f : ptx::ex2(-nm[j][0] - ma); nm[j][0] = -ma; }
+                if (mb + nm[j][1] > 8.f) { ab = nm[j][1] == kUnseen ? 0.f : ptx::ex2(-nm[j][1] - mb); nm[j][1] = -mb; }
                 l[j][0] *= aa; l[j][1] *= ab;
 #pragma unroll
                 for (int i = 0; i < kMT; ++i) {
                     o[i][j][0] *= aa; o[i][j][1] *= ab; o[i][j][2] *= aa; o[i][j][3] *= ab;
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = fmaf(c[e], p.sl2, nm[j][e & 1]);
             }
-            const float ua = m[j][0] == -INFINITY ? 0.f : m[j][0], ub = m[j][1] == -INFINITY ? 0.f : m[j][1];
-            const float p0 = ptx::ex2(x[0] - ua), p1 = ptx::ex2(x[1] - ub);
-            const float p2 = ptx::ex2(x[2] - ua), p3 = ptx::ex2(x[3] - ub);
+            const float p0 = ptx::ex2(x[0]), p1 = ptx::ex2(x[1]), p2 = ptx::ex2(x[2]), p3 = ptx::ex2(x[3]);
             l[j][0] += p0 + p2;
             l[j][1] += p1 + p3;
-            const uint32_t b0 = movmatrix_t(h2u(__floats2half2_rn(p0, p1)));
-            const uint32_t b1 = movmatrix_t(h2u(__floats2half2_rn(p2, p3)));
+            pb[j][0] = movmatrix_t(h2u(__floats2half2_rn(p0, p1)));
+            pb[j][1] = movmatrix_t(h2u(__floats2half2_rn(p2, p3)));
+        }
+        // Vᵀ fragments: words of a key pair interleaved by halves, so that a
+        // nibble pair is one channel of both keys; [pair][word][low / high half]
+        uint32_t va[2][kMT / 4][2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&r.v[2 * i]);
+            const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&r.v[2 * i + 1]);
+            const __half2 s = __halves2half2(__ushort_as_half(r.vs[2 * i]), __ushort_as_half(r.vs[2 * i + 1]));
+#pragma unroll
+            for (int x = 0; x < kMT / 4; ++x) {
+                dequant_word(ptx::prmt(w0[x], w1[x], 0x5410u), s, va[i][x][0]);
+                dequant_word(ptx::prmt(w0[x], w1[x], 0x7632u), s, va[i][x][1]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int i = 0; i < kMT; ++i)
                 mma16816(o[i][j], va[0][i / 4][0][i % 4], va[0][i / 4][1][i % 4], va[1][i / 4][0][i % 4],
-                         va[1][i / 4][1][i % 4], b0, b1);
-        }
+                         va[1][i / 4][1][i % 4], pb[j][0], pb[j][1]);
     };
-    // tiles in flight per warp: two where the registers allow two CTAs per SM all the same
-    constexpr int kDepth = (NT == 1 && D == 64) ? 2 : 1;
-    Raw<D> ring[kDepth];
-    int tile = t_begin + warp;
+    if constexpr (!uses_ring(D)) {
+        // the next tile's codes are in flight while this one is worked on; slots
+        // that are not seen are not read
+        const int64_t first = static_cast<int64_t>(b_begin) * kBlock + warp * 16;
+        const int64_t hb = b * p.c.code_sb + hk * p.c.code_sh, hs = b * p.c.sc_sb + hk * p.c.sc_sh;
+        using KT = typename KWords<D>::T;
+        using VT = typename VWords<D>::T;
+        const uint8_t* kp = p.c.kc + hb + (first + key_of(g)) * (D / 2) + (D / 8) * t;
+        const uint8_t* vp = p.c.vc + hb + (first + t) * (D / 2) + (D / 16) * g;
+        const uint16_t* ksp = reinterpret_cast<const uint16_t*>(p.c.ks + hs) + (first + key_of(g)) * (D / kGroup) + (D / 4 * t) / kGroup;
+        const uint16_t* vsp = reinterpret_cast<const uint16_t*>(p.c.vs + hs) + (first + t) * (D / kGroup) + (D / 8 * g) / kGroup;
+        auto load = [&](Raw<D>& r, int k0) {       // tiles in order: the pointers move along
+            const bool whole = k0 + 16 <= kend && mask == nullptr;
+            if (whole) {
 #pragma unroll
-    for (int i = 0; i < kDepth; ++i)
-        if (tile + i * W < t_end) load(ring[i], tile + i * W);
-    for (; tile < t_end; tile += kDepth * W) {
+                for (int e = 0; e < 2; ++e) {
+                    r.k[e] = *reinterpret_cast<const KT*>(kp + 8 * e * (D / 2));
+                    r.ks[e] = ksp[8 * e * (D / kGroup)];
+                }
 #pragma unroll
-        for (int i = 0; i < kDepth; ++i) {
-            const int cur_tile = tile + i * W;
-            if (i > 0 && cur_tile >= t_end) break;
-            const Raw<D> cur = ring[i];
-            if (cur_tile + kDepth * W < t_end) load(ring[i], cur_tile + kDepth * W);
-            step(cur, cur_tile);
+                for (int e = 0; e < 4; ++e) {
+                    r.v[e] = *reinterpret_cast<const VT*>(vp + 4 * e * (D / 2));
+                    r.vs[e] = vsp[4 * e * (D / kGroup)];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    r.k[e] = {}; r.ks[e] = 0;
+                    if (seen(k0 + key_of(g) + 8 * e)) {
+                        r.k[e] = *reinterpret_cast<const KT*>(kp + 8 * e * (D / 2));
+                        r.ks[e] = ksp[8 * e * (D / kGroup)];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    r.v[e] = {}; r.vs[e] = 0;
+                    if (seen(k0 + t + 4 * e)) {
+                        r.v[e] = *reinterpret_cast<const VT*>(vp + 4 * e * (D / 2));
+                        r.vs[e] = vsp[4 * e * (D / kGroup)];
+                    }
+                }
+            }
+            kp += kBlock * (D / 2); vp += kBlock * (D / 2);
+            ksp += kBlock * (D / kGroup); vsp += kBlock * (D / kGroup);
+        };
+        const int k_end = min(kend, (b_begin + nblk) * kBlock);
+        int k0 = static_cast<int>(first);
+        // two tiles ahead, in three sets of registers by turns (copies between them
+        // were a twentieth of a tile's instructions)
+        Raw<D> ra, rb, rc;
+        auto turn = [&](const Raw<D>& now, Raw<D>& later) {
+            if (k0 + 2 * kBlock < k_end) load(later, k0 + 2 * kBlock);
+            step(now, k0);
+            k0 += kBlock;
+            return k0 < k_end;
+        };
+        if (k0 < k_end) load(ra, k0);
+        if (k0 + kBlock < k_end) load(rb, k0 + kBlock);
+        while (k0 < k_end) {
+            if (!turn(ra, rc)) break;
+            if (!turn(rb, ra)) break;
+            turn(rc, rb);
         }
+    } else {
+        // this lane's codes and scales of a tile in shared memory. Slots that are not
+        // seen may hold anything: their scale is taken as 0.
+        auto fetch = [&](Raw<D>& r, const uint8_t* kc, const uint8_t* vc, const uint16_t* ks, const uint16_t* vs,
+                         int in_block, int k0) {
+    #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int key = in_block + key_of(g) + 8 * i;
+                r.k[i] = *reinterpret_cast<const typename KWords<D>::T*>(kc + key * (D / 2) + (D / 8) * t);
+                r.ks[i] = ks[key * (D / kGroup) + (D / 4 * t) / kGroup];
+            }
+    #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = in_block + t + 4 * i;            // key_of(2t + (i & 1) + 8·(i >> 1))
+                r.v[i] = *reinterpret_cast<const typename VWords<D>::T*>(vc + key * (D / 2) + (D / 16) * g);
+                r.vs[i] = vs[key * (D / kGroup) + (D / 8 * g) / kGroup];
+            }
+            if (k0 + 16 > kend || mask != nullptr) {
+    #pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (!seen(k0 + key_of(g) + 8 * i)) r.ks[i] = 0;
+    #pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!seen(k0 + t + 4 * i)) r.vs[i] = 0;
+            }
+        };
+        // ── copies of block i (one lane), once its stage is free ───────────────
+        auto copy_block = [&](int i) {
+            const int s = i % kStages;
+            if (i >= kStages && !ptx::mbar_wait(&bars[kStages + s], ((i / kStages) - 1) & 1)) return false;
+            const int64_t hb = b * p.c.code_sb + hk * p.c.code_sh, hs = b * p.c.sc_sb + hk * p.c.sc_sh;
+            const int64_t key0 = static_cast<int64_t>(b_begin + i) * kBlock;
+            // whole groups of four slots: the capacity is a multiple of 4
+            const uint32_t n4 = static_cast<uint32_t>(min(static_cast<int64_t>(kBlock), (kend + 3) / 4 * 4 - key0));
+            const uint32_t cb = n4 * (D / 2), sb = n4 * (D / kGroup) * 2;
+            uint8_t* st = ring + s * kStage;
+            ptx::mbar_arrive_expect_tx(&bars[s], 2 * (cb + sb));
+            ptx::bulk_load(st, p.c.kc + hb + key0 * (D / 2), cb, &bars[s]);
+            ptx::bulk_load(st + kCode, p.c.vc + hb + key0 * (D / 2), cb, &bars[s]);
+            ptx::bulk_load(st + 2 * kCode, p.c.ks + hs + key0 * (D / kGroup), sb, &bars[s]);
+            ptx::bulk_load(st + 2 * kCode + kScale, p.c.vs + hs + key0 * (D / kGroup), sb, &bars[s]);
+            return true;
+        };
+        int issued = 0;                                // blocks copied, in the copying lane
+        auto copy_up_to = [&](int end) {
+            while (ok && issued < end) {
+                if (copy_block(issued)) ++issued;
+                else ok = false;
+            }
+        };
+        if (own_warp(D, NT) && warp == W) {
+            if (lane == 0) copy_up_to(nblk);
+        } else {
+            auto take = [&](Raw<D>& r, int i) {
+                const int s = i % kStages;
+                if (!own_warp(D, NT) && warp == 0) {      // (stage of block i + kStages − 1: block i − 1 was its last)
+                    if (lane == 0) copy_up_to(min(nblk, i + kStages - (i > 0 ? 1 : 0)));
+                    __syncwarp();
+                }
+                if (!ok || !ptx::mbar_wait(&bars[s], (i / kStages) & 1)) ok = false;
+                ok = __all_sync(0xffffffffu, ok) != 0;
+                const uint8_t* st = ring + s * kStage;
+                if (ok)
+                    fetch(r, st, st + kCode, reinterpret_cast<const uint16_t*>(st + 2 * kCode),
+                          reinterpret_cast<const uint16_t*>(st + 2 * kCode + kScale), warp * 16,
+                          (b_begin + i) * kBlock + warp * 16);
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&bars[kStages + s]);
+            };
+            auto work = [&](const Raw<D>& r, int i) {
+                const int k0 = (b_begin + i) * kBlock + warp * 16;
+                if (ok && k0 < kend) step(r, k0);
+            };
+            Raw<D> r{};
+            for (int i = 0; i < nblk; ++i) {
+                take(r, i);
+                work(r, i);
+            }
+        }
+        // nothing is in flight when the ring becomes the joining buffer
+        if (lane == 0)
+            for (int i = max(0, issued - kStages); i < issued; ++i)
+                if (!ptx::mbar_wait(&bars[i % kStages], (i / kStages) & 1)) ok = false;
     }
+    __syncthreads();
 
     // ── join the warps ──────────────────────────────────────────────────────
     // a lane holds, of rows 8j + 2t and + 1, the channels [D/8·g, +D/8): value
     // 8x + 2y + e of them is o[4x + y][j][row + 2e]
+    if (warp < W)
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -336,7 +455,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, off);
             const int r = j * 8 + 2 * t + e;
-            if (g == 0) { sM[warp * kRows + r] = m[j][e]; sL[warp * kRows + r] = ls; }
+            if (g == 0) { sM[warp * kRows + r] = nm[j][e] == kUnseen ? -INFINITY : -nm[j][e]; sL[warp * kRows + r] = ls; }
             float* dst = sO + (warp * kRows + r) * D + (D / 8) * g;
 #pragma unroll
             for (int x = 0; x < kMT / 2; ++x)
@@ -358,7 +477,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const
         }
         *reinterpret_cast<uint2*>(dst) = u;
     };
-    for (int i = tid; i < rows * (D / 4); i += W * 32) {
+    for (int i = tid; i < rows * (D / 4); i += kThreads) {
         const int r = i / (D / 4), d = (i % (D / 4)) * 4;
         float M = -INFINITY, L = 0.f;
         for (int w = 0; w < W; ++w) M = fmaxf(M, sM[w * kRows + r]);
@@ -372,7 +491,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const
             a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
         }
         if (p.splits == 1) {
-            store(r, d, a, L != 0.f ? 1.f / L : 0.f);
+            if (ok) store(r, d, a, L != 0.f ? 1.f / L : 0.f);
         } else {
             *reinterpret_cast<float4*>(pO + r * D + d) = a;
             if (d == 0) { pM[r] = M; pL[r] = L; }
@@ -383,7 +502,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const
         ptx::cluster_sync();                       // every partial is written
         const uint32_t aO = ptx::smem_u32(pO), aM = ptx::smem_u32(pM), aL = ptx::smem_u32(pL);
         const int mine = split < rows ? (rows - split + p.splits - 1) / p.splits : 0;
-        for (int i = tid; i < mine * (D / 4); i += W * 32) {
+        for (int i = tid; i < mine * (D / 4); i += kThreads) {
             const int r = split + (i / (D / 4)) * p.splits, d = (i % (D / 4)) * 4;
             float M = -INFINITY, L = 0.f;
             for (int k = 0; k < p.splits; ++k) M = fmaxf(M, ptx::dsmem_ld_f32(ptx::dsmem_map(aM + 4 * r, k)));
@@ -397,19 +516,20 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const
                 const float4 v = ptx::dsmem_ld_f32x4(ptx::dsmem_map(aO + 4 * (r * D + d), k));
                 a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
             }
-            store(r, d, a, L != 0.f ? 1.f / L : 0.f);
+            if (ok) store(r, d, a, L != 0.f ? 1.f / L : 0.f);
         }
         ptx::cluster_sync();                       // nobody leaves while its partial may be read
     }
     if (bad) atomicExch(&g_sfb_device_error, SFB_ERR_RANGE);
+    if (!ok) atomicExch(&g_sfb_device_error, SFB_ERR_DEVICE_TIMEOUT);
 }
 
-template <typename T, int D, int NT, int W>
+template <typename T, int D, int NT>
 int launch_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     const DeviceInfo& dev = device_info();
-    constexpr int smem = attn_smem(D, NT, W);
+    constexpr int smem = attn_smem(D, NT);
     static_assert(smem <= 227 * 1024, "shared memory budget");
-    auto kern = kv4_attn_kernel<T, D, NT, W>;
+    auto kern = kv4_attn_kernel<T, D, NT>;
     static std::atomic<bool> done[64];             // kernel attributes, once per device (idempotent)
     if (!done[dev.ordinal & 63].load(std::memory_order_acquire)) {
         const cudaError_t e1 = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -423,18 +543,25 @@ int launch_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     }
     p.rtiles = (p.R + NT * 8 - 1) / (NT * 8);
     const int64_t units = static_cast<int64_t>(p.c.B) * p.c.Hkv * p.rtiles;
-    const int tiles = (p.Sk + 15) / 16;
+    const int blocks = (p.Sk + kBlock - 1) / kBlock;
     int sp = num_splits;
     if (sp == 0) {
-        // enough CTAs for every SM, at least two tiles for each of a CTA's warps
-        sp = static_cast<int>(std::min<int64_t>(16, std::max<int64_t>(1, dev.num_sms / units)));
-        sp = std::min(sp, std::max(1, tiles / (2 * W)));
+        // Two CTAs for every SM (a power of two: a cluster of 8 measured 43 µs
+        // where 12 took 56, 4 sessions of 8 heads and 16 k slots). With more units
+        // than that, cut the long ones into 4096 slots and more until there are
+        // about 1024 CTAs, so that sessions of different lengths fill the SMs
+        // evenly (32 of them: see the table). At least a block a CTA.
+        const int64_t fill = std::max<int64_t>(1, 2 * dev.num_sms / units);
+        sp = 1;
+        while (sp < 16 && 2 * sp <= fill) sp *= 2;
+        const int64_t fine = std::min<int64_t>(1024 / units, p.Sk / 4096);
+        if (fine > sp) sp = static_cast<int>(std::min<int64_t>(fine, 8));
     }
-    p.splits = std::min(sp, std::max(1, tiles));
+    p.splits = std::min(sp, std::max(1, blocks));
     if (static_cast<int64_t>(p.c.Hkv) * p.rtiles > 65535 || p.c.B > 65535) return SFB_ERR_SHAPE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.splits, p.c.Hkv * p.rtiles, p.c.B);
-    cfg.blockDim = dim3(W * 32, 1, 1);
+    cfg.blockDim = dim3(attn_threads(D, NT), 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -452,13 +579,13 @@ int launch_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
 template <typename T>
 int pick_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     if (p.c.D == 64) {
-        if (p.R <= 8) return launch_attn<T, 64, 1, 8>(p, num_splits, s);
-        if (p.R <= 16) return launch_attn<T, 64, 2, 8>(p, num_splits, s);
+        if (p.R <= 8) return launch_attn<T, 64, 1>(p, num_splits, s);
+        if (p.R <= 16) return launch_attn<T, 64, 2>(p, num_splits, s);
         return kv4tc::pick<T>(p, num_splits, s);
     }
-    if (p.R <= 8) return launch_attn<T, 128, 1, 8>(p, num_splits, s);
-    if (p.R <= 16) return launch_attn<T, 128, 2, 8>(p, num_splits, s);
-    return launch_attn<T, 128, 4, 8>(p, num_splits, s);
+    if (p.R <= 8) return launch_attn<T, 128, 1>(p, num_splits, s);
+    if (p.R <= 16) return launch_attn<T, 128, 2>(p, num_splits, s);
+    return launch_attn<T, 128, 4>(p, num_splits, s);
 }
 
 }  // namespace kv4

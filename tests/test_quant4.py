@@ -117,6 +117,7 @@ BAD_CACHES = [
     (dict(k_codes=0), _capi.SFB_ERR_INVALID), (dict(v_scale=0), _capi.SFB_ERR_INVALID),
     (dict(head_dim=96), _capi.SFB_ERR_SHAPE), (dict(head_dim=0), _capi.SFB_ERR_SHAPE),
     (dict(heads_kv=0), _capi.SFB_ERR_SHAPE), (dict(capacity=-1), _capi.SFB_ERR_SHAPE),
+    (dict(capacity=66), _capi.SFB_ERR_SHAPE),
     (dict(k_codes=0x1008), _capi.SFB_ERR_ALIGN), (dict(v_scale=0x1002), _capi.SFB_ERR_ALIGN),
     ({"code_stride[1]": 2056}, _capi.SFB_ERR_ALIGN), ({"scale_stride[0]": 514}, _capi.SFB_ERR_ALIGN),
 ]
