@@ -8,13 +8,15 @@
 // type of the attention's products: nothing is lost between the cache and the
 // tensor cores, and no scale has to be carried into their epilogue.
 //
-// Both kernels are bound by bytes. A row of D channels is held by D / 8 lanes,
-// 8 values each: one 16-byte load of a 16-bit type, one 32-bit word of codes;
-// 4 lanes make one 32-channel group. A warp takes 32 / (D / 8) consecutive
-// tokens of one head, so that its codes are one contiguous 128-byte run of the
-// cache, and neighbouring warps take neighbouring heads, whose source rows are
-// contiguous in a projection's output.
+// Both kernels are bound by bytes, if they spend few instructions on each: a row
+// of D channels is held by D / 8 lanes, 8 values each (one 16-byte load of a
+// 16-bit type, one 32-bit word of codes), 4 lanes make one 32-channel group; a
+// warp holds 32 / (D / 8) consecutive tokens of one head, so that its codes are
+// one contiguous 128-byte run of the cache, and takes kRuns such runs, loaded
+// before the first is worked on; neighbouring warps take neighbouring heads,
+// whose source rows are contiguous in a projection's output.
 #include "common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace sfb {
 
@@ -42,23 +44,51 @@ constexpr int kGroup = 32;                       // channels per scale
 constexpr int kMoveThreads = 256;
 constexpr float kMaxScale = 9344.f;              // 7 · 9344 = 65408, the largest such product in fp16
 
-// Eight codes (c + 8) of one 32-bit word: value 2i at bits 4i, 2i+1 at 16+4i.
-__device__ __forceinline__ int nibble_shift(int e) { return 4 * (e >> 1) + 16 * (e & 1); }
+// (x & mask) | 0x64006400 in one LOP3
+template <uint32_t kMask>
+__device__ __forceinline__ uint32_t nib_magic(uint32_t x) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "n"(kMask), "n"(0x64006400u));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
-struct Where { int b, hh, tok; bool ok; };       // hh: K heads, then V heads
+// The eight codes of a word as four half2 times s: o[i] = (nibble at 4i, nibble at 16 + 4i).
+__device__ __forceinline__ void dequant_word(uint32_t w, __half2 s, uint32_t (&o)[4]) {
+    const __half2 k1032 = __half2half2(__ushort_as_half(0x6408));           // 1024 + 8
+    const __half2 k16 = __half2half2(__ushort_as_half(0x2c00));             // 1 / 16
+    const __half2 k72 = __half2half2(__ushort_as_half(0xd480));             // −(64 + 8)
+    const uint32_t w8 = w >> 8;
+    o[0] = h2u(__hmul2(__hsub2(u2h(nib_magic<0x000f000fu>(w)), k1032), s));
+    o[1] = h2u(__hmul2(__hfma2(u2h(nib_magic<0x00f000f0u>(w)), k16, k72), s));
+    o[2] = h2u(__hmul2(__hsub2(u2h(nib_magic<0x000f000fu>(w8)), k1032), s));
+    o[3] = h2u(__hmul2(__hfma2(u2h(nib_magic<0x00f000f0u>(w8)), k16, k72), s));
+}
+
+constexpr int kRuns = 4;
+
+// Where a warp's work is: session, head (K heads, then V heads), first token.
+struct Where { int b, h; int32_t tok; bool is_v, ok; };
 
 template <int D>
 __device__ __forceinline__ Where where(const Kv4MoveParams& p) {
     constexpr int kLanes = D / 8, kTok = 32 / kLanes;
     const uint32_t w = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5);
+    const uint32_t heads2 = 2 * p.c.Hkv, wt = w / heads2, hh = w - wt * heads2;
     Where r;
     r.ok = w < p.warps;
-    const uint32_t heads2 = 2 * p.c.Hkv;
-    const uint32_t wt = w / heads2;
-    r.hh = static_cast<int>(w - wt * heads2);
+    r.is_v = hh >= static_cast<uint32_t>(p.c.Hkv);
+    r.h = static_cast<int>(hh) - (r.is_v ? p.c.Hkv : 0);
     r.b = static_cast<int>(wt / static_cast<uint32_t>(p.tgroups));
-    r.tok = static_cast<int>(wt - r.b * p.tgroups) * kTok + (threadIdx.x & 31) / kLanes;
-    r.ok = r.ok && r.tok < p.seq;
+    r.tok = static_cast<int>(wt - r.b * p.tgroups) * (kTok * kRuns) + (threadIdx.x & 31) / kLanes;
+    return r;
+}
+
+// fmaxf that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 
@@ -66,88 +96,119 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(const Kv4MoveParams p) {
     pdl_trigger();
     pdl_wait();
-    constexpr int kLanes = D / 8;
-    Where r = where<D>(p);
+    constexpr int kLanes = D / 8, kTok = 32 / kLanes;
+    const Where r = where<D>(p);
     const int sub = threadIdx.x % kLanes;
-    const bool is_v = r.hh >= p.c.Hkv;
-    const int h = is_v ? r.hh - p.c.Hkv : r.hh;
-    int64_t slot = 0;
+    if (!r.ok) return;                             // (whole warps)
+    const int32_t n = p.len != nullptr ? min(p.seq, p.len[r.b]) : p.seq;
+    const int64_t slot0 = static_cast<int64_t>(p.start != nullptr ? p.start[r.b] : p.slot0) + r.tok;
+    const int64_t sb = r.is_v ? p.v_st[0] : p.k_st[0], sh = r.is_v ? p.v_st[1] : p.k_st[1], ss = r.is_v ? p.v_st[2] : p.k_st[2];
+    const T* src = static_cast<const T*>(r.is_v ? p.v : p.k) + r.b * sb + r.h * sh + r.tok * ss + sub * 8;
+    uint8_t* codes = (r.is_v ? p.c.vc : p.c.kc) + r.b * p.c.code_sb + r.h * p.c.code_sh + sub * 4;
+    __half* sc = (r.is_v ? p.c.vs : p.c.ks) + r.b * p.c.sc_sb + r.h * p.c.sc_sh + (sub >> 2);
     bool bad = false;
-    if (r.ok) {
-        if (p.len != nullptr && r.tok >= p.len[r.b]) r.ok = false;
-        slot = static_cast<int64_t>(p.start != nullptr ? p.start[r.b] : p.slot0) + r.tok;
-        if (r.ok && (slot < 0 || slot >= p.c.cap)) { bad = true; r.ok = false; }
+    float x[kRuns][8];
+#pragma unroll
+    for (int u = 0; u < kRuns; ++u) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+        if (r.tok + u * kTok < n) nrope::load8(src + u * kTok * ss, x[u]);
     }
-    float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (r.ok) {
-        const int64_t* st = is_v ? p.v_st : p.k_st;
-        const T* src = static_cast<const T*>(is_v ? p.v : p.k) + r.b * st[0] + h * st[1] + r.tok * st[2] + sub * 8;
-        nrope::load8(src, x);
-    }
-    // max |x| of the group as an integer: infinities and NaN order above every number
-    uint32_t mx = 0;
+    for (int u = 0; u < kRuns; ++u) {
+        float mx = fabsf(x[u][0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(x[i]) & 0x7fffffffu);
-    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    float s = __half2float(__float2half_rn(__bfloat162float(__float2bfloat16_rn(__uint_as_float(mx) / 7.f))));
-    const bool fits = mx < 0x7f800000u && s <= kMaxScale;
-    uint32_t word = 0x88888888u;
-    if (fits && s > 0.f) {
-        // x / s correctly rounded, as the division would give it, for eight x and
-        // one reciprocal: q = x·y and one residual step q + (x − q·s)·y with y =
-        // 1 / s correctly rounded (Markstein, 1990)
-        const float y = 1.f / s;
-        word = 0;
+        for (int i = 1; i < 8; ++i) mx = max_nan(mx, fabsf(x[u][i]));
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float s = __half2float(__float2half_rn(__bfloat162float(__float2bfloat16_rn(mx / 7.f))));
+        const bool fits = s <= kMaxScale;          // not for an infinity or a NaN
+        uint32_t word = 0x88888888u;
+        if (fits && s > 0.f) {
+            // x / s correctly rounded, as the division would give it, for eight x and
+            // one reciprocal: q = x·y and one residual step q + (x − q·s)·y with y =
+            // 1 / s correctly rounded (Markstein, 1990). Then rounded to an integer
+            // by adding 1.5·2^23, and four of them combined exactly in fp32.
+            const float y = 1.f / s, magic = 12582912.f;
+            float half_[2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float q = x[i] * y;
-            q = fmaf(fmaf(-q, s, x[i]), y, q);
-            const float c = fminf(7.f, fmaxf(-7.f, rintf(q)));
-            word |= static_cast<uint32_t>(static_cast<int>(c) + 8) << nibble_shift(i);
+            for (int e = 0; e < 2; ++e) {          // values 2i + e: one 16-bit half of the word
+                float acc = 34952.f;               // the + 8 of every nibble: 8·(1 + 16 + 256 + 4096)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float q = x[u][2 * i + e] * y;
+                    q = fmaf(fmaf(-q, s, x[u][2 * i + e]), y, q);
+                    if (s < 6.1035e-5f) q = fminf(7.f, fmaxf(-7.f, q));   // only a subnormal scale is off by more than 2^-9
+                    acc = fmaf((q + magic) - magic, static_cast<float>(1 << (4 * i)), acc);
+                }
+                half_[e] = acc + 8388608.f;
+            }
+            word = ptx::prmt(__float_as_uint(half_[0]), __float_as_uint(half_[1]), 0x5410u);
         }
-    }
-    if (r.ok) {
-        uint8_t* codes = (is_v ? p.c.vc : p.c.kc) + r.b * p.c.code_sb + h * p.c.code_sh + slot * (D / 2);
-        *reinterpret_cast<uint32_t*>(codes + sub * 4) = word;
-        if ((sub & 3) == 0) {
-            __half* sc = (is_v ? p.c.vs : p.c.ks) + r.b * p.c.sc_sb + h * p.c.sc_sh + slot * (D / kGroup);
-            sc[sub >> 2] = fits ? __float2half_rn(s) : __ushort_as_half(0x7fff);
+        const int64_t slot = slot0 + u * kTok;
+        if (r.tok + u * kTok < n) {
+            if (slot >= 0 && slot < p.c.cap) {
+                *reinterpret_cast<uint32_t*>(codes + slot * (D / 2)) = word;
+                if ((sub & 3) == 0) sc[slot * (D / kGroup)] = fits ? __float2half_rn(s) : __ushort_as_half(0x7fff);
+            } else {
+                bad = true;
+            }
         }
     }
     if (bad) atomicExch(&g_sfb_device_error, SFB_ERR_RANGE);
+}
+
+// Four half2 (values 0 1, 2 3, 4 5, 6 7) as 8 values of the output type.
+__device__ __forceinline__ void store_halves(__half* p, const uint32_t (&h)[4]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
+}
+template <typename T>
+__device__ __forceinline__ void store_halves(T* p, const uint32_t (&h)[4]) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(u2h(h[i]));
+        x[2 * i] = f.x; x[2 * i + 1] = f.y;
+    }
+    nrope::store8(p, x);
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(const Kv4MoveParams p) {
     pdl_trigger();
     pdl_wait();
-    constexpr int kLanes = D / 8;
+    constexpr int kLanes = D / 8, kTok = 32 / kLanes;
     const Where r = where<D>(p);
     const int sub = threadIdx.x % kLanes;
-    const bool is_v = r.hh >= p.c.Hkv;
-    const int h = is_v ? r.hh - p.c.Hkv : r.hh;
-    T* out = static_cast<T*>(is_v ? p.v : p.k);
+    T* out = static_cast<T*>(r.is_v ? p.v : p.k);
     if (!r.ok || out == nullptr) return;
-    const int64_t slot = static_cast<int64_t>(p.slot0) + r.tok;
-    const uint8_t* codes = (is_v ? p.c.vc : p.c.kc) + r.b * p.c.code_sb + h * p.c.code_sh + slot * (D / 2);
-    const __half* sc = (is_v ? p.c.vs : p.c.ks) + r.b * p.c.sc_sb + h * p.c.sc_sh + slot * (D / kGroup);
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + sub * 4);
-    const float s = __half2float(sc[sub >> 2]);
-    float x[8];
+    const int64_t slot0 = static_cast<int64_t>(p.slot0) + r.tok;
+    const int64_t sb = r.is_v ? p.v_st[0] : p.k_st[0], sh = r.is_v ? p.v_st[1] : p.k_st[1], ss = r.is_v ? p.v_st[2] : p.k_st[2];
+    const uint8_t* codes = (r.is_v ? p.c.vc : p.c.kc) + r.b * p.c.code_sb + r.h * p.c.code_sh + slot0 * (D / 2) + sub * 4;
+    const __half* sc = (r.is_v ? p.c.vs : p.c.ks) + r.b * p.c.sc_sb + r.h * p.c.sc_sh + slot0 * (D / kGroup) + (sub >> 2);
+    out += r.b * sb + r.h * sh + r.tok * ss + sub * 8;
+    uint32_t word[kRuns];
+    __half s[kRuns];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        x[i] = static_cast<float>(static_cast<int>((word >> nibble_shift(i)) & 15u) - 8) * s;
-    const int64_t* st = is_v ? p.v_st : p.k_st;
-    nrope::store8(out + r.b * st[0] + h * st[1] + r.tok * st[2] + sub * 8, x);
+    for (int u = 0; u < kRuns; ++u) {
+        if (r.tok + u * kTok < p.seq) {
+            word[u] = *reinterpret_cast<const uint32_t*>(codes + u * kTok * (D / 2));
+            s[u] = sc[u * kTok * (D / kGroup)];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kRuns; ++u) {
+        if (r.tok + u * kTok >= p.seq) break;
+        uint32_t h[4];
+        dequant_word(word[u], __half2half2(s[u]), h);        // exact
+        store_halves(out + u * kTok * ss, h);
+    }
 }
 
 template <typename T>
 int launch_move(Kv4MoveParams& p, bool append, cudaStream_t s) {
     const int tok = 32 / (p.c.D / 8);
-    p.tgroups = static_cast<int32_t>((static_cast<int64_t>(p.seq) + tok - 1) / tok);
+    p.tgroups = static_cast<int32_t>((static_cast<int64_t>(p.seq) + tok * kRuns - 1) / (tok * kRuns));
     const int64_t warps = static_cast<int64_t>(p.c.B) * p.tgroups * 2 * p.c.Hkv;
     if (static_cast<int64_t>(p.c.B) * p.tgroups > 0x7fffffff || warps > 0xffffff00ll) return SFB_ERR_SHAPE;
     p.warps = static_cast<uint32_t>(warps);

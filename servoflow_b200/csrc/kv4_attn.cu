@@ -70,28 +70,6 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-// (x & mask) | 0x64006400 in one LOP3
-template <uint32_t kMask>
-__device__ __forceinline__ uint32_t nib_magic(uint32_t x) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "n"(kMask), "n"(0x64006400u));
-    return r;
-}
-__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-
-// The eight codes of a word as four half2 times s: o[i] = (nibble at 4i, nibble at 16 + 4i).
-__device__ __forceinline__ void dequant_word(uint32_t w, __half2 s, uint32_t (&o)[4]) {
-    const __half2 k1032 = __half2half2(__ushort_as_half(0x6408));           // 1024 + 8
-    const __half2 k16 = __half2half2(__ushort_as_half(0x2c00));             // 1 / 16
-    const __half2 k72 = __half2half2(__ushort_as_half(0xd480));             // −(64 + 8)
-    const uint32_t w8 = w >> 8;
-    o[0] = h2u(__hmul2(__hsub2(u2h(nib_magic<0x000f000fu>(w)), k1032), s));
-    o[1] = h2u(__hmul2(__hfma2(u2h(nib_magic<0x00f000f0u>(w)), k16, k72), s));
-    o[2] = h2u(__hmul2(__hsub2(u2h(nib_magic<0x000f000fu>(w8)), k1032), s));
-    o[3] = h2u(__hmul2(__hfma2(u2h(nib_magic<0x00f000f0u>(w8)), k16, k72), s));
-}
-
 template <int D> struct KWords;
 template <> struct KWords<64>  { using T = uint2; };
 template <> struct KWords<128> { using T = uint4; };

@@ -31,7 +31,7 @@ struct NormRopeParams {
     int32_t table_len, S, H, Hkv, D, rot, norm;
     int32_t chunks;                                   // threads (of a head's lane) per token
     uint32_t tokens;
-    float eps;
+    float eps, inv_d;                                 // 1 / D
 };
 
 namespace nrope {
@@ -144,7 +144,7 @@ norm_rope_kernel(const NormRopeParams p) {
             for (int i = 0; i < 4; ++i) ss = fmaf(f[2 * i], f[2 * i], fmaf(f[2 * i + 1], f[2 * i + 1], ss));
 #pragma unroll
             for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = 1.f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
+            const float inv = rsqrtf(fmaf(ss, p.inv_d, p.eps));
             const bool is_q = h < p.H;
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * (is_q ? gq[i] : gk[i]);
@@ -238,7 +238,7 @@ int qk_norm_rope_launch(const sfb_norm_rope_args& a, cudaStream_t s) {
     p.pos = a.positions; p.pos_sb = a.pos_stride_b;
     p.table_len = a.table_len;
     p.S = a.seq; p.H = H; p.Hkv = Hkv; p.D = a.head_dim; p.rot = a.rotary_dim;
-    p.norm = a.norm ? 1 : 0; p.eps = a.eps;
+    p.norm = a.norm ? 1 : 0; p.eps = a.eps; p.inv_d = 1.f / static_cast<float>(a.head_dim);
     const int64_t tokens = static_cast<int64_t>(a.batch) * a.seq;
     if (tokens > 0x7fffffff) return SFB_ERR_SHAPE;
     p.tokens = static_cast<uint32_t>(tokens);
