@@ -35,7 +35,7 @@ struct Kv4MoveParams {
     int32_t seq, slot0;
     const int32_t *start, *len;
     uint32_t warps;
-    int32_t tgroups;               // token groups per session
+    FastDiv tgroups, heads2;       // token groups per session, K and V heads
 };
 
 namespace kv4 {
@@ -75,13 +75,13 @@ template <int D>
 __device__ __forceinline__ Where where(const Kv4MoveParams& p) {
     constexpr int kLanes = D / 8, kTok = 32 / kLanes;
     const uint32_t w = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5);
-    const uint32_t heads2 = 2 * p.c.Hkv, wt = w / heads2, hh = w - wt * heads2;
+    const uint32_t wt = p.heads2.div(w), hh = w - wt * p.heads2.d;
     Where r;
     r.ok = w < p.warps;
     r.is_v = hh >= static_cast<uint32_t>(p.c.Hkv);
     r.h = static_cast<int>(hh) - (r.is_v ? p.c.Hkv : 0);
-    r.b = static_cast<int>(wt / static_cast<uint32_t>(p.tgroups));
-    r.tok = static_cast<int>(wt - r.b * p.tgroups) * (kTok * kRuns) + (threadIdx.x & 31) / kLanes;
+    r.b = static_cast<int>(p.tgroups.div(wt));
+    r.tok = static_cast<int>(wt - r.b * p.tgroups.d) * (kTok * kRuns) + (threadIdx.x & 31) / kLanes;
     return r;
 }
 
@@ -208,9 +208,11 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(const Kv4MovePar
 template <typename T>
 int launch_move(Kv4MoveParams& p, bool append, cudaStream_t s) {
     const int tok = 32 / (p.c.D / 8);
-    p.tgroups = static_cast<int32_t>((static_cast<int64_t>(p.seq) + tok * kRuns - 1) / (tok * kRuns));
-    const int64_t warps = static_cast<int64_t>(p.c.B) * p.tgroups * 2 * p.c.Hkv;
-    if (static_cast<int64_t>(p.c.B) * p.tgroups > 0x7fffffff || warps > 0xffffff00ll) return SFB_ERR_SHAPE;
+    const int64_t groups = (static_cast<int64_t>(p.seq) + tok * kRuns - 1) / (tok * kRuns);
+    const int64_t warps = static_cast<int64_t>(p.c.B) * groups * 2 * p.c.Hkv;
+    if (p.c.Hkv > 0x3fffffff || p.c.B * groups > 0x7fffff00ll || warps > 0x7fffff00ll) return SFB_ERR_SHAPE;
+    p.tgroups.set(static_cast<uint32_t>(groups));
+    p.heads2.set(static_cast<uint32_t>(2 * p.c.Hkv));
     p.warps = static_cast<uint32_t>(warps);
     const int64_t blocks = (warps * 32 + kMoveThreads - 1) / kMoveThreads;
     auto kern = p.c.D == 64 ? (append ? kv4_append_kernel<T, 64> : kv4_read_kernel<T, 64>)

@@ -8,35 +8,53 @@
 // (qk-norm, src/models/rdt1b/dit_block.cu:185-196 → norm.cuh:89-122) are one
 // here: fp32 from the load to the single rounding of the store.
 //
-// Bound: bytes (each value read once and written once). A head is held by
-// D / 8 lanes, 8 values (one 16-byte load of a 16-bit type) each, so the mean
-// is log2(lanes) shuffles, and the rotation's partner value of the half-split
-// form is one shuffle away (pairs (i, i + rot/2) with rot % 16 == 0 keep the
-// same slot of another lane; the interleaved form's partner is in the lane).
-// A thread takes up to kHeads heads of one token: they share the token's
-// cos / sin values, whose loads would otherwise be four times the data's
-// (8 + 8 fp32 values per 8 16-bit ones).
+// Bound: bytes (each value read once and written once), if few instructions go
+// with them. A head is held by D / 8 lanes, 8 values (one 16-byte load of a
+// 16-bit type) each, so the mean is log2(lanes) shuffles, and the rotation's
+// partner value of the half-split form is one shuffle away (pairs (i, i + rot/2)
+// with rot % 16 == 0 keep the same slot of another lane; the interleaved form's
+// partner is in the lane). A thread takes kHeads neighbouring heads of one token:
+// they share its position's cos / sin values (8 + 8 fp32 loads beside 8 16-bit
+// ones) and the index arithmetic. Blocks of q come before blocks of k, so that
+// which of the two a thread works on costs nothing per head.
 #include "common.cuh"
 
 namespace sfb {
 
+// Division of n < 2^31 by a constant (Granlund and Montgomery, 1994).
+struct FastDiv {
+    uint32_t mul, shift, d;
+    void set(uint32_t x) {
+        d = x; shift = 0;
+        while ((1u << shift) < x) ++shift;
+        mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - x)) / x + 1);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
+struct NormRopeSide {
+    const void* x;
+    void* out;
+    const void* w;
+    int64_t st[3], so[3];                             // element strides: batch, head, seq
+    int32_t heads;
+    FastDiv chunks;                                   // groups of kHeads heads
+};
+
 struct NormRopeParams {
-    const void *q, *k;
-    void *q_out, *k_out;
-    int64_t q_st[3], qo_st[3], k_st[3], ko_st[3];     // element strides: batch, head, seq
-    const void *q_w, *k_w;
+    NormRopeSide side[2];                             // q, k
     const float *cos_t, *sin_t;
     const int32_t* pos;
     int64_t pos_sb;
-    int32_t table_len, S, H, Hkv, D, rot, norm;
-    int32_t chunks;                                   // threads (of a head's lane) per token
-    uint32_t tokens;
+    FastDiv S;
+    int32_t table_len, D, rot, norm;
+    uint32_t tokens, blocks_q;
     float eps, inv_d;                                 // 1 / D
 };
 
 namespace nrope {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
     const uint4 u = *reinterpret_cast<const uint4*>(p);
@@ -73,70 +91,67 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
     *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
 }
 
-// kLanes: lanes per head (8, 16 or 32; D / 8 of them hold values);
-// kHeads: heads per thread; kInter: pairs (2i, 2i+1) instead of (i, i + rot/2).
-template <typename T, int kLanes, int kHeads, bool kInter>
+// kLanes: lanes per head (8, 16 or 32; D / 8 of them hold values); kHeads: heads
+// per thread; kRot: 0 no rotation, 1 pairs (i, i + rot/2), 2 pairs (2i, 2i+1).
+template <typename T, int kLanes, int kHeads, int kRot>
 __global__ void __launch_bounds__(kThreads)
 norm_rope_kernel(const NormRopeParams p) {
     pdl_trigger();
-    pdl_wait();
-    const uint32_t unit = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-    const int sub = threadIdx.x % kLanes;
-    const uint32_t tok = unit / static_cast<uint32_t>(p.chunks);
-    const int chunk = static_cast<int>(unit - tok * p.chunks);
+    const bool is_k = blockIdx.x >= p.blocks_q;
+    const NormRopeSide& sd = p.side[is_k ? 1 : 0];
+    const uint32_t unit = (blockIdx.x - (is_k ? p.blocks_q : 0)) * (kThreads / kLanes) + threadIdx.x / kLanes;
+    const int d0 = (threadIdx.x % kLanes) * 8;
+    const uint32_t tok = sd.chunks.div(unit), h0 = (unit - tok * sd.chunks.d) * kHeads;
     const bool in_range = tok < p.tokens;             // whole warps take the shuffles below
-    const uint32_t bi = in_range ? tok / static_cast<uint32_t>(p.S) : 0;
-    const int64_t b = bi, s = in_range ? tok - bi * p.S : 0;
-    const int64_t pos = in_range && p.rot > 0 && p.pos != nullptr ? p.pos[b * p.pos_sb + s] : s;
-    const int d0 = sub * 8;
+    const uint32_t b = p.S.div(in_range ? tok : 0), s = (in_range ? tok : 0) - b * p.S.d;
     const bool act = in_range && d0 < p.D;
-    const int heads = p.H + p.Hkv;
-
+    const int nh = act ? min(kHeads, sd.heads - static_cast<int>(h0)) : 0;
+    const int64_t hs = sd.st[1], ho = sd.so[1];
+    const T* src = static_cast<const T*>(sd.x) + b * sd.st[0] + h0 * hs + s * sd.st[2] + d0;
+    pdl_wait();
+    const int64_t pos = kRot != 0 && p.pos != nullptr ? p.pos[b * p.pos_sb + s] : static_cast<int64_t>(s);
     float x[kHeads][8];
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
-        const int h = chunk + j * p.chunks;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
-        if (act && h < heads) {
-            const T* src = h < p.H
-                ? static_cast<const T*>(p.q) + b * p.q_st[0] + h * p.q_st[1] + s * p.q_st[2]
-                : static_cast<const T*>(p.k) + b * p.k_st[0] + (h - p.H) * p.k_st[1] + s * p.k_st[2];
-            load8(src + d0, x[j]);
-        }
+        if (j < nh) load8(src + j * hs, x[j]);
     }
-    // the weights of this lane's channels (q's and k's differ only by head)
-    float gq[8], gk[8];
+    float g[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) gq[i] = gk[i] = 1.f;
-    if (p.norm && act) {
-        if (p.q_w != nullptr && chunk < p.H) load8(static_cast<const T*>(p.q_w) + d0, gq);
-        if (p.k_w != nullptr && chunk + (kHeads - 1) * p.chunks >= p.H) load8(static_cast<const T*>(p.k_w) + d0, gk);
-    }
-    // the token's angles: 8 (half-split) or 4 (interleaved) pairs for this lane
+    for (int i = 0; i < 8; ++i) g[i] = 1.f;
+    if (sd.w != nullptr && act) load8(static_cast<const T*>(sd.w) + d0, g);
+    // the token's angles: 8 (half-split) or 4 (interleaved) pairs for this lane;
+    // cosine 1 and sine 0 past the rotated channels
     float c[8], sn[8];
     bool bad = false;
-    const bool rotates = p.rot > 0 && d0 < p.rot;
-    if (p.rot > 0 && in_range) {
+    const bool first = d0 < p.rot / 2;
+    if constexpr (kRot != 0) {
         bad = pos < 0 || pos >= p.table_len;
-        if (rotates && !bad) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { c[i] = 1.f; sn[i] = 0.f; }
+        if (d0 < p.rot && !bad) {
             const int64_t base = pos * (p.rot / 2);
-            if constexpr (kInter) {
+            if constexpr (kRot == 2) {
                 const float4 cc = *reinterpret_cast<const float4*>(p.cos_t + base + d0 / 2);
                 const float4 ss = *reinterpret_cast<const float4*>(p.sin_t + base + d0 / 2);
                 c[0] = cc.x; c[1] = cc.y; c[2] = cc.z; c[3] = cc.w;
                 sn[0] = ss.x; sn[1] = ss.y; sn[2] = ss.z; sn[3] = ss.w;
             } else {
-                const int i0 = d0 < p.rot / 2 ? d0 : d0 - p.rot / 2;
+                const int i0 = first ? d0 : d0 - p.rot / 2;
                 load8(p.cos_t + base + i0, c);
                 load8(p.sin_t + base + i0, sn);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sn[i] = first ? -sn[i] : sn[i];      // a·cos − b·sin, b·cos + a·sin
             }
         }
     }
+    // the lane of the pair's other half (this one where nothing is rotated)
+    const int lane = threadIdx.x & 31, hop = p.rot / 16;
+    const int peer = d0 < p.rot ? (first ? lane + hop : lane - hop) : lane;
+    T* dst = static_cast<T*>(sd.out) + b * sd.so[0] + h0 * ho + s * sd.so[2] + d0;
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
-        const int h = chunk + j * p.chunks;
-        const bool have = act && h < heads;
         float (&f)[8] = x[j];
         if (p.norm) {
             float ss = 0.f;
@@ -145,65 +160,63 @@ norm_rope_kernel(const NormRopeParams p) {
 #pragma unroll
             for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             const float inv = rsqrtf(fmaf(ss, p.inv_d, p.eps));
-            const bool is_q = h < p.H;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * (is_q ? gq[i] : gk[i]);
+            for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * g[i];
         }
-        if (p.rot > 0) {
-            if constexpr (kInter) {
-                if (rotates && !bad) {
+        if constexpr (kRot == 2) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float a = f[2 * i], bb = f[2 * i + 1];
-                        f[2 * i]     = a * c[i] - bb * sn[i];
-                        f[2 * i + 1] = bb * c[i] + a * sn[i];
-                    }
-                }
-            } else {
-                const bool first = d0 < p.rot / 2;
-                const int lane = threadIdx.x & 31, hop = p.rot / 16;
-                const int peer = rotates ? (first ? lane + hop : lane - hop) : lane;
+            for (int i = 0; i < 4; ++i) {
+                const float a = f[2 * i], bb = f[2 * i + 1];
+                f[2 * i]     = a * c[i] - bb * sn[i];
+                f[2 * i + 1] = bb * c[i] + a * sn[i];
+            }
+        } else if constexpr (kRot == 1) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float o = __shfl_sync(0xffffffffu, f[i], peer);
-                    if (rotates && !bad) f[i] = first ? f[i] * c[i] - o * sn[i] : f[i] * c[i] + o * sn[i];
-                }
+            for (int i = 0; i < 8; ++i) {
+                const float o = __shfl_sync(0xffffffffu, f[i], peer);
+                f[i] = f[i] * c[i] + o * sn[i];
             }
         }
-        if (have && !bad) {
-            T* dst = h < p.H
-                ? static_cast<T*>(p.q_out) + b * p.qo_st[0] + h * p.qo_st[1] + s * p.qo_st[2]
-                : static_cast<T*>(p.k_out) + b * p.ko_st[0] + (h - p.H) * p.ko_st[1] + s * p.ko_st[2];
-            store8(dst + d0, f);
-        }
+        if (j < nh && !bad) store8(dst + j * ho, f);
     }
-    if (bad) atomicExch(&g_sfb_device_error, SFB_ERR_RANGE);
+    if (kRot != 0 && act && bad) atomicExch(&g_sfb_device_error, SFB_ERR_RANGE);
 }
 
-template <typename T, int kLanes, bool kInter>
+template <typename T, int kLanes, int kHeads, int kRot>
 int launch(NormRopeParams& p, cudaStream_t s) {
-    // Four heads per thread once that still leaves half the GPU's threads busy:
-    // four loads in flight each, the angles' loads a quarter. One head per
-    // thread below that, where a call is latency.
-    const int heads = p.H + p.Hkv;
-    const int64_t one = static_cast<int64_t>(p.tokens) * heads * kLanes;
-    const bool many = one >= static_cast<int64_t>(std::max(device_info().num_sms, 1)) * 1024 * 4;
-    const int per = many ? 4 : 1;
-    p.chunks = (heads + per - 1) / per;
-    const int64_t units = static_cast<int64_t>(p.tokens) * p.chunks, blocks = (units * kLanes + kThreads - 1) / kThreads;
-    if (units > 0xffffff00ll || blocks > 0x7fffffff) return SFB_ERR_SHAPE;
-    auto kern = many ? norm_rope_kernel<T, kLanes, 4, kInter> : norm_rope_kernel<T, kLanes, 1, kInter>;
+    int64_t blocks[2];
+    for (int i = 0; i < 2; ++i) {
+        NormRopeSide& sd = p.side[i];
+        const uint32_t chunks = static_cast<uint32_t>((sd.heads + kHeads - 1) / kHeads);
+        const int64_t units = static_cast<int64_t>(p.tokens) * chunks;
+        if (units >= 0x7fffff00ll) return SFB_ERR_SHAPE;
+        sd.chunks.set(std::max(chunks, 1u));
+        blocks[i] = (units * kLanes + kThreads - 1) / kThreads;
+    }
+    if (blocks[0] + blocks[1] > 0x7fffffff) return SFB_ERR_SHAPE;
+    p.blocks_q = static_cast<uint32_t>(blocks[0]);
+    auto kern = norm_rope_kernel<T, kLanes, kHeads, kRot>;
     prefer_max_shared(kern);
-    return launch_kernel(kern, static_cast<unsigned>(blocks), kThreads, 0, s, true, p);
+    return launch_kernel(kern, static_cast<unsigned>(blocks[0] + blocks[1]), kThreads, 0, s, true, p);
+}
+
+template <typename T, int kLanes>
+int pick_rot(NormRopeParams& p, bool inter, cudaStream_t s) {
+    // Four heads per thread once that still leaves half the GPU's threads busy:
+    // four loads in flight each, the angles' loads and the index arithmetic a
+    // quarter. One head per thread below that, where a call is latency.
+    const int64_t one = static_cast<int64_t>(p.tokens) * (p.side[0].heads + p.side[1].heads) * kLanes;
+    const bool many = one >= static_cast<int64_t>(std::max(device_info().num_sms, 1)) * 1024 * 4;
+    if (p.rot == 0) return many ? launch<T, kLanes, 4, 0>(p, s) : launch<T, kLanes, 1, 0>(p, s);
+    if (inter) return many ? launch<T, kLanes, 4, 2>(p, s) : launch<T, kLanes, 1, 2>(p, s);
+    return many ? launch<T, kLanes, 4, 1>(p, s) : launch<T, kLanes, 1, 1>(p, s);
 }
 
 template <typename T>
 int pick(NormRopeParams& p, bool inter, cudaStream_t s) {
-    if (p.D <= 64)
-        return inter ? launch<T, 8, true>(p, s) : launch<T, 8, false>(p, s);
-    if (p.D <= 128)
-        return inter ? launch<T, 16, true>(p, s) : launch<T, 16, false>(p, s);
-    return inter ? launch<T, 32, true>(p, s) : launch<T, 32, false>(p, s);
+    if (p.D <= 64) return pick_rot<T, 8>(p, inter, s);
+    if (p.D <= 128) return pick_rot<T, 16>(p, inter, s);
+    return pick_rot<T, 32>(p, inter, s);
 }
 
 }  // namespace nrope
@@ -228,19 +241,20 @@ int qk_norm_rope_launch(const sfb_norm_rope_args& a, cudaStream_t s) {
     if (!al(a.q_weight) || !al(a.k_weight) || !al(a.cos_table) || !al(a.sin_table)) return SFB_ERR_ALIGN;
     if (!is_sm100(device_info())) return SFB_ERR_UNSUPPORTED;
     NormRopeParams p{};
-    p.q = a.q; p.k = a.k; p.q_out = a.q_out; p.k_out = a.k_out;
+    NormRopeSide &q = p.side[0], &k = p.side[1];
+    q.x = a.q; q.out = a.q_out; q.w = a.q_weight; q.heads = H;
+    k.x = a.k; k.out = a.k_out; k.w = a.k_weight; k.heads = Hkv;
     for (int i = 0; i < 3; ++i) {
-        p.q_st[i] = a.q_stride[i]; p.qo_st[i] = a.q_out_stride[i];
-        p.k_st[i] = a.k_stride[i]; p.ko_st[i] = a.k_out_stride[i];
+        q.st[i] = a.q_stride[i]; q.so[i] = a.q_out_stride[i];
+        k.st[i] = a.k_stride[i]; k.so[i] = a.k_out_stride[i];
     }
-    p.q_w = a.q_weight; p.k_w = a.k_weight;
     p.cos_t = a.cos_table; p.sin_t = a.sin_table;
     p.pos = a.positions; p.pos_sb = a.pos_stride_b;
     p.table_len = a.table_len;
-    p.S = a.seq; p.H = H; p.Hkv = Hkv; p.D = a.head_dim; p.rot = a.rotary_dim;
+    p.S.set(static_cast<uint32_t>(a.seq)); p.D = a.head_dim; p.rot = a.rotary_dim;
     p.norm = a.norm ? 1 : 0; p.eps = a.eps; p.inv_d = 1.f / static_cast<float>(a.head_dim);
     const int64_t tokens = static_cast<int64_t>(a.batch) * a.seq;
-    if (tokens > 0x7fffffff) return SFB_ERR_SHAPE;
+    if (tokens > 0x7fffff00ll) return SFB_ERR_SHAPE;
     p.tokens = static_cast<uint32_t>(tokens);
     const bool inter = a.interleaved != 0;
     if (a.dtype == SFB_BF16) return nrope::pick<__nv_bfloat16>(p, inter, s);
