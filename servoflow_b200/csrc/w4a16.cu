@@ -13,8 +13,14 @@
 // exact in fp32; a group's sum is scaled in fp32 and added to the row's: no
 // rounding to 16 bits anywhere before the output.
 //
-// A CTA takes 16 output channels and up to 8·NT rows of X; its warps take the
-// groups in turn and are joined in shared memory.
+// Two kernels. Up to 16 rows are bound by the weights' bytes, if few instructions
+// go with them (a 1 KB chunk of 16 channels is 96 for the codes and MMAs alone): a
+// CTA takes 16 or 32 channels, its eight warps chunks of 128 inputs by turns, with
+// everything of a warp's next chunk (codes, scales, X) in flight while it works on
+// one, in two sets of registers by turns. More rows are bound by X, which every
+// CTA reads from L2: a CTA takes 64 channels (32 when those are too few CTAs) and
+// 8·NT rows, X goes through a ring of shared memory that the warps of the channel
+// tiles share, and the warps left over split the inputs.
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 
@@ -35,6 +41,14 @@ namespace w4 {
 
 constexpr int kWarps = 8;
 
+// (x & 0x000f000f) | kMagic in one LOP3 (two constants: the compiler takes two)
+template <uint32_t kMagic>
+__device__ __forceinline__ uint32_t nib_or(uint32_t x) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "n"(0x000f000fu), "n"(kMagic));
+    return r;
+}
+
 template <typename T> struct Ops;
 template <> struct Ops<__nv_bfloat16> {
     static __device__ __forceinline__ float to_f(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -43,17 +57,24 @@ template <> struct Ops<__nv_bfloat16> {
         const __nv_bfloat162 k136 = __bfloat162bfloat162(__ushort_as_bfloat16(0x4308));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+            const uint32_t u = nib_or<0x43004300u>(w >> (4 * i));
             const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), k136);
             o[i] = *reinterpret_cast<const uint32_t*>(&v);
         }
     }
     static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                      "{%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
     }
 };
 template <> struct Ops<__half> {
@@ -63,7 +84,7 @@ template <> struct Ops<__half> {
         const __half2 k1032 = __half2half2(__ushort_as_half(0x6408));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+            const uint32_t u = nib_or<0x64006400u>(w >> (4 * i));
             const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), k1032);
             o[i] = *reinterpret_cast<const uint32_t*>(&v);
         }
@@ -72,12 +93,14 @@ template <> struct Ops<__half> {
                                                uint32_t b0, uint32_t b1) {
         kv4::mma16816(c, a0, a1, a2, a3, b0, b1);
     }
+    static __device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    }
 };
-
-template <int kWords> struct WordsOf;
-template <> struct WordsOf<1> { using T = uint32_t; };
-template <> struct WordsOf<2> { using T = uint2; };
-template <> struct WordsOf<4> { using T = uint4; };
 
 __device__ __forceinline__ float scale_at(const void* s, int dt, int64_t i) {
     if (dt == SFB_F16) return __half2float(static_cast<const __half*>(s)[i]);
@@ -85,106 +108,353 @@ __device__ __forceinline__ float scale_at(const void* s, int dt, int64_t i) {
     return static_cast<const float*>(s)[i];
 }
 
-// G: group; NT: tiles of 8 rows of X; kAct as sfb_w4a16_linear.
-template <typename T, int G, int NT>
-__global__ void __launch_bounds__(kWarps * 32) w4a16_kernel(const W4Params p, const int act) {
-    using O = Ops<T>;
-    constexpr int kWords = G / 32;                 // 32-bit words of codes per lane and channel
-    using Words = typename WordsOf<kWords>::T;
-    __shared__ float red[kWarps][16][NT * 8 + 1];
-    pdl_trigger();
-    pdl_wait();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (NT * 8);
-    const int na = min(n0 + g, p.N - 1), nb = min(n0 + g + 8, p.N - 1);   // past the last channel: not stored
-    const uint8_t* wa = p.w + static_cast<int64_t>(na) * (p.K / 2) + t * (G / 8);
-    const uint8_t* wb = p.w + static_cast<int64_t>(nb) * (p.K / 2) + t * (G / 8);
-    const T* x = static_cast<const T*>(p.x);
+constexpr int kChunk = 128;                        // inputs of a chunk
+constexpr int kThreads = kWarps * 32;
 
-    float acc[NT][4];
+// A lane's codes of a chunk are four words of 8. Inside a chunk the inputs are
+// dealt out in blocks of 64 (of 32 for groups of 32): lane t has a quarter of each
+// block, word w of the four belongs to block w / kQ. Groups are whole blocks.
+__host__ __device__ constexpr int block_of(int G) { return G < 64 ? 32 : 64; }
+
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, int bytes_in, int size_) {
+    // size_ bytes, of which bytes_in are read and the rest zeros
+    if (size_ == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes_in) : "memory");
+    else if (size_ == 8)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes_in) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes_in) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// The join and the epilogue. red: [parts][channels][rows + 1] fp32 sums. A thread
+// keeps one channel; its bias and residuals are loaded (`before`) ahead of the
+// barrier that the sums wait for.
+template <typename T, int kChannels, int kRows, int kThr, int kPartSums>
+struct Epilogue {
+    static constexpr int kStep = kThr / kChannels, kIt = (kRows + kStep - 1) / kStep;
+    static_assert(kThr % kChannels == 0, "a thread keeps its channel");
+    int nn, mm0, m0;
+    float bias, res[kIt];
+
+    __device__ __forceinline__ void before(const W4Params& p, int n0, int m0_) {
+        using O = Ops<T>;
+        nn = n0 + threadIdx.x % kChannels;
+        mm0 = threadIdx.x / kChannels;
+        m0 = m0_;
+        bias = p.bias != nullptr && nn < p.N ? O::to_f(static_cast<const T*>(p.bias) + nn) : 0.f;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-    Words ra{}, rb{};
-    if (warp < p.groups) {
-        ra = *reinterpret_cast<const Words*>(wa + static_cast<int64_t>(warp) * (G / 2));
-        rb = *reinterpret_cast<const Words*>(wb + static_cast<int64_t>(warp) * (G / 2));
+        for (int i = 0; i < kIt; ++i) {
+            const int mm = mm0 + i * kStep;
+            const int64_t m = m0 + mm;
+            res[i] = 0.f;
+            if (p.residual != nullptr && nn < p.N && mm < kRows && m < p.M)
+                res[i] = p.y_f32 ? static_cast<const float*>(p.residual)[m * p.ldr + nn]
+                                 : O::to_f(static_cast<const T*>(p.residual) + m * p.ldr + nn);
+        }
     }
-    for (int c = warp; c < p.groups; c += kWarps) {
-        const Words ca = ra, cb = rb;
-        if (c + kWarps < p.groups) {
-            ra = *reinterpret_cast<const Words*>(wa + static_cast<int64_t>(c + kWarps) * (G / 2));
-            rb = *reinterpret_cast<const Words*>(wb + static_cast<int64_t>(c + kWarps) * (G / 2));
-        }
-        const float sa = scale_at(p.scale, p.scale_dtype, static_cast<int64_t>(na) * p.groups + c);
-        const float sb = scale_at(p.scale, p.scale_dtype, static_cast<int64_t>(nb) * p.groups + c);
-        float part[NT][4];
+    __device__ __forceinline__ void after(const W4Params& p, int act, const float* red) {
+        if (nn >= p.N) return;
+        const int ch = threadIdx.x % kChannels;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.f;
+        for (int i = 0; i < kIt; ++i) {
+            const int mm = mm0 + i * kStep;
+            const int64_t m = m0 + mm;
+            if (mm >= kRows || m >= p.M) break;
+            float v = bias;
 #pragma unroll
-        for (int q = 0; q < kWords; ++q) {         // 8 codes of a lane: two MMA steps
-            uint32_t fa[4], fb[4];
-            O::codes(reinterpret_cast<const uint32_t*>(&ca)[q], fa);
-            O::codes(reinterpret_cast<const uint32_t*>(&cb)[q], fb);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int m = m0 + j * 8 + g;
-                uint4 xv = make_uint4(0, 0, 0, 0);
-                if (m < p.M)
-                    xv = *reinterpret_cast<const uint4*>(x + m * p.ldx + static_cast<int64_t>(c) * G + t * (G / 4) + q * 8);
-                O::mma(part[j], fa[0], fb[0], fa[1], fb[1], xv.x, xv.y);
-                O::mma(part[j], fa[2], fb[2], fa[3], fb[3], xv.z, xv.w);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            acc[j][0] = fmaf(sa, part[j][0], acc[j][0]);
-            acc[j][1] = fmaf(sa, part[j][1], acc[j][1]);
-            acc[j][2] = fmaf(sb, part[j][2], acc[j][2]);
-            acc[j][3] = fmaf(sb, part[j][3], acc[j][3]);
+            for (int w = 0; w < kPartSums; ++w) v += red[(w * kChannels + ch) * (kRows + 1) + mm];
+            if (act == 1) v = w8::gelu_tanh(v);
+            else if (act == 2) v = v / (1.f + expf(-v));
+            v += res[i];
+            if (p.y_f32) static_cast<float*>(p.y)[m * p.ldy + nn] = v;
+            else static_cast<T*>(p.y)[m * p.ldy + nn] = Ops<T>::from_f(v);
         }
     }
+};
+
+// part (+)= one word's products for every tile of 8 rows; the first word of a
+// group starts the sums.
+template <typename T, int NT>
+__device__ __forceinline__ void word_mma(float (&part)[NT][4], uint32_t wa, uint32_t wb, const uint4 (&x)[NT], bool first) {
+    using O = Ops<T>;
+    uint32_t fa[4], fb[4];
+    O::codes(wa, fa);
+    O::codes(wb, fb);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        red[warp][g][j * 8 + 2 * t] = acc[j][0];
-        red[warp][g][j * 8 + 2 * t + 1] = acc[j][1];
-        red[warp][g + 8][j * 8 + 2 * t] = acc[j][2];
-        red[warp][g + 8][j * 8 + 2 * t + 1] = acc[j][3];
+        if (first) O::mma0(part[j], fa[0], fb[0], fa[1], fb[1], x[j].x, x[j].y);
+        else O::mma(part[j], fa[0], fb[0], fa[1], fb[1], x[j].x, x[j].y);
+        O::mma(part[j], fa[2], fb[2], fa[3], fb[3], x[j].z, x[j].w);
     }
-    __syncthreads();
-    for (int i = tid; i < 16 * NT * 8; i += kWarps * 32) {
-        const int ch = i & 15, mm = i >> 4, nn = n0 + ch, m = m0 + mm;
-        if (nn >= p.N || m >= p.M) continue;
-        float v = 0.f;
+}
+template <int NT>
+__device__ __forceinline__ void zero(float (&v)[NT][4]) {
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) v += red[w][ch][mm];
-        if (p.bias != nullptr) v += O::to_f(static_cast<const T*>(p.bias) + nn);
-        if (act == 1) v = w8::gelu_tanh(v);
-        else if (act == 2) v = v / (1.f + expf(-v));
-        if (p.y_f32) {
-            if (p.residual != nullptr) v += static_cast<const float*>(p.residual)[m * p.ldr + nn];
-            static_cast<float*>(p.y)[m * p.ldy + nn] = v;
-        } else {
-            if (p.residual != nullptr) v += O::to_f(static_cast<const T*>(p.residual) + m * p.ldr + nn);
-            static_cast<T*>(p.y)[m * p.ldy + nn] = O::from_f(v);
-        }
+    for (int j = 0; j < NT; ++j) v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.f;
+}
+template <int NT>
+__device__ __forceinline__ void add_scaled(float (&acc)[NT][4], const float (&part)[NT][4], float sa, float sb) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        acc[j][0] = fmaf(sa, part[j][0], acc[j][0]);
+        acc[j][1] = fmaf(sa, part[j][1], acc[j][1]);
+        acc[j][2] = fmaf(sb, part[j][2], acc[j][2]);
+        acc[j][3] = fmaf(sb, part[j][3], acc[j][3]);
+    }
+}
+// This lane's part of the 16-channel tile at rows [0, 16) of dst, row stride kRow.
+template <int NT>
+__device__ __forceinline__ void put_acc(float* dst, int kRow, const float (&acc)[NT][4], int g, int t) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        float* d = dst + g * kRow + j * 8 + 2 * t;
+        d[0] = acc[j][0];
+        d[1] = acc[j][1];
+        d[8 * kRow] = acc[j][2];
+        d[8 * kRow + 1] = acc[j][3];
     }
 }
 
-template <typename T, int G, int NT>
-int launch(const W4Params& p, int act, cudaStream_t s) {
-    const int64_t bx = (static_cast<int64_t>(p.N) + 15) / 16, by = (static_cast<int64_t>(p.M) + NT * 8 - 1) / (NT * 8);
+// ── few rows ────────────────────────────────────────────────────────────────
+__host__ __device__ constexpr int few_smem(int NT, int MT) { return kWarps * 16 * MT * (NT * 8 + 1) * 4; }
+
+// A scale as it lies in memory, and its value.
+__device__ __forceinline__ uint32_t raw_scale(const void* s, bool f32, int64_t i) {
+    return f32 ? static_cast<const uint32_t*>(s)[i] : static_cast<const uint16_t*>(s)[i];
+}
+__device__ __forceinline__ float scale_value(uint32_t raw, int dt) {
+    if (dt == SFB_F16) return __half2float(__ushort_as_half(static_cast<unsigned short>(raw)));
+    return __uint_as_float(dt == SFB_BF16 ? raw << 16 : raw);
+}
+
+template <typename T, int G, int NT, int MT>
+__global__ void __launch_bounds__(kThreads) w4a16_few_kernel(const W4Params p, const int act) {
+    constexpr int kB = block_of(G), kQ = kB / 32, kBlocks = kChunk / kB, kU = kChunk / G;
+    extern __shared__ float red[];
+    pdl_trigger();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * (16 * MT), m0 = blockIdx.y * (NT * 8);
+    const int whole = p.K / kChunk, chunks = (p.K + kChunk - 1) / kChunk;
+    const uint8_t* wr[2 * MT];                     // channels g, g + 8 of each tile; past the last: not stored
+    int64_t sr[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+        const int64_t n = min(n0 + 8 * i + g, p.N - 1);
+        wr[i] = p.w + n * (p.K / 2) + t * (kB / 8);
+        sr[i] = n * p.groups;
+    }
+    const T* xrow[NT];
+    bool xok[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int m = m0 + j * 8 + g;
+        xok[j] = m < p.M;
+        xrow[j] = static_cast<const T*>(p.x) + static_cast<int64_t>(xok[j] ? m : 0) * p.ldx + t * (kB / 4);
+    }
+    const bool f32 = p.scale_dtype == SFB_F32;
+    pdl_wait();
+    struct Set { uint32_t w[2 * MT][4]; uint4 x[4][NT]; uint32_t s[2 * MT][kU]; };
+    // kTail: the chunk ends before 128 inputs; what is past K is zeros
+    auto load = [&](Set& s, int c, auto tail) {
+        constexpr bool kTail = decltype(tail)::value;
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+            const int k0 = c * kChunk + k * kB;
+            const bool in = !kTail || k0 < p.K;
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i) {
+                if constexpr (kQ == 2) {
+                    const uint2 v = in ? *reinterpret_cast<const uint2*>(wr[i] + k0 / 2) : make_uint2(0, 0);
+                    s.w[i][2 * k] = v.x; s.w[i][2 * k + 1] = v.y;
+                } else {
+                    s.w[i][k] = in ? *reinterpret_cast<const uint32_t*>(wr[i] + k0 / 2) : 0u;
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < kQ; ++q)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    s.x[k * kQ + q][j] = in && xok[j] ? *reinterpret_cast<const uint4*>(xrow[j] + k0 + q * 8) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i)
+                s.s[i][u] = !kTail || c * kU + u < p.groups ? raw_scale(p.scale, f32, sr[i] + c * kU + u) : 0u;
+    };
+    auto fetch = [&](Set& s, int c) {
+        if (c < whole) load(s, c, std::false_type());
+        else if (c < chunks) load(s, c, std::true_type());
+    };
+    float acc[MT][NT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) zero(acc[i]);
+    auto work = [&](const Set& s) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                float part[NT][4];
+#pragma unroll
+                for (int w = u * (4 / kU); w < (u + 1) * (4 / kU); ++w)
+                    word_mma<T, NT>(part, s.w[2 * i][w], s.w[2 * i + 1][w], s.x[w], w == u * (4 / kU));
+                add_scaled(acc[i], part, scale_value(s.s[2 * i][u], p.scale_dtype), scale_value(s.s[2 * i + 1][u], p.scale_dtype));
+            }
+    };
+    Set a, b;
+    int c = warp;
+    fetch(a, c);
+    while (c < chunks) {
+        fetch(b, c + kWarps);
+        work(a);
+        c += kWarps;
+        if (c >= chunks) break;
+        fetch(a, c + kWarps);
+        work(b);
+        c += kWarps;
+    }
+    constexpr int kRow = NT * 8 + 1;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) put_acc<NT>(red + (warp * MT + i) * 16 * kRow, kRow, acc[i], g, t);
+    Epilogue<T, 16 * MT, NT * 8, kThreads, kWarps> e;
+    e.before(p, n0, m0);
+    __syncthreads();
+    e.after(p, act, red);
+}
+
+// ── more rows ───────────────────────────────────────────────────────────────
+// WM channel tiles of 16 by four parts of the inputs: a ring stage holds one chunk
+// of X for each part.
+constexpr int kParts = 4, kManyStages = 2;
+constexpr int kManyPitch = kParts * kChunk * 2 + 16;             // bytes per row of X in a stage
+__host__ __device__ constexpr int many_threads(int WM) { return kParts * WM * 32; }
+__host__ __device__ constexpr int many_smem(int NT, int WM) {
+    const int ring = kManyStages * NT * 8 * kManyPitch, red = kParts * WM * 16 * (NT * 8 + 1) * 4;
+    return ring > red ? ring : red;
+}
+
+template <typename T, int G, int NT, int WM>
+__global__ void __launch_bounds__(many_threads(WM)) w4a16_many_kernel(const W4Params p, const int act) {
+    constexpr int kB = block_of(G), kQ = kB / 32, kBlocks = kChunk / kB, kU = kChunk / G;
+    constexpr int WK = kParts, kStages = kManyStages, kPitch = kManyPitch, kRows = NT * 8;
+    constexpr int kSpan = WK * kChunk;             // inputs of a stage
+    extern __shared__ __align__(16) uint8_t smem[];
+    pdl_trigger();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int wm = warp % WM, wk = warp / WM;
+    const int n0 = blockIdx.x * (16 * WM), m0 = blockIdx.y * kRows;
+    const int steps = (p.K + kSpan - 1) / kSpan;
+    const int64_t na = min(n0 + 16 * wm + g, p.N - 1), nb = min(n0 + 16 * wm + g + 8, p.N - 1);
+    const uint8_t* wa = p.w + na * (p.K / 2) + t * (kB / 8);
+    const uint8_t* wb = p.w + nb * (p.K / 2) + t * (kB / 8);
+    const uint32_t sbase = ptx::smem_u32(smem);
+    pdl_wait();
+    auto copy = [&](int i) {                       // X of step i; zeros past M and K
+        const int stage = i % kStages;
+        for (int e = tid; e < kRows * (kSpan / 8); e += many_threads(WM)) {
+            const int r = e / (kSpan / 8), c = e % (kSpan / 8), k = i * kSpan + c * 8;
+            const bool in = m0 + r < p.M && k < p.K;
+            const T* src = static_cast<const T*>(p.x) + (in ? static_cast<int64_t>(m0 + r) * p.ldx + k : 0);
+            cp_async(sbase + (stage * kRows + r) * kPitch + c * 16, src, in ? 16 : 0, 16);
+        }
+    };
+    struct Set { uint32_t a[4], b[4]; float sa[kU], sb[kU]; };
+    auto load = [&](Set& s, int i) {
+        const int c = i * WK + wk;
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+            const int k0 = c * kChunk + k * kB;
+            const bool in = k0 < p.K;
+            if constexpr (kQ == 2) {
+                const uint2 x = in ? *reinterpret_cast<const uint2*>(wa + k0 / 2) : make_uint2(0, 0);
+                const uint2 y = in ? *reinterpret_cast<const uint2*>(wb + k0 / 2) : make_uint2(0, 0);
+                s.a[2 * k] = x.x; s.a[2 * k + 1] = x.y; s.b[2 * k] = y.x; s.b[2 * k + 1] = y.y;
+            } else {
+                s.a[k] = in ? *reinterpret_cast<const uint32_t*>(wa + k0 / 2) : 0u;
+                s.b[k] = in ? *reinterpret_cast<const uint32_t*>(wb + k0 / 2) : 0u;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int grp = c * kU + u;
+            const bool in = grp < p.groups;
+            s.sa[u] = in ? scale_at(p.scale, p.scale_dtype, na * p.groups + grp) : 0.f;
+            s.sb[u] = in ? scale_at(p.scale, p.scale_dtype, nb * p.groups + grp) : 0.f;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        if (i < steps) copy(i);
+        cp_async_commit();
+    }
+    float acc[NT][4];
+    zero(acc);
+    Set cur, nxt;
+    if (steps > 0) load(nxt, 0);
+    for (int i = 0; i < steps; ++i) {
+        cur = nxt;
+        cp_async_wait<kStages - 2>();
+        __syncthreads();                           // X of step i is there; step i − 1's stage is free
+        if (i + kStages - 1 < steps) copy(i + kStages - 1);
+        cp_async_commit();
+        if (i + 1 < steps) load(nxt, i + 1);
+        const uint8_t* xs = smem + (i % kStages) * kRows * kPitch + g * kPitch + wk * kChunk * 2 + t * (kB / 2);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            float part[NT][4];
+#pragma unroll
+            for (int w = u * (4 / kU); w < (u + 1) * (4 / kU); ++w) {
+                uint4 x[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    x[j] = *reinterpret_cast<const uint4*>(xs + j * 8 * kPitch + (w / kQ) * kB * 2 + (w % kQ) * 16);
+                word_mma<T, NT>(part, cur.a[w], cur.b[w], x, w == u * (4 / kU));
+            }
+            add_scaled(acc, part, cur.sa[u], cur.sb[u]);
+        }
+    }
+    Epilogue<T, 16 * WM, kRows, many_threads(WM), WK> e;
+    e.before(p, n0, m0);
+    cp_async_wait<0>();
+    __syncthreads();                               // the ring becomes the joining buffer
+    constexpr int kRow = kRows + 1;
+    float* red = reinterpret_cast<float*>(smem);   // [WK][16·WM][kRow]
+    put_acc<NT>(red + (wk * 16 * WM + 16 * wm) * kRow, kRow, acc, g, t);
+    __syncthreads();
+    e.after(p, act, red);
+}
+
+template <typename K>
+int launch(K kern, int smem, int threads, int channels, int rows, const W4Params& p, int act, cudaStream_t s) {
+    const int64_t bx = (static_cast<int64_t>(p.N) + channels - 1) / channels, by = (static_cast<int64_t>(p.M) + rows - 1) / rows;
     if (by > 65535) return SFB_ERR_SHAPE;
-    auto kern = w4a16_kernel<T, G, NT>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) { record_cuda_error(e, "w4a16 kernel attributes"); return SFB_ERR_CUDA; }
     prefer_max_shared(kern);
-    return launch_kernel(kern, dim3(static_cast<unsigned>(bx), static_cast<unsigned>(by)), kWarps * 32, 0, s, true, p, act);
+    return launch_kernel(kern, dim3(static_cast<unsigned>(bx), static_cast<unsigned>(by)), threads, smem, s, true, p, act);
 }
 
 template <typename T, int G>
 int pick_nt(const W4Params& p, int act, cudaStream_t s) {
-    if (p.M <= 8) return launch<T, G, 1>(p, act, s);
-    if (p.M <= 16) return launch<T, G, 2>(p, act, s);
-    if (p.M <= 32) return launch<T, G, 4>(p, act, s);
-    return launch<T, G, 9>(p, act, s);
+    if (p.M <= 16) {
+        // 32 channels a CTA (X and the loop's arithmetic for two tiles) once those
+        // are two CTAs for every SM
+        const bool two = (p.N + 31) / 32 >= 2 * std::max(device_info().num_sms, 1);
+        if (p.M <= 8) return two ? launch(w4a16_few_kernel<T, G, 1, 2>, few_smem(1, 2), kThreads, 32, 8, p, act, s)
+                                 : launch(w4a16_few_kernel<T, G, 1, 1>, few_smem(1, 1), kThreads, 16, 8, p, act, s);
+        return two ? launch(w4a16_few_kernel<T, G, 2, 2>, few_smem(2, 2), kThreads, 32, 16, p, act, s)
+                   : launch(w4a16_few_kernel<T, G, 2, 1>, few_smem(2, 1), kThreads, 16, 16, p, act, s);
+    }
+    // 64 channels a CTA once those fill half the SMs
+    const int64_t tiles = (static_cast<int64_t>(p.M) + 71) / 72;
+    const bool wide = (p.N + 63) / 64 * tiles * 2 >= std::max(device_info().num_sms, 1);
+    if (p.M <= 32) return wide ? launch(w4a16_many_kernel<T, G, 4, 4>, many_smem(4, 4), many_threads(4), 64, 32, p, act, s)
+                               : launch(w4a16_many_kernel<T, G, 4, 2>, many_smem(4, 2), many_threads(2), 32, 32, p, act, s);
+    return wide ? launch(w4a16_many_kernel<T, G, 9, 4>, many_smem(9, 4), many_threads(4), 64, 72, p, act, s)
+                : launch(w4a16_many_kernel<T, G, 9, 2>, many_smem(9, 2), many_threads(2), 32, 72, p, act, s);
 }
 
 template <typename T>
