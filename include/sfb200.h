@@ -473,8 +473,21 @@ int sfb_rdt1b_tick_stats(void* handle, int64_t* ticks, int64_t* encodes);
  * bit for bit. Changing it drops the captured graphs. No counterpart in the
  * reference. */
 int sfb_rdt1b_set_path(void* handle, int32_t path);
+/* Form of the cross-attention K/V cache: 16 (the default: K bf16, V fp16) or 4
+ * (sfb_kv4_cache; 72 bytes a token and head instead of 256, at the accuracy
+ * of 4 bits). The first change to 4 allocates the 4-bit caches (setup time).
+ * Drops the captured graphs and the tick's condition: encode again before the
+ * next forward or sample, which otherwise return SFB_ERR_INVALID. With 4 bits
+ * every session count takes the per-projection kernels (path 1). No counterpart
+ * in the reference. */
+int sfb_rdt1b_set_cache(void* handle, int32_t bits);
+/* Block `layer`'s 4-bit cache (batch = max_sessions; device pointers into the
+ * model), filled by the last encode with 4 bits. Of a language block only the
+ * valid slots are written. SFB_ERR_INVALID before the first set_cache(4). */
+int sfb_rdt1b_kv4_cache(void* handle, int32_t layer, sfb_kv4_cache* cache);
 /* Profiles one network evaluation of session 0 at timestep t on the
- * persistent-kernel path (path 0, whatever the handle's path): CUDA events
+ * persistent-kernel path (path 0, whatever the handle's path; with the 16-bit
+ * cache only, else SFB_ERR_INVALID): CUDA events
  * around each of its launches on `stream`. Writes the launch count to
  * *n_launches and, when max_launches is large enough, each launch's
  * algorithmic bytes (weights, scales and biases read, activations read and

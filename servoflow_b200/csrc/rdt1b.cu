@@ -46,6 +46,11 @@ int rms_norm_launch(const void* x, int64_t ldx, const void* w, void* out, int64_
 int head_rms_norm_launch(void* x, int64_t ld, int rows, int heads, const void* w, float eps,
                          cudaStream_t s);
 int bf16_to_f16_launch(void* x, int64_t ld, int rows, int cols, cudaStream_t s);
+int qk_norm_rope_launch(const sfb_norm_rope_args& a, cudaStream_t s);
+int kv4_append_launch(const sfb_kv4_cache* cache, const void* k, const int64_t* k_st, const void* v,
+                      const int64_t* v_st, int32_t dtype, int32_t seq, const int32_t* start, int32_t slot0,
+                      const int32_t* len, cudaStream_t s);
+int kv4_attention_launch(const sfb_kv4_cache* cache, const sfb_kv4_attn_args& a, cudaStream_t s);
 
 namespace rdt {
 
@@ -120,6 +125,10 @@ struct Model {
     __nv_bfloat16 *state, *lang_c, *img_c;
     int32_t* lang_len;
     std::vector<__nv_bfloat16*> kv;
+    // the cache's form: 16 bits in `kv`, or 4 bits in `kv4` (made by the first
+    // set_cache(4)); what the last encode filled
+    int cache_bits = 16, enc_bits = 16;
+    std::vector<sfb_kv4_cache> kv4;
     // step workspaces
     float* x;                                 // residual stream [B·S, D], fp32
     __nv_bfloat16 *xn, *qkv, *attn, *h, *ain, *ah1, *ah2, *seq, *tsc, *fsc, *th, *temb, *fh, *femb;
@@ -508,6 +517,47 @@ static int attention(const Model& m, const __nv_bfloat16* q, int64_t q_sb, int64
     return attention_tc_launch(a, s, o);
 }
 
+// The 4-bit form of every block's cross-attention cache (setup time).
+static int alloc_kv4(Model& m) {
+    const auto& c = m.c;
+    if (!m.kv4.empty()) return SFB_OK;
+    std::vector<sfb_kv4_cache> made(c.num_layers);
+    for (int l = 0; l < c.num_layers; ++l) {
+        sfb_kv4_cache& k = made[l];
+        const int64_t cap = ((l % 2 == 0 ? c.max_lang_len : c.img_len) + 31) / 32 * 32;
+        const int64_t rows = static_cast<int64_t>(c.max_sessions) * c.heads * cap;
+        k.batch = c.max_sessions; k.heads_kv = c.heads; k.capacity = static_cast<int32_t>(cap); k.head_dim = 64;
+        k.code_stride[1] = cap * 32; k.code_stride[0] = c.heads * k.code_stride[1];
+        k.scale_stride[1] = cap * 2; k.scale_stride[0] = c.heads * k.scale_stride[1];
+        SFB_TRY(dalloc(m, &k.k_codes, rows * 32)); SFB_TRY(dalloc(m, &k.v_codes, rows * 32));
+        SFB_TRY(dalloc(m, &k.k_scale, rows * 4));  SFB_TRY(dalloc(m, &k.v_scale, rows * 4));
+    }
+    m.kv4 = made;
+    return SFB_OK;
+}
+
+// Block l's cross-attention on the 4-bit cache: the queries' norm in place on the
+// projection's output, then the attention.
+static int cross_attention_kv4(const Model& m, int l, int B, cudaStream_t s) {
+    const int D = m.c.hidden, S = m.S();
+    sfb_norm_rope_args n;
+    std::memset(&n, 0, sizeof(n));
+    n.q = m.h; n.q_out = m.h; n.q_weight = m.blocks[l].cqn;
+    n.q_stride[0] = static_cast<int64_t>(S) * D; n.q_stride[1] = 64; n.q_stride[2] = D;
+    for (int i = 0; i < 3; ++i) n.q_out_stride[i] = n.q_stride[i];
+    n.batch = B; n.seq = S; n.heads = m.c.heads; n.head_dim = 64; n.norm = 1; n.eps = 1e-6f; n.dtype = SFB_BF16;
+    SFB_TRY(qk_norm_rope_launch(n, s));
+    sfb_kv4_attn_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.q = m.h; a.out = m.attn;
+    for (int i = 0; i < 3; ++i) a.q_stride[i] = a.out_stride[i] = n.q_stride[i];
+    a.heads = m.c.heads; a.seq_q = S; a.seq_k = l % 2 == 0 ? m.c.max_lang_len : m.c.img_len; a.dtype = SFB_BF16;
+    a.kv_len = l % 2 == 0 ? m.lang_len : nullptr;
+    sfb_kv4_cache k = m.kv4[l];
+    k.batch = B;
+    return kv4_attention_launch(&k, a, s);
+}
+
 // Condition encoding for one control tick (rdt1b.cpp:167-239 + the per-block
 // K/V projections of dit_block.cu:288-308, hoisted out of the step loop).
 static int encode(Model& m, int B, const void* lang, const int32_t* lang_len, const void* img,
@@ -539,9 +589,20 @@ static int encode(Model& m, int B, const void* lang, const int32_t* lang_len, co
         const int rows = lang_blk ? Ml : Mi;
         SFB_TRY(linear(m.blocks[l].ckv, lang_blk ? m.lang_c : m.img_c, D, rows, m.kv[l], 2 * D, 0, nullptr, 0, s));
         SFB_TRY(head_rms_norm_launch(m.kv[l], 2 * D, rows, c.heads, m.blocks[l].ckn, eps, s));
+        if (m.cache_bits == 4) {
+            // the projection's output, K normed, is only passed through here
+            const int Lk = lang_blk ? c.max_lang_len : c.img_len;
+            const int64_t st[3] = {static_cast<int64_t>(Lk) * 2 * D, 64, 2 * D};
+            sfb_kv4_cache k = m.kv4[l];
+            k.batch = B;
+            SFB_TRY(kv4_append_launch(&k, m.kv[l], st, m.kv[l] + D, st, SFB_BF16, Lk, nullptr, 0,
+                                      lang_blk ? m.lang_len : nullptr, s));
+            continue;
+        }
         // V is stored in fp16 (the attention's P·V operand type), converted once per tick
         SFB_TRY(bf16_to_f16_launch(m.kv[l] + D, 2 * D, rows, D, s));
     }
+    m.enc_bits = m.cache_bits;
     // Timestep embeddings of the sampler's steps and the control-frequency
     // embedding (sincos → Linear → SiLU → Linear, rdt1b.cpp:305-320). They
     // depend on the weights and the fixed schedule only, so they are made
@@ -568,6 +629,10 @@ static int forward(Model& m, int B, float t, cudaStream_t s, int step = -1) {
     const int D = c.hidden, S = m.S(), T = c.horizon, A = c.action_dim;
     const int M = B * S, Ma = B * (T + 1);
     const float eps = 1e-6f;
+    if (m.enc_bits != m.cache_bits) {
+        snprintf(last_error_buf(), 256, "the conditions were encoded into the %d-bit cache: encode again", m.enc_bits);
+        return SFB_ERR_INVALID;
+    }
     // state adaptor on [state, x_t] with an all-ones action mask
     prefer_max_shared(rdt::adaptor_input_kernel);
     prefer_max_shared(rdt::sincos_kernel);
@@ -593,7 +658,7 @@ static int forward(Model& m, int B, float t, cudaStream_t s, int step = -1) {
     SFB_TRY(launch_kernel(rdt::assemble_x_kernel, grid_for(static_cast<int64_t>(M) * D / 8, 256), 256, 0, s, true,
         temb, m.femb, m.seq, m.x_pos, m.x, B, S, D));
 
-    if (B == 1 && m.dense_ok && m.path != 1) {
+    if (B == 1 && m.dense_ok && m.path != 1 && m.cache_bits == 16) {
         // one session: the projections (and on path 0 the attentions) run as
         // stages of the persistent kernel, the pre-norms folded into them
         prefer_max_shared(rdt::norm_prep_kernel);
@@ -635,9 +700,13 @@ static int forward(Model& m, int B, float t, cudaStream_t s, int step = -1) {
         const int Lk = lang_blk ? c.max_lang_len : c.img_len;
         SFB_TRY(rms_norm_launch(m.x, D, bl.norm2, m.xn, D, M, D, eps, s, true));
         SFB_TRY(linear(bl.cq, m.xn, D, M, m.h, D, 0, nullptr, 0, s));
-        SFB_TRY(attention(m, m.h, static_cast<int64_t>(S) * D, D, m.kv[l], m.kv[l] + D,
-                          static_cast<int64_t>(Lk) * 2 * D, 2 * D, m.attn, B, S, Lk,
-                          lang_blk ? m.lang_len : nullptr, true, bl.cqn, nullptr, s));
+        if (m.cache_bits == 4) {
+            SFB_TRY(cross_attention_kv4(m, l, B, s));
+        } else {
+            SFB_TRY(attention(m, m.h, static_cast<int64_t>(S) * D, D, m.kv[l], m.kv[l] + D,
+                              static_cast<int64_t>(Lk) * 2 * D, 2 * D, m.attn, B, S, Lk,
+                              lang_blk ? m.lang_len : nullptr, true, bl.cqn, nullptr, s));
+        }
         SFB_TRY(linear(bl.cproj, m.attn, D, M, m.x, D, 0, m.x, D, s, true));
         // x = x + fc2(gelu(fc1(norm3(x))))
         SFB_TRY(rms_norm_launch(m.x, D, bl.norm3, m.xn, D, M, D, eps, s, true));
@@ -915,6 +984,33 @@ int sfb_rdt1b_set_path(void* handle, int32_t path) {
     return SFB_OK;
 }
 
+int sfb_rdt1b_set_cache(void* handle, int32_t bits) {
+    auto* m = static_cast<rdt::Model*>(handle);
+    if (m == nullptr || (bits != 16 && bits != 4)) return SFB_ERR_INVALID;
+    SFB_MODEL_ENTRY(m);
+    if (bits == m->cache_bits) return SFB_OK;
+    if (bits == 4) SFB_TRY(rdt::alloc_kv4(*m));
+    // captured graphs hold the other cache's kernels
+    cudaError_t e = cudaStreamSynchronize(m->own);
+    for (auto& g : m->graphs) cudaGraphExecDestroy(g.second);
+    m->graphs.clear();
+    m->graph_kernels.clear();
+    m->cache_bits = bits;
+    m->cond_valid = false;
+    if (e != cudaSuccess) { record_cuda_error(e, "rdt1b set cache"); return SFB_ERR_CUDA; }
+    return SFB_OK;
+}
+
+int sfb_rdt1b_kv4_cache(void* handle, int32_t layer, sfb_kv4_cache* cache) {
+    auto* m = static_cast<rdt::Model*>(handle);
+    if (m == nullptr || cache == nullptr) return SFB_ERR_INVALID;
+    SFB_MODEL_ENTRY(m);
+    if (layer < 0 || layer >= m->c.num_layers) return SFB_ERR_SHAPE;
+    if (m->kv4.empty()) return SFB_ERR_INVALID;
+    *cache = m->kv4[layer];
+    return SFB_OK;
+}
+
 int sfb_rdt1b_param(void* handle, const char* name, void** ptr, int64_t* numel, int32_t* dtype) {
     auto* m = static_cast<rdt::Model*>(handle);
     if (m == nullptr || name == nullptr || ptr == nullptr || numel == nullptr || dtype == nullptr)
@@ -943,6 +1039,7 @@ int sfb_rdt1b_profile_dense(void* handle, float t, int32_t max_launches, int32_t
     auto* m = static_cast<rdt::Model*>(handle);
     if (m == nullptr || n_launches == nullptr) return SFB_ERR_INVALID;
     SFB_MODEL_ENTRY(m);
+    if (m->cache_bits != 16) return SFB_ERR_INVALID;
     if (!m->dense_ok) return SFB_ERR_UNSUPPORTED;
     const int n = static_cast<int>(m->dl[0].size());
     *n_launches = n;

@@ -37,6 +37,8 @@ def _declare(lib):
                                        c.c_int32]
     lib.sfb_rdt1b_graph_kernels.argtypes = [c.c_void_p, c.c_int32, c.POINTER(c.c_int64)]
     lib.sfb_rdt1b_set_path.argtypes = [c.c_void_p, c.c_int32]
+    lib.sfb_rdt1b_set_cache.argtypes = [c.c_void_p, c.c_int32]
+    lib.sfb_rdt1b_kv4_cache.argtypes = [c.c_void_p, c.c_int32, c.c_void_p]
     lib.sfb_rdt1b_profile_dense.argtypes = [c.c_void_p, c.c_float, c.c_int32, c.POINTER(c.c_int32),
                                             c.POINTER(c.c_double), c.POINTER(c.c_float), c.c_void_p]
     lib.sfb_rdt1b_tick.argtypes = [c.c_void_p, c.c_int32, c.c_uint64, c.c_void_p, c.c_void_p, c.c_void_p,
@@ -50,7 +52,7 @@ def _declare(lib):
                                               c.POINTER(c.c_int64)]
     lib.sfb_rdt1b_params_missing.argtypes = [c.c_void_p, c.POINTER(c.c_int64), c.c_char_p, c.c_int32]
     for f in ("default_config", "create", "destroy", "encode", "forward", "sample", "param",
-              "schedule", "graph_kernels", "set_path", "tick", "invalidate_condition", "tick_stats", "config_from_json", "load_safetensors", "load_checkpoint",
+              "schedule", "graph_kernels", "set_path", "set_cache", "kv4_cache", "tick", "invalidate_condition", "tick_stats", "config_from_json", "load_safetensors", "load_checkpoint",
               "params_missing"):
         getattr(lib, "sfb_rdt1b_" + f).restype = c.c_int
     lib._rdt_declared = True
@@ -139,6 +141,26 @@ class RDT1B:
         projection, norm and attention (default), 2 the persistent kernel
         between cross-attention kernels."""
         _capi.check(self.lib.sfb_rdt1b_set_path(self.h, int(path)), "set_path")
+
+    def set_cache(self, bits: int) -> None:
+        """Form of the cross-attention K/V cache (sfb_rdt1b_set_cache): 16 or 4
+        bits. Encode again afterwards."""
+        _capi.check(self.lib.sfb_rdt1b_set_cache(self.h, int(bits)), "set_cache")
+
+    def kv4_cache(self, layer: int):
+        """A copy (quant4.KV4Cache) of a block's 4-bit cross-attention cache."""
+        from .quant4 import KV4Cache
+        buf = ctypes.create_string_buffer(_capi.KV4_CACHE.size)
+        _capi.check(self.lib.sfb_rdt1b_kv4_cache(self.h, int(layer), buf), "kv4_cache")
+        kc, vc, ks, vs, _, _, _, _, B, H, C, D = _capi.KV4_CACHE.unpack(buf.raw)
+        torch.cuda.synchronize()
+        out = []
+        for ptr, shape, dt in ((kc, (B, H, C, D // 2), torch.uint8), (vc, (B, H, C, D // 2), torch.uint8),
+                               (ks, (B, H, C, D // 32), torch.float16), (vs, (B, H, C, D // 32), torch.float16)):
+            t = torch.empty(shape, dtype=dt, device="cuda")
+            _copy_d2d(t.data_ptr(), ptr, t.numel() * t.element_size())
+            out.append(t)
+        return KV4Cache(*out)
 
     def profile_dense(self, t: float = 999.0):
         """[(algorithmic bytes, microseconds)] of each persistent-kernel launch of
