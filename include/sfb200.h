@@ -346,6 +346,8 @@ int sfb_kv4_read(const sfb_kv4_cache* cache, void* k, const int64_t* k_stride, v
  *   sees slot j iff j <= n - seq_q + i with n = min(kv_len[b], seq_k) (n =
  *   seq_k without kv_len). Queries before the first slot see none.
  * - A query that sees no slot produces zeros. Masked slots may hold anything.
+ *   With is_causal, a NaN scale of V in one of the last seq_q slots makes the
+ *   whole rows that see the slot NaN, elsewhere its channels of them.
  * - heads % heads_kv == 0; scale 0 means 1/sqrt(head_dim).
  * - num_splits: key splits merged inside one thread-block cluster (0 = choose,
  *   else 1..16). Allocates nothing, keeps no workspace. */

@@ -77,6 +77,15 @@ template <int D> struct VWords;
 template <> struct VWords<64>  { using T = uint32_t; };
 template <> struct VWords<128> { using T = uint2; };
 
+// A scale that is not finite makes its group NaN. For a slot that only some of a
+// tile's rows see (causal calls) the others would take 0 · NaN from such a V, so
+// there V is taken as 0 and K as NaN: the rows that see the slot become NaN whole.
+__device__ __forceinline__ bool not_finite(uint32_t scale_bits) { return (scale_bits & 0x7c00u) == 0x7c00u; }
+__device__ __forceinline__ void contain(__half2& ks, __half2& vs) {
+    const uint32_t v = h2u(vs);
+    if (not_finite(v) || not_finite(v >> 16)) { ks = u2h(0x7fff7fffu); vs = u2h(0u); }
+}
+
 constexpr float kUnseen = 1e30f;
 constexpr int kWarps = 8;                                        // computing
 __host__ __device__ constexpr bool uses_ring(int D) { return D == 128; }
@@ -165,6 +174,12 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
     __syncthreads();
 
     const uint8_t* mask = p.key_mask != nullptr ? p.key_mask + b * p.mask_sb : nullptr;
+    auto row_bad = [](const uint16_t* vs) {         // a slot's scales of V
+        bool x = false;
+#pragma unroll
+        for (int i = 0; i < D / kGroup; ++i) x |= not_finite(vs[i]);
+        return x;
+    };
     auto seen = [&](int key) { return key < kend && (mask == nullptr || mask[key] != 0); };
     bool ok = true;
 
@@ -284,7 +299,7 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
         const uint16_t* ksp = reinterpret_cast<const uint16_t*>(p.c.ks + hs) + (first + key_of(g)) * (D / kGroup) + (D / 4 * t) / kGroup;
         const uint16_t* vsp = reinterpret_cast<const uint16_t*>(p.c.vs + hs) + (first + t) * (D / kGroup) + (D / 8 * g) / kGroup;
         auto load = [&](Raw<D>& r, int k0) {       // tiles in order: the pointers move along
-            const bool whole = k0 + 16 <= kend && mask == nullptr;
+            const bool whole = k0 + 16 <= kfull && mask == nullptr;
             if (whole) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -303,6 +318,9 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
                     if (seen(k0 + key_of(g) + 8 * e)) {
                         r.k[e] = *reinterpret_cast<const KT*>(kp + 8 * e * (D / 2));
                         r.ks[e] = ksp[8 * e * (D / kGroup)];
+                        const int key = k0 + key_of(g) + 8 * e;
+                        if (key >= kfull && row_bad(reinterpret_cast<const uint16_t*>(p.c.vs + hs) + static_cast<int64_t>(key) * (D / kGroup)))
+                            r.ks[e] = 0x7fff;
                     }
                 }
 #pragma unroll
@@ -311,6 +329,7 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
                     if (seen(k0 + t + 4 * e)) {
                         r.v[e] = *reinterpret_cast<const VT*>(vp + 4 * e * (D / 2));
                         r.vs[e] = vsp[4 * e * (D / kGroup)];
+                        if (k0 + t + 4 * e >= kfull && not_finite(r.vs[e])) r.vs[e] = 0;
                     }
                 }
             }
@@ -340,25 +359,30 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
         // seen may hold anything: their scale is taken as 0.
         auto fetch = [&](Raw<D>& r, const uint8_t* kc, const uint8_t* vc, const uint16_t* ks, const uint16_t* vs,
                          int in_block, int k0) {
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int key = in_block + key_of(g) + 8 * i;
                 r.k[i] = *reinterpret_cast<const typename KWords<D>::T*>(kc + key * (D / 2) + (D / 8) * t);
                 r.ks[i] = ks[key * (D / kGroup) + (D / 4 * t) / kGroup];
             }
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = in_block + t + 4 * i;            // key_of(2t + (i & 1) + 8·(i >> 1))
                 r.v[i] = *reinterpret_cast<const typename VWords<D>::T*>(vc + key * (D / 2) + (D / 16) * g);
                 r.vs[i] = vs[key * (D / kGroup) + (D / 8 * g) / kGroup];
             }
-            if (k0 + 16 > kend || mask != nullptr) {
-    #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (!seen(k0 + key_of(g) + 8 * i)) r.ks[i] = 0;
-    #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (!seen(k0 + t + 4 * i)) r.vs[i] = 0;
+            if (k0 + 16 > kfull || mask != nullptr) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int key = k0 + key_of(g) + 8 * i;
+                    if (!seen(key)) r.ks[i] = 0;
+                    else if (key >= kfull && row_bad(vs + (in_block + key - k0) * (D / kGroup))) r.ks[i] = 0x7fff;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = k0 + t + 4 * i;
+                    if (!seen(key) || (key >= kfull && not_finite(r.vs[i]))) r.vs[i] = 0;
+                }
             }
         };
         // ── copies of block i (one lane), once its stage is free ───────────────

@@ -427,14 +427,28 @@ __global__ void __launch_bounds__(many_threads(WM)) w4a16_many_kernel(const W4Pa
     e.after(p, act, red);
 }
 
-template <typename K>
-int launch(K kern, int smem, int threads, int channels, int rows, const W4Params& p, int act, cudaStream_t s) {
+template <auto Kern>
+int launch(int smem, int threads, int channels, int rows, const W4Params& p, int act, cudaStream_t s) {
     const int64_t bx = (static_cast<int64_t>(p.N) + channels - 1) / channels, by = (static_cast<int64_t>(p.M) + rows - 1) / rows;
     if (by > 65535) return SFB_ERR_SHAPE;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) { record_cuda_error(e, "w4a16 kernel attributes"); return SFB_ERR_CUDA; }
-    prefer_max_shared(kern);
-    return launch_kernel(kern, dim3(static_cast<unsigned>(bx), static_cast<unsigned>(by)), threads, smem, s, true, p, act);
+    static std::atomic<bool> done[64];             // kernel attributes, once per device (idempotent)
+    std::atomic<bool>& set = done[device_info().ordinal & 63];
+    if (!set.load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) { record_cuda_error(e, "w4a16 kernel attributes"); return SFB_ERR_CUDA; }
+        prefer_max_shared(Kern);
+        set.store(true, std::memory_order_release);
+    }
+    return launch_kernel(Kern, dim3(static_cast<unsigned>(bx), static_cast<unsigned>(by)), threads, smem, s, true, p, act);
+}
+
+template <typename T, int G, int NT, int MT>
+int few(const W4Params& p, int act, cudaStream_t s) {
+    return launch<w4a16_few_kernel<T, G, NT, MT>>(few_smem(NT, MT), kThreads, 16 * MT, NT * 8, p, act, s);
+}
+template <typename T, int G, int NT, int WM>
+int many(const W4Params& p, int act, cudaStream_t s) {
+    return launch<w4a16_many_kernel<T, G, NT, WM>>(many_smem(NT, WM), many_threads(WM), 16 * WM, NT * 8, p, act, s);
 }
 
 template <typename T, int G>
@@ -443,18 +457,18 @@ int pick_nt(const W4Params& p, int act, cudaStream_t s) {
         // 32 channels a CTA (X and the loop's arithmetic for two tiles) once those
         // are two CTAs for every SM
         const bool two = (p.N + 31) / 32 >= 2 * std::max(device_info().num_sms, 1);
-        if (p.M <= 8) return two ? launch(w4a16_few_kernel<T, G, 1, 2>, few_smem(1, 2), kThreads, 32, 8, p, act, s)
-                                 : launch(w4a16_few_kernel<T, G, 1, 1>, few_smem(1, 1), kThreads, 16, 8, p, act, s);
-        return two ? launch(w4a16_few_kernel<T, G, 2, 2>, few_smem(2, 2), kThreads, 32, 16, p, act, s)
-                   : launch(w4a16_few_kernel<T, G, 2, 1>, few_smem(2, 1), kThreads, 16, 16, p, act, s);
+        if (p.M <= 8) return two ? few<T, G, 1, 2>(p, act, s)
+                                 : few<T, G, 1, 1>(p, act, s);
+        return two ? few<T, G, 2, 2>(p, act, s)
+                   : few<T, G, 2, 1>(p, act, s);
     }
     // 64 channels a CTA once those fill half the SMs
     const int64_t tiles = (static_cast<int64_t>(p.M) + 71) / 72;
     const bool wide = (p.N + 63) / 64 * tiles * 2 >= std::max(device_info().num_sms, 1);
-    if (p.M <= 32) return wide ? launch(w4a16_many_kernel<T, G, 4, 4>, many_smem(4, 4), many_threads(4), 64, 32, p, act, s)
-                               : launch(w4a16_many_kernel<T, G, 4, 2>, many_smem(4, 2), many_threads(2), 32, 32, p, act, s);
-    return wide ? launch(w4a16_many_kernel<T, G, 9, 4>, many_smem(9, 4), many_threads(4), 64, 72, p, act, s)
-                : launch(w4a16_many_kernel<T, G, 9, 2>, many_smem(9, 2), many_threads(2), 32, 72, p, act, s);
+    if (p.M <= 32) return wide ? many<T, G, 4, 4>(p, act, s)
+                               : many<T, G, 4, 2>(p, act, s);
+    return wide ? many<T, G, 9, 4>(p, act, s)
+                : many<T, G, 9, 2>(p, act, s);
 }
 
 template <typename T>

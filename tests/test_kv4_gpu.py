@@ -399,3 +399,25 @@ def test_wrapper_refusals(be, gpu):
     bad = KV4Cache(cache.k_codes, cache.v_codes, cache.k_scale.float(), cache.v_scale)
     with pytest.raises(E):
         be.kv4_attention(q, bad, out)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq,Sk", [(9, 40), (20, 33), (67, 300), (130, 260)])
+def test_nan_slots_do_not_reach_rows_before_them(be, gpu, D, Sq, Sk):
+    """Causal calls: a slot whose V (or K) is NaN is in the same tile as rows that do
+    not see it. Those keep their values, the rows that see it are NaN."""
+    be.device_error(reset=True)
+    bad = Sk - Sq // 3                                      # seen by the last rows alone
+    q = torch.randn(1, 2, Sq, D, generator=torch.Generator().manual_seed(31)).to(torch.float16).to(gpu)
+    sees = torch.arange(Sq, device=gpu) + Sk - Sq >= bad
+    for field in ("v_scale", "k_scale"):
+        cache = KV4Cache.allocate(1, 2, (Sk + 3) // 4 * 4, D)
+        fill(cache, 32)
+        clean, out = torch.empty_like(q), torch.empty_like(q)
+        be.kv4_attention(q, cache, clean, seq_k=Sk, is_causal=True)
+        getattr(cache, field)[:, :, bad, 1] = float("nan")
+        be.kv4_attention(q, cache, out, seq_k=Sk, is_causal=True)
+        torch.cuda.synchronize()
+        assert torch.equal(out[:, :, ~sees], clean[:, :, ~sees])
+        assert out[:, :, sees].isnan().any(-1).all()
+    assert be.device_error() == 0
