@@ -1,4 +1,5 @@
-// kv4_attn.cu — attention over the 4-bit K/V cache (sfb_kv4_attention).
+// kv4_attn.cu — attention over the 4-bit K/V cache (sfb_kv4_attention), up to 8
+// rows per K/V head; kv4_attn_tc.cu has the form for more.
 //
 //   out[r, :] = softmax_j( scale · q[r, :]·k[j, :] ) · v[j, :],  k, v = c·s
 //
@@ -20,10 +21,12 @@
 // 64 channels a lane loads its codes of the next tile straight into registers
 // while it works on this one. With 128 those registers would cost the second CTA
 // per SM, so blocks go through a ring in shared memory, four untiled bulk copies
-// each (codes and scales of K and V), issued by a ninth warp (by warp 0 with 32
-// rows, whose warps need the ninth's registers). 32 sessions of 8 to 16 k slots
-// of 8 heads: 178 µs from registers, 153 through the ring; 32 sessions of 4374
-// slots of 32 64-channel heads: 105 µs from registers, 111 through the ring.
+// each (codes and scales of K and V), issued by a ninth warp. 32 sessions of 8 to
+// 16 k slots of 8 heads: 178 µs from registers, 153 through the ring (144 as it is
+// now: 3.2 TB/s of codes and scales); 32 sessions of 4374 slots of 32 64-channel
+// heads: 105 µs from registers (101 now, 3.2 TB/s), 111 through the ring. What
+// bounds both is the issue of instructions, about 210 a tile and warp of 64
+// channels and 440 of 128, most of them to make fragments of the codes.
 // A nibble becomes fp16 exactly with one bit operation and one add or fma
 // (0x6400 | n = 1024 + n), the scale is one exact fp16 product (kv4.cu).
 // Pᵀ moves from the accumulator's layout to the B operand's by two movmatrix.
@@ -87,22 +90,22 @@ __device__ __forceinline__ void contain(__half2& ks, __half2& vs) {
 }
 
 constexpr float kUnseen = 1e30f;
+constexpr int kRows = 8;                                         // rows of a CTA
 constexpr int kWarps = 8;                                        // computing
 __host__ __device__ constexpr bool uses_ring(int D) { return D == 128; }
-__host__ __device__ constexpr bool own_warp(int D, int NT) { return uses_ring(D) && NT < 4; }   // a ninth issues the copies
-__host__ __device__ constexpr int attn_threads(int D, int NT) { return (kWarps + (own_warp(D, NT) ? 1 : 0)) * 32; }
+__host__ __device__ constexpr int attn_threads(int D) { return (kWarps + (uses_ring(D) ? 1 : 0)) * 32; }   // a ninth warp issues the copies
 constexpr int kBlock = 16 * kWarps;                              // keys per ring stage
 __host__ __device__ constexpr int code_bytes(int D) { return kBlock * D / 2; }
 __host__ __device__ constexpr int scale_bytes(int D) { return kBlock * (D / kGroup) * 2; }
 __host__ __device__ constexpr int stage_bytes(int D) { return 2 * (code_bytes(D) + scale_bytes(D)); }
 __host__ __device__ constexpr int ring_stages(int D) { return uses_ring(D) ? 4 : 0; }
 __host__ __device__ constexpr int attn_pad(int D) { return D + 8; }   // halves per row of Q in shared memory
-__host__ __device__ constexpr int join_bytes(int D, int NT) {         // per-warp O, m, l and the CTA's partial
-    return (kWarps + 1) * NT * 8 * (D + 2) * 4;
+__host__ __device__ constexpr int join_bytes(int D) {         // per-warp O, m, l and the CTA's partial
+    return (kWarps + 1) * kRows * (D + 2) * 4;
 }
-__host__ __device__ constexpr int attn_smem(int D, int NT) {
-    const int ring = stage_bytes(D) * ring_stages(D), join = join_bytes(D, NT);
-    return NT * 8 * attn_pad(D) * 2 + (ring > join ? ring : join) + 16 * ring_stages(D);
+__host__ __device__ constexpr int attn_smem(int D) {
+    const int ring = stage_bytes(D) * ring_stages(D), join = join_bytes(D);
+    return kRows * attn_pad(D) * 2 + (ring > join ? ring : join) + 16 * ring_stages(D);
 }
 // Codes and scales of one 16-key tile as a lane holds them: K of MMA rows g and
 // g + 8 (channels [D/4·t, +D/4)), V of rows 2t, 2t+1, 2t+8, 2t+9 (channels [D/8·g, +D/8)).
@@ -116,9 +119,9 @@ struct Raw {
 // The key of a 16-key tile that is row m of the MMAs.
 __device__ __forceinline__ int key_of(int m) { return ((m & 7) >> 1) + 4 * (m & 1) + 8 * (m >> 3); }
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn_kernel(const Kv4AttnParams p) {
-    constexpr int kRows = NT * 8, kPad = attn_pad(D), kSteps = D / 16, kMT = D / 16, W = kWarps, kThreads = attn_threads(D, NT);
+template <typename T, int D>
+__global__ void __launch_bounds__(attn_threads(D), 2) kv4_attn_kernel(const Kv4AttnParams p) {
+    constexpr int kPad = attn_pad(D), kSteps = D / 16, kMT = D / 16, W = kWarps, kThreads = attn_threads(D);
     constexpr int kStages = ring_stages(D), kCode = code_bytes(D), kScale = scale_bytes(D), kStage = stage_bytes(D);
     extern __shared__ __align__(16) uint8_t smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem);                   // full, then empty
@@ -132,8 +135,8 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
     float* pL = pM + kRows;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x, hk = blockIdx.y / p.rtiles, rt = blockIdx.y - hk * p.rtiles, b = blockIdx.z;
-    const int r0 = rt * kRows, rows = min(kRows, p.R - r0);
+    const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+    const int rows = p.R;
     if (kStages > 0 && tid == 0) {
         for (int i = 0; i < kStages; ++i) { ptx::mbar_init(&bars[i], 1); ptx::mbar_init(&bars[kStages + i], W); }
         ptx::fence_mbarrier_init();
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
     if (p.kv_len != nullptr) n = min(n, max(0, p.kv_len[b]));
     // a row sees the slots below limit(row)
     auto limit = [&](int r) { return p.causal ? min(n, max(0, n - p.Sq + r / p.g + 1)) : n; };
-    const int kend = limit(r0 + rows - 1), kfull = limit(r0);             // limits grow with the row
+    const int kend = limit(rows - 1), kfull = limit(0);             // limits grow with the row
     const int blocks = (kend + kBlock - 1) / kBlock;
     const int per = blocks / p.splits, rem = blocks - per * p.splits;
     const int b_begin = split * per + min(split, rem), nblk = per + (split < rem ? 1 : 0);
@@ -156,7 +159,7 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
         const int r = i / (D / 8), d = (i % (D / 8)) * 8;
         uint4 u = make_uint4(0, 0, 0, 0);
         if (r < rows) {
-            const int rr = r0 + r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
+            const int rr = r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
             const T* src = static_cast<const T*>(p.q) + b * p.q_st[0] + h * p.q_st[1] + qi * p.q_st[2] + d;
             u = *reinterpret_cast<const uint4*>(src);
             if constexpr (std::is_same<T, __nv_bfloat16>::value) {
@@ -184,23 +187,12 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
     bool ok = true;
 
     const float sgn = p.sl2 < 0.f ? -1.f : 1.f;    // a masked logit is −∞ after the scaling
-    float o[kMT][NT][4], nm[NT][2], l[NT][2];      // nm: −reference
+    float o[kMT][4], nm[2] = {kUnseen, kUnseen}, l[2] = {0.f, 0.f};      // nm: −reference
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        nm[j][0] = nm[j][1] = kUnseen;
-        l[j][0] = l[j][1] = 0.f;
+    for (int i = 0; i < kMT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    uint4 qr[kSteps / 2];                          // Q fragments
 #pragma unroll
-        for (int i = 0; i < kMT; ++i) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
-    }
-    constexpr bool kQReg = NT <= 2;                // Q fragments held in registers
-    uint4 qr[kQReg ? NT : 1][kQReg ? kSteps / 2 : 1];
-    if constexpr (kQReg) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int s = 0; s < kSteps / 2; ++s)
-                qr[j][s] = reinterpret_cast<const uint4*>(sQ + (j * 8 + g) * kPad + (D / 4) * t)[s];
-    }
+    for (int s = 0; s < kSteps / 2; ++s) qr[s] = reinterpret_cast<const uint4*>(sQ + g * kPad + (D / 4) * t)[s];
     auto step = [&](const Raw<D>& r, int k0) {
         const bool edge = k0 + 16 > kfull || mask != nullptr;
         // K fragments: half2 2s and 2s+1 of a key's words are step s
@@ -217,20 +209,17 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
                 for (int e = 0; e < 4; ++e) ka[i][4 * x + e] = d4[e];
             }
         }
-        uint32_t pb[NT][2];                        // Pᵀ fragments
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        uint32_t pb[2];                            // Pᵀ fragments
+        {
             float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < kSteps; s += 2) {
-                uint4 q4;
-                if constexpr (kQReg) q4 = qr[j][s / 2];
-                else q4 = reinterpret_cast<const uint4*>(sQ + (j * 8 + g) * kPad + (D / 4) * t)[s / 2];
+                const uint4 q4 = qr[s / 2];
                 mma16816(c, ka[0][2 * s], ka[1][2 * s], ka[0][2 * s + 1], ka[1][2 * s + 1], q4.x, q4.y);
                 mma16816(c, ka[0][2 * s + 2], ka[1][2 * s + 2], ka[0][2 * s + 3], ka[1][2 * s + 3], q4.z, q4.w);
             }
             if (edge) {
-                const int ra = min(r0 + j * 8 + 2 * t, p.R - 1), rb = min(r0 + j * 8 + 2 * t + 1, p.R - 1);
+                const int ra = min(2 * t, p.R - 1), rb = min(2 * t + 1, p.R - 1);
                 const int la = limit(ra), lb = limit(rb), ka_ = k0 + key_of(g), kb_ = ka_ + 8;
                 const bool v0 = seen(ka_), v1 = seen(kb_);
                 if (!v0 || ka_ >= la) c[0] = -INFINITY * sgn;
@@ -240,8 +229,8 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
             }
             // exponents against the rows' references; a row that saw no key yet has
             // the reference −kUnseen, so that its first key passes it
-            float x[4] = {fmaf(c[0], p.sl2, nm[j][0]), fmaf(c[1], p.sl2, nm[j][1]), fmaf(c[2], p.sl2, nm[j][0]),
-                          fmaf(c[3], p.sl2, nm[j][1])};
+            float x[4] = {fmaf(c[0], p.sl2, nm[0]), fmaf(c[1], p.sl2, nm[1]), fmaf(c[2], p.sl2, nm[0]),
+                          fmaf(c[3], p.sl2, nm[1])};
             if (__any_sync(0xffffffffu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > 8.f)) {
                 float ma = fmaxf(c[0] * p.sl2, c[2] * p.sl2), mb = fmaxf(c[1] * p.sl2, c[3] * p.sl2);
 #pragma unroll
@@ -250,21 +239,21 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
                     mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, off));
                 }
                 float aa = 1.f, ab = 1.f;
-                if (ma + nm[j][0] > 8.f) { aa = nm[j][0] == kUnseen ? 0.f : ptx::ex2(-nm[j][0] - ma); nm[j][0] = -ma; }
-                if (mb + nm[j][1] > 8.f) { ab = nm[j][1] == kUnseen ? 0.f : ptx::ex2(-nm[j][1] - mb); nm[j][1] = -mb; }
-                l[j][0] *= aa; l[j][1] *= ab;
+                if (ma + nm[0] > 8.f) { aa = nm[0] == kUnseen ? 0.f : ptx::ex2(-nm[0] - ma); nm[0] = -ma; }
+                if (mb + nm[1] > 8.f) { ab = nm[1] == kUnseen ? 0.f : ptx::ex2(-nm[1] - mb); nm[1] = -mb; }
+                l[0] *= aa; l[1] *= ab;
 #pragma unroll
                 for (int i = 0; i < kMT; ++i) {
-                    o[i][j][0] *= aa; o[i][j][1] *= ab; o[i][j][2] *= aa; o[i][j][3] *= ab;
+                    o[i][0] *= aa; o[i][1] *= ab; o[i][2] *= aa; o[i][3] *= ab;
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = fmaf(c[e], p.sl2, nm[j][e & 1]);
+                for (int e = 0; e < 4; ++e) x[e] = fmaf(c[e], p.sl2, nm[e & 1]);
             }
             const float p0 = ptx::ex2(x[0]), p1 = ptx::ex2(x[1]), p2 = ptx::ex2(x[2]), p3 = ptx::ex2(x[3]);
-            l[j][0] += p0 + p2;
-            l[j][1] += p1 + p3;
-            pb[j][0] = movmatrix_t(h2u(__floats2half2_rn(p0, p1)));
-            pb[j][1] = movmatrix_t(h2u(__floats2half2_rn(p2, p3)));
+            l[0] += p0 + p2;
+            l[1] += p1 + p3;
+            pb[0] = movmatrix_t(h2u(__floats2half2_rn(p0, p1)));
+            pb[1] = movmatrix_t(h2u(__floats2half2_rn(p2, p3)));
         }
         // Vᵀ fragments: words of a key pair interleaved by halves, so that a
         // nibble pair is one channel of both keys; [pair][word][low / high half]
@@ -281,11 +270,9 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
             }
         }
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int i = 0; i < kMT; ++i)
-                mma16816(o[i][j], va[0][i / 4][0][i % 4], va[0][i / 4][1][i % 4], va[1][i / 4][0][i % 4],
-                         va[1][i / 4][1][i % 4], pb[j][0], pb[j][1]);
+        for (int i = 0; i < kMT; ++i)
+            mma16816(o[i], va[0][i / 4][0][i % 4], va[0][i / 4][1][i % 4], va[1][i / 4][0][i % 4],
+                     va[1][i / 4][1][i % 4], pb[0], pb[1]);
     };
     if constexpr (!uses_ring(D)) {
         // the next tile's codes are in flight while this one is worked on; slots
@@ -403,21 +390,14 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
             return true;
         };
         int issued = 0;                                // blocks copied, in the copying lane
-        auto copy_up_to = [&](int end) {
-            while (ok && issued < end) {
+        if (warp == W) {
+            while (lane == 0 && ok && issued < nblk) {
                 if (copy_block(issued)) ++issued;
                 else ok = false;
             }
-        };
-        if (own_warp(D, NT) && warp == W) {
-            if (lane == 0) copy_up_to(nblk);
         } else {
             auto take = [&](Raw<D>& r, int i) {
                 const int s = i % kStages;
-                if (!own_warp(D, NT) && warp == 0) {      // (stage of block i + kStages − 1: block i − 1 was its last)
-                    if (lane == 0) copy_up_to(min(nblk, i + kStages - (i > 0 ? 1 : 0)));
-                    __syncwarp();
-                }
                 if (!ok || !ptx::mbar_wait(&bars[s], (i / kStages) & 1)) ok = false;
                 ok = __all_sync(0xffffffffu, ok) != 0;
                 const uint8_t* st = ring + s * kStage;
@@ -446,29 +426,27 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
     __syncthreads();
 
     // ── join the warps ──────────────────────────────────────────────────────
-    // a lane holds, of rows 8j + 2t and + 1, the channels [D/8·g, +D/8): value
-    // 8x + 2y + e of them is o[4x + y][j][row + 2e]
-    if (warp < W)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
+    // a lane holds, of rows 2t and 2t + 1, the channels [D/8·g, +D/8): value
+    // 8x + 2y + e of them is o[4x + y][row + 2e]
+    if (warp < W) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float ls = l[j][e];
+            float ls = l[e];
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, off);
-            const int r = j * 8 + 2 * t + e;
-            if (g == 0) { sM[warp * kRows + r] = nm[j][e] == kUnseen ? -INFINITY : -nm[j][e]; sL[warp * kRows + r] = ls; }
+            const int r = 2 * t + e;
+            if (g == 0) { sM[warp * kRows + r] = nm[e] == kUnseen ? -INFINITY : -nm[e]; sL[warp * kRows + r] = ls; }
             float* dst = sO + (warp * kRows + r) * D + (D / 8) * g;
 #pragma unroll
             for (int x = 0; x < kMT / 2; ++x)
                 *reinterpret_cast<float4*>(dst + 4 * x) =
-                    make_float4(o[2 * x][j][e], o[2 * x][j][e + 2], o[2 * x + 1][j][e], o[2 * x + 1][j][e + 2]);
+                    make_float4(o[2 * x][e], o[2 * x][e + 2], o[2 * x + 1][e], o[2 * x + 1][e + 2]);
         }
     }
     __syncthreads();
     T* out = static_cast<T*>(p.out);
     auto store = [&](int r, int d, float4 a, float inv) {
-        const int rr = r0 + r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
+        const int rr = r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
         T* dst = out + b * p.o_st[0] + h * p.o_st[1] + qi * p.o_st[2] + d;
         uint2 u;
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
@@ -526,12 +504,12 @@ __global__ void __launch_bounds__(attn_threads(D, NT), NT == 1 ? 2 : 1) kv4_attn
     if (!ok) atomicExch(&g_sfb_device_error, SFB_ERR_DEVICE_TIMEOUT);
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D>
 int launch_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     const DeviceInfo& dev = device_info();
-    constexpr int smem = attn_smem(D, NT);
+    constexpr int smem = attn_smem(D);
     static_assert(smem <= 227 * 1024, "shared memory budget");
-    auto kern = kv4_attn_kernel<T, D, NT>;
+    auto kern = kv4_attn_kernel<T, D>;
     static std::atomic<bool> done[64];             // kernel attributes, once per device (idempotent)
     if (!done[dev.ordinal & 63].load(std::memory_order_acquire)) {
         const cudaError_t e1 = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -543,8 +521,7 @@ int launch_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
         prefer_max_shared(kern);
         done[dev.ordinal & 63].store(true, std::memory_order_release);
     }
-    p.rtiles = (p.R + NT * 8 - 1) / (NT * 8);
-    const int64_t units = static_cast<int64_t>(p.c.B) * p.c.Hkv * p.rtiles;
+    const int64_t units = static_cast<int64_t>(p.c.B) * p.c.Hkv;
     const int blocks = (p.Sk + kBlock - 1) / kBlock;
     int sp = num_splits;
     if (sp == 0) {
@@ -552,7 +529,8 @@ int launch_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
         // where 12 took 56, 4 sessions of 8 heads and 16 k slots). With more units
         // than that, cut the long ones into 4096 slots and more until there are
         // about 1024 CTAs, so that sessions of different lengths fill the SMs
-        // evenly (32 of them: see the table). At least a block a CTA.
+        // evenly (32 of 8 to 16 k slots, 8 heads: 145 µs, 162 without). At least a
+        // block a CTA.
         const int64_t fill = std::max<int64_t>(1, 2 * dev.num_sms / units);
         sp = 1;
         while (sp < 16 && 2 * sp <= fill) sp *= 2;
@@ -560,10 +538,10 @@ int launch_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
         if (fine > sp) sp = static_cast<int>(std::min<int64_t>(fine, 8));
     }
     p.splits = std::min(sp, std::max(1, blocks));
-    if (static_cast<int64_t>(p.c.Hkv) * p.rtiles > 65535 || p.c.B > 65535) return SFB_ERR_SHAPE;
+    if (p.c.Hkv > 65535 || p.c.B > 65535) return SFB_ERR_SHAPE;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.splits, p.c.Hkv * p.rtiles, p.c.B);
-    cfg.blockDim = dim3(attn_threads(D, NT), 1, 1);
+    cfg.gridDim = dim3(p.splits, p.c.Hkv, p.c.B);
+    cfg.blockDim = dim3(attn_threads(D), 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -580,14 +558,11 @@ int launch_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
 
 template <typename T>
 int pick_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
-    if (p.c.D == 64) {
-        if (p.R <= 8) return launch_attn<T, 64, 1>(p, num_splits, s);
-        if (p.R <= 16) return launch_attn<T, 64, 2>(p, num_splits, s);
-        return kv4tc::pick<T>(p, num_splits, s);
-    }
-    if (p.R <= 8) return launch_attn<T, 128, 1>(p, num_splits, s);
-    if (p.R <= 16) return launch_attn<T, 128, 2>(p, num_splits, s);
-    return launch_attn<T, 128, 4>(p, num_splits, s);
+    // Up to 8 rows fill this kernel's N side. 16 rows, here with two such tiles and
+    // there: 16 sessions of 8192 slots of 4 heads, 64 channels 32.5 and 28.8 µs, 128
+    // channels 49.5 and 34.3; one session of 2000 slots 6.5 and 6.5, 9.1 and 7.3 µs.
+    if (p.R > kRows) return kv4tc::pick<T>(p, num_splits, s);
+    return p.c.D == 64 ? launch_attn<T, 64>(p, num_splits, s) : launch_attn<T, 128>(p, num_splits, s);
 }
 
 }  // namespace kv4

@@ -1,24 +1,24 @@
 // kv4_attn_tc.cu — attention over the 4-bit K/V cache on the 5th-generation
-// tensor cores, for more than 16 rows per K/V head (head_dim 64): an action
-// chunk's cross-attention, a prompt chunk, grouped heads. kv4_attn.cu holds the
+// tensor cores, for more than 8 rows per K/V head: an action chunk's
+// cross-attention, a prompt chunk, grouped heads. kv4_attn.cu holds the
 // form for few rows and the definitions (rows, masks, cache).
 //
 // As there, the keys are the MMA's M side. A tile is 128 keys by NQ rows:
 //   Sᵀ[128 keys, NQ] = K · Qᵀ      A = K (fp16) in TMEM, B = Q in shared memory
-//   Oᵀ[64, NQ]      += Vᵀ · Pᵀ     A = Vᵀ, B = Pᵀ, both in shared memory as the
+//   Oᵀ[D, NQ]       += Vᵀ · Pᵀ     A = Vᵀ, B = Pᵀ, both in shared memory as the
 //                                  rows of V and P lie (MN-major)
 // 67 rows of an action chunk then cost 80 columns of exponentials (the bound: 16
 // a clock per SM, 640 clocks a tile) instead of the 128 or 96 lanes that the
 // rows cost as M. A thread of the softmax owns one key, so masks by length or
 // key are one predicate per thread; a thread of the dequantisation owns one
-// key's codes, 32 bytes of K and of V loaded two tiles ahead, and writes K to
-// its TMEM lane and V to its row of shared memory. K in TMEM rather than shared
+// key's codes of 64 channels, 32 bytes of K and of V loaded a tile ahead, and
+// writes K to its TMEM lane and V to its row of shared memory. K in TMEM rather than shared
 // memory: the shared-memory port, at 128 B/clk, is the second bound (dequantised
 // V 16 KB in and out, P 20 KB in and out, Q 10 KB out: 600 clocks a tile).
 //
 // Warps: a softmax group of four for every 16 columns (a thread then holds its
 // key's logits and row sums in registers, S is read once and no column has two
-// owners), four that dequantise, one that issues the MMAs. Sᵀ and Pᵀ are double-
+// owners), four that dequantise for every 64 channels, one that issues the MMAs. Sᵀ and Pᵀ are double-
 // buffered; Sᵀ of tile j + 2 is issued behind P·V of tile j, so that one barrier
 // tells a group both that its logits are there and that its P buffer is free.
 // The reference of a row (the m of exp2(x − m)) is shared by a group's 128
@@ -28,8 +28,14 @@
 // takes the logits out of TMEM twice, or twice the registers: 32 sessions of 67
 // rows by 4374 slots of 32 heads took 324 and 365 µs instead of 268.)
 //
-// TMEM columns: Sᵀ at 96·(tile & 1), Oᵀ at 192, K at 384 + 32·stage. With M = 64
-// the accumulator's row d is in lane 32·(d / 16) + d % 16.
+// Measured: 32 sessions of 67 rows by 4374 slots, 32 heads of 64, 244 µs (315
+// TFLOP/s); one session 15.4 µs; 8 sessions of 16 heads of 128, 48 µs (399). The
+// bound is a tile's chain of waits (S, softmax, P, P·V), about 1900 clocks where
+// the exponents alone are 640: the warps of an SM run it nearly in step, one CTA
+// per SM being all that TMEM, shared memory and registers allow.
+//
+// With M = 64 the accumulator's row d is in lane 32·(d / 16) + d % 16, with 128 in
+// lane d.
 // Every wait is bounded; an expired one records SFB_ERR_DEVICE_TIMEOUT.
 #include "common.cuh"
 #include "sm100_ptx.cuh"
@@ -39,32 +45,38 @@ namespace kv4tc {
 
 constexpr int kC = 16;                            // columns of a softmax group
 __host__ __device__ constexpr int soft_warps(int nq) { return nq / kC * 4; }
-__host__ __device__ constexpr int threads(int nq) { return (soft_warps(nq) + 5) * 32; }   // + 4 dequantising, 1 issuing
-constexpr int kStages = 4;                        // dequantised K / V tiles
+__host__ __device__ constexpr int deq_warps(int d) { return d / 16; }   // four for every 64 channels
+__host__ __device__ constexpr int threads(int d, int nq) { return (soft_warps(nq) + deq_warps(d) + 1) * 32; }   // + 1 issuing
+constexpr int kMaxStages = 4;
+__host__ __device__ constexpr int stages(int d) { return d == 64 ? 4 : 3; }   // dequantised K / V tiles
 constexpr int kKeys = 128;
-constexpr int kVBytes = kKeys * 128;              // fp16 V tile
-constexpr int kPBlock = kKeys * 128;              // 64 columns of P
-constexpr int kMaxQ = 96;
-constexpr int kTmemS = 0, kTmemO = 192, kTmemK = 384;
-constexpr int kOffQ = 0;                                      // [96 rows] × 128 B
-constexpr int kOffV = kOffQ + kMaxQ * 128;
-constexpr int kOffP = kOffV + kStages * kVBytes;              // [tile & 1][2 blocks]
-constexpr int kOffCol = kOffP + 2 * 2 * kPBlock;              // per column: −m, m, alpha, limit
-constexpr int kColBytes = kMaxQ * 4 * (4 + 4);                // and [4 windows] maxima, then row sums
-constexpr int kOffBar = kOffCol + kColBytes;
-constexpr int kNumBars = 2 * kStages + 2 + 2 + 1 + 1;
-constexpr int kOffTmem = kOffBar + 8 * kNumBars;
-constexpr int kSmemBytes = kOffTmem + 16 + 1024;              // + alignment slack
-static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
-static_assert(kMaxQ <= 128 && kOffV % 1024 == 0 && kOffP % 1024 == 0 && kOffCol % 16 == 0 && kOffBar % 8 == 0, "alignment");
-// the partial result of a CTA, over P once every MMA is done: [NQ][64] O, [NQ] m, l
-static_assert(kMaxQ * 64 * 4 + 2 * kMaxQ * 4 <= 4 * kPBlock, "partial fits over P");
+constexpr int kBlock64 = kKeys * 128;             // 64 channels of V, or 64 columns of P, of a tile
+__host__ __device__ constexpr int max_q(int d) { return d == 64 ? 96 : 80; }
+// TMEM columns: Sᵀ of tile j at 96·(j & 1), Oᵀ at 192, K (d / 2 columns a stage) at the end
+constexpr int kTmemS = 0, kTmemO = 192;
+__host__ __device__ constexpr int tmem_k(int d) { return 512 - stages(d) * (d / 2); }
+__host__ __device__ constexpr int v_bytes(int d) { return d / 64 * kBlock64; }
+constexpr int kOffQ = 0;                                      // [D / 64][max_q rows] × 128 B
+__host__ __device__ constexpr int off_v(int d) { return d / 64 * max_q(d) * 128; }
+__host__ __device__ constexpr int off_p(int d) { return off_v(d) + stages(d) * v_bytes(d); }     // [tile & 1][2 blocks]
+__host__ __device__ constexpr int off_col(int d) { return off_p(d) + 2 * 2 * kBlock64; }       // per column: −m, m, alpha, limit
+__host__ __device__ constexpr int off_bar(int d) { return off_col(d) + max_q(d) * 4 * (4 + 4); }   // and [4 windows] maxima, then row sums
+constexpr int kNumBars = 2 * kMaxStages + 2 + 2 + 1 + 1;
+__host__ __device__ constexpr int off_tmem(int d) { return off_bar(d) + 8 * kNumBars; }
+__host__ __device__ constexpr int smem_bytes(int d) { return off_tmem(d) + 16 + 1024; }        // + alignment slack
+__host__ __device__ constexpr bool layout_ok(int d) {
+    return smem_bytes(d) <= 227 * 1024 && kTmemO + max_q(d) <= tmem_k(d) && max_q(d) <= 128 && off_v(d) % 1024 == 0 &&
+           off_p(d) % 1024 == 0 && off_col(d) % 16 == 0 && off_bar(d) % 8 == 0 &&
+           // the partial result of a CTA, over P once every MMA is done: [NQ][D] O, [NQ] m, l
+           max_q(d) * d * 4 + 2 * max_q(d) * 4 <= 4 * kBlock64;
+}
+static_assert(layout_ok(64) && layout_ok(128), "layout");
 
 __host__ __device__ constexpr int bar_ready(int s) { return s; }                // K, V of a stage written
-__host__ __device__ constexpr int bar_free(int s) { return kStages + s; }       // both MMAs of a stage done
-__host__ __device__ constexpr int bar_s(int u) { return 2 * kStages + u; }      // Sᵀ of a tile, u = tile & 1
-__host__ __device__ constexpr int bar_p(int u) { return 2 * kStages + 2 + u; }  // Sᵀ read and Pᵀ written
-constexpr int kBarO = 2 * kStages + 4;                                          // P·V of a tile done
+__host__ __device__ constexpr int bar_free(int s) { return kMaxStages + s; }       // both MMAs of a stage done
+__host__ __device__ constexpr int bar_s(int u) { return 2 * kMaxStages + u; }      // Sᵀ of a tile, u = tile & 1
+__host__ __device__ constexpr int bar_p(int u) { return 2 * kMaxStages + 2 + u; }  // Sᵀ read and Pᵀ written
+constexpr int kBarO = 2 * kMaxStages + 4;                                          // P·V of a tile done
 constexpr int kBarDrain = kBarO + 1;
 constexpr float kUnseen = 1e30f;
 constexpr uint64_t kWaitNs = 1000000000ull, kDrainNs = 100000000ull;
@@ -120,11 +132,14 @@ __device__ __forceinline__ bool bar_or(uint32_t id, bool x) {
         : "=r"(r) : "r"(x ? 1u : 0u), "r"(id) : "memory");
     return r != 0;
 }
-template <typename T, int NQ>
-__global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4AttnParams p) {
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(threads(D, NQ), 1) kv4_attn_tc_kernel(const Kv4AttnParams p) {
     using namespace ptx;
-    constexpr int D = 64, kSoftWarps = soft_warps(NQ), kSoftThreads = kSoftWarps * 32, kThreads = threads(NQ);
-    constexpr int kDeqWarp0 = kSoftWarps, kCtrlWarp = kSoftWarps + 4;
+    constexpr int kSoftWarps = soft_warps(NQ), kSoftThreads = kSoftWarps * 32, kThreads = threads(D, NQ);
+    constexpr int kDeqWarp0 = kSoftWarps, kCtrlWarp = kSoftWarps + deq_warps(D);
+    constexpr int kMaxQ = max_q(D), kVBytes = v_bytes(D), kTmemK = tmem_k(D), kStages = stages(D);
+    constexpr int kOffV = off_v(D), kOffP = off_p(D), kOffCol = off_col(D), kOffBar = off_bar(D), kOffTmem = off_tmem(D);
+    static_assert(NQ <= kMaxQ && kThreads <= 1024, "columns");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // (stays a shared-memory address)
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
@@ -142,7 +157,7 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
     const int rows = static_cast<int>(static_cast<int64_t>(p.R) * (rt + 1) / p.rtiles) - r0;
 
     if (tid == kCtrlWarp * 32) {
-        for (int s = 0; s < kStages; ++s) { mbar_init(&bars[bar_ready(s)], 4); mbar_init(&bars[bar_free(s)], 1); }
+        for (int s = 0; s < kStages; ++s) { mbar_init(&bars[bar_ready(s)], deq_warps(D)); mbar_init(&bars[bar_free(s)], 1); }
         for (int u = 0; u < 2; ++u) {
             mbar_init(&bars[bar_s(u)], 1);
             mbar_init(&bars[bar_p(u)], kSoftWarps);
@@ -170,8 +185,8 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
 
     // ── Q (fp16, 128-byte-swizzled rows; zeros past the last row), columns ──
     bool bad = false;
-    for (int i = tid; i < NQ * 8; i += kThreads) {
-        const int r = i >> 3, c = i & 7;
+    for (int i = tid; i < NQ * (D / 8); i += kThreads) {
+        const int r = i / (D / 8), c = i % (D / 8);
         uint4 u = make_uint4(0, 0, 0, 0);
         if (r < rows) {
             const int rr = r0 + r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
@@ -188,7 +203,7 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
                 if (p.sl2 < 0.f) w[e] ^= 0x80008000u;      // the kernel's scale is |scale|
             }
         }
-        *reinterpret_cast<uint4*>(smem + kOffQ + r * 128 + ((c ^ (r & 7)) << 4)) = u;
+        *reinterpret_cast<uint4*>(smem + kOffQ + (c >> 3) * kMaxQ * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = u;
     }
     if (tid < NQ) {
         lim[tid] = tid < rows ? limit(r0 + tid) : kend;
@@ -207,34 +222,42 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
     float* pL = pM + kMaxQ;
 
     if (warp >= kDeqWarp0 && warp < kCtrlWarp) {
-        // ── dequantisation: thread = key ────────────────────────────────────
-        const int key_in = (warp - kDeqWarp0) * 32 + lane;
-        const uint32_t lane_off = static_cast<uint32_t>((warp - kDeqWarp0) * 32) << 16;
+        // ── dequantisation: thread = key and 64 channels of it ──────────────
+        const int key_in = ((warp - kDeqWarp0) & 3) * 32 + lane, part = (warp - kDeqWarp0) >> 2;
+        const uint32_t lane_off = static_cast<uint32_t>(((warp - kDeqWarp0) & 3) * 32) << 16;
         const int64_t first = static_cast<int64_t>(t_begin) * kKeys + key_in;
-        const uint8_t* kp = p.c.kc + b * p.c.code_sb + hk * p.c.code_sh + first * (D / 2);
-        const uint8_t* vp = p.c.vc + b * p.c.code_sb + hk * p.c.code_sh + first * (D / 2);
-        const __half2* ksp = reinterpret_cast<const __half2*>(p.c.ks + b * p.c.sc_sb + hk * p.c.sc_sh) + first;
-        const __half2* vsp = reinterpret_cast<const __half2*>(p.c.vs + b * p.c.sc_sb + hk * p.c.sc_sh) + first;
+        int64_t co = b * p.c.code_sb + hk * p.c.code_sh + first * (D / 2) + part * 32;      // of the tile to load
+        int64_t so = b * p.c.sc_sb + hk * p.c.sc_sh + (first * (D / 64) + part) * 2;
+        int lkey = t_begin * kKeys + key_in;
         struct RawRow { uint4 k0, k1, v0, v1; __half2 ks, vs; };
         // a slot that is not seen is not read; its codes stand for 0 · 0
-        auto load = [&](RawRow& r, int j) {
-            const int key = (t_begin + j) * kKeys + key_in;
+        auto load = [&](RawRow& r) {
             r.k0 = r.k1 = r.v0 = r.v1 = make_uint4(0, 0, 0, 0);
             r.ks = r.vs = __float2half2_rn(0.f);
-            if (key < kend && (mask == nullptr || mask[key] != 0)) {
-                const int64_t o = static_cast<int64_t>(j) * kKeys;
-                const uint4* k4 = reinterpret_cast<const uint4*>(kp + o * (D / 2));
-                const uint4* v4 = reinterpret_cast<const uint4*>(vp + o * (D / 2));
+            if (lkey < kend && (mask == nullptr || mask[lkey] != 0)) {
+                const uint4* k4 = reinterpret_cast<const uint4*>(p.c.kc + co);
+                const uint4* v4 = reinterpret_cast<const uint4*>(p.c.vc + co);
                 r.k0 = k4[0]; r.k1 = k4[1]; r.v0 = v4[0]; r.v1 = v4[1];
-                r.ks = ksp[o]; r.vs = vsp[o];
-                if (key >= kfull) kv4::contain(r.ks, r.vs);
+                r.ks = *reinterpret_cast<const __half2*>(p.c.ks + so); r.vs = *reinterpret_cast<const __half2*>(p.c.vs + so);
             }
+            co += kKeys * (D / 2); so += kKeys * (D / kv4::kGroup); lkey += kKeys;
         };
         RawRow nxt;
-        if (ntl > 0) load(nxt, 0);
+        if (ntl > 0) load(nxt);
         for (int j = 0; j < ntl; ++j) {
-                const RawRow r = nxt;
-                if (j + 1 < ntl) load(nxt, j + 1);
+                RawRow r = nxt;
+                if (j + 1 < ntl) load(nxt);
+                if ((t_begin + j + 1) * kKeys > kfull) {           // slots that only some rows see
+                    const int key = (t_begin + j) * kKeys + key_in;
+                    if (key >= kfull && key < kend) {
+                        kv4::contain(r.ks, r.vs);
+                        if constexpr (D > 64) {                    // (the other half's V makes K NaN too)
+                            __half2 v = *reinterpret_cast<const __half2*>(
+                                p.c.vs + b * p.c.sc_sb + hk * p.c.sc_sh + (static_cast<int64_t>(key) * (D / 64) + 1 - part) * 2);
+                            kv4::contain(r.ks, v);
+                        }
+                    }
+                }
                 const int s = j % kStages;
                 if (j >= kStages) {
                     // (stages ahead of the MMAs: this wait is the long one, and not urgent)
@@ -254,9 +277,9 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
 #pragma unroll
                         for (int i = 0; i < 4; ++i) kf[4 * x + i] = d4[i];
                     }
-                    tmem_st16(tmem + kTmemK + 32 * s + 16 * h + lane_off, kf);
+                    tmem_st16(tmem + kTmemK + (D / 2) * s + 32 * part + 16 * h + lane_off, kf);
                 }
-                uint8_t* vrow = smem + kOffV + s * kVBytes + key_in * 128;
+                uint8_t* vrow = smem + kOffV + s * kVBytes + part * kBlock64 + key_in * 128;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint4 w = h ? r.v1 : r.v0;
@@ -280,16 +303,16 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
         if (ntl > 0) {
             // ── MMA issue ───────────────────────────────────────────────────
             constexpr uint32_t idS = idesc_f16(128, NQ, 0, 0, 0);       // K(tmem) · Qᵀ, both K-major
-            constexpr uint32_t idO = idesc_f16(64, NQ, 0, 1, 1);        // Vᵀ · Pᵀ, both MN-major
+            constexpr uint32_t idO = idesc_f16(D, NQ, 0, 1, 1);        // Vᵀ · Pᵀ, both MN-major
             const uint32_t aq = smem_u32(smem + kOffQ);
             auto issue_s = [&](int j) {
                 const int s = j % kStages;
                 tc_fence_after_sync();
                 if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_f16_ts(tmem + kTmemS + 96 * (j & 1), tmem + kTmemK + 32 * s + 8 * kk,
-                                   smem_desc_sw128(aq + kk * 32, 16, 1024), idS, kk > 0 ? 1u : 0u);
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        mma_f16_ts(tmem + kTmemS + 96 * (j & 1), tmem + kTmemK + (D / 2) * s + 8 * kk,
+                                   smem_desc_sw128(aq + (kk >> 2) * kMaxQ * 128 + (kk & 3) * 32, 16, 1024), idS, kk > 0 ? 1u : 0u);
                     mma_commit(&bars[bar_s(j & 1)]);
                 }
                 __syncwarp();
@@ -298,12 +321,12 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
                 const int s = j % kStages;
                 tc_fence_after_sync();
                 const uint32_t av = smem_u32(smem + kOffV + s * kVBytes);
-                const uint32_t ap = smem_u32(smem + kOffP + (j & 1) * 2 * kPBlock);
+                const uint32_t ap = smem_u32(smem + kOffP + (j & 1) * 2 * kBlock64);
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        mma_f16_ss(tmem + kTmemO, smem_desc_sw128(av + k * 2048, kVBytes, 1024),
-                                   smem_desc_sw128(ap + k * 2048, kPBlock, 1024), idO, (j > 0 || k > 0) ? 1u : 0u);
+                        mma_f16_ss(tmem + kTmemO, smem_desc_sw128(av + k * 2048, kBlock64, 1024),
+                                   smem_desc_sw128(ap + k * 2048, kBlock64, 1024), idO, (j > 0 || k > 0) ? 1u : 0u);
                     mma_commit(&bars[bar_free(s)]);
                     mma_commit(&bars[kBarO]);
                 }
@@ -341,7 +364,7 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int c = 2 * grp + i;
-            poff[i] = kOffP + (c >> 3) * kPBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+            poff[i] = kOffP + (c >> 3) * kBlock64 + row * 128 + (((c & 7) ^ (row & 7)) << 4);
         }
         float2 l[kC / 2];
 #pragma unroll
@@ -381,10 +404,7 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
                 tmem_ld_wait();
                 if (edge) hide();
                 {
-                    float v[kC];
-#pragma unroll
-                    for (int i = 0; i < kC; ++i) v[i] = x[i];
-                    const float mx = reduce16(v, lane, [](float a, float c) { return fmaxf(a, c); });
+                    const float mx = reduce16(x, lane, [](float a, float c) { return fmaxf(a, c); });
                     if (lane < kC) wred[win * kMaxQ + c0 + lane] = mx;
                 }
                 named_bar_sync(1 + grp, 128);
@@ -419,6 +439,9 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
                     tmem_st_wait();
                 }
                 named_bar_sync(1 + grp, 128);                       // alpha is read before it is written again
+                tmem_ld16(tS + 96 * u, x);                          // (again: registers)
+                tmem_ld_wait();
+                if (edge) hide();
                 to_exponents();
             }
             // P = 2^(x·sl2 − m), row sums, fp16 P into this key's row
@@ -431,7 +454,7 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
                     l[(i + e) / 2] = add2(l[(i + e) / 2], p0);
                     h[e / 2] = kv4::h2u(__floats2half2_rn(p0.x, p0.y));
                 }
-                *reinterpret_cast<uint4*>(smem + poff[i / 8] + u * 2 * kPBlock) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4*>(smem + poff[i / 8] + u * 2 * kBlock64) = make_uint4(h[0], h[1], h[2], h[3]);
             }
             fence_proxy_async_smem();
             tc_fence_before_sync();
@@ -451,12 +474,12 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
         tc_fence_after_sync();
         named_bar_sync(7, kSoftThreads);
         {
-            // lanes 0..15 hold row d of Oᵀ
-            const int d = 16 * win + (lane & 15);
+            // with M = 64 lanes 0..15 hold row d of Oᵀ, with 128 all do
+            const int d = D == 64 ? 16 * win + (lane & 15) : row;
             float a[kC];
             tmem_ld16(tO, a);
             tmem_ld_wait();
-            if (lane < 16) {
+            if (D > 64 || lane < 16) {
 #pragma unroll
                 for (int i = 0; i < kC; ++i) pO[(c0 + i) * D + d] = ntl > 0 ? a[i] : 0.f;
             }
@@ -521,13 +544,13 @@ __global__ void __launch_bounds__(threads(NQ), 1) kv4_attn_tc_kernel(const Kv4At
     }
 }
 
-template <typename T, int NQ>
+template <typename T, int D, int NQ>
 int launch(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     const DeviceInfo& dev = device_info();
-    auto kern = kv4_attn_tc_kernel<T, NQ>;
+    auto kern = kv4_attn_tc_kernel<T, D, NQ>;
     static std::atomic<bool> done[64];             // kernel attributes, once per device (idempotent)
     if (!done[dev.ordinal & 63].load(std::memory_order_acquire)) {
-        const cudaError_t e1 = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        const cudaError_t e1 = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(D));
         const cudaError_t e2 = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e1 != cudaSuccess || e2 != cudaSuccess) {
             record_cuda_error(e1 != cudaSuccess ? e1 : e2, "kv4 attention attributes");
@@ -549,8 +572,8 @@ int launch(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     if (static_cast<int64_t>(p.c.Hkv) * p.rtiles > 65535 || p.c.B > 65535) return SFB_ERR_SHAPE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.splits, p.c.Hkv * p.rtiles, p.c.B);
-    cfg.blockDim = dim3(threads(NQ), 1, 1);
-    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.blockDim = dim3(threads(D, NQ), 1, 1);
+    cfg.dynamicSmemBytes = smem_bytes(D);
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -569,9 +592,11 @@ template <typename T>
 int pick(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     auto cost = [&](int nq) { return static_cast<int64_t>((p.R + nq - 1) / nq) * (nq + 16); };
     const int64_t c48 = cost(48), c80 = cost(80), c96 = cost(96);
-    if (c96 <= c80 && c96 <= c48) return launch<T, 96>(p, num_splits, s);
-    if (c80 <= c48) return launch<T, 80>(p, num_splits, s);
-    return launch<T, 48>(p, num_splits, s);
+    if (p.R <= 16) return p.c.D == 128 ? launch<T, 128, 16>(p, num_splits, s) : launch<T, 64, 16>(p, num_splits, s);
+    if (p.c.D == 128) return c80 <= c48 ? launch<T, 128, 80>(p, num_splits, s) : launch<T, 128, 48>(p, num_splits, s);
+    if (c96 <= c80 && c96 <= c48) return launch<T, 64, 96>(p, num_splits, s);
+    if (c80 <= c48) return launch<T, 64, 80>(p, num_splits, s);
+    return launch<T, 64, 48>(p, num_splits, s);
 }
 
 }  // namespace kv4tc
