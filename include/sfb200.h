@@ -477,7 +477,8 @@ int sfb_rdt1b_tick_stats(void* handle, int64_t* ticks, int64_t* encodes);
 int sfb_rdt1b_set_path(void* handle, int32_t path);
 /* Form of the cross-attention K/V cache: 16 (the default: K bf16, V fp16) or 4
  * (sfb_kv4_cache; 72 bytes a token and head instead of 256, at the accuracy
- * of 4 bits). The first change to 4 allocates the 4-bit caches (setup time).
+ * of 4 bits). The first change to 4 allocates the 4-bit caches (setup time); the
+ * 16-bit ones stay, so that it can be changed back.
  * Drops the captured graphs and the tick's condition: encode again before the
  * next forward or sample, which otherwise return SFB_ERR_INVALID. With 4 bits
  * every session count takes the per-projection kernels (path 1). No counterpart

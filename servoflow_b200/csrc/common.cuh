@@ -5,6 +5,7 @@
 #pragma once
 
 #include <atomic>
+#include <new>
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>

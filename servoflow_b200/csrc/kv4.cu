@@ -267,7 +267,7 @@ int kv4_append_launch(const sfb_kv4_cache* cache, const void* k, const int64_t* 
     Kv4MoveParams p{};
     SFB_TRY(kv4_cache_check(cache, p.c));
     if (dtype != SFB_F32 && dtype != SFB_F16 && dtype != SFB_BF16) return SFB_ERR_DTYPE;
-    if (seq < 0) return SFB_ERR_SHAPE;
+    if (seq < 0 || seq > 0x7fffff00) return SFB_ERR_SHAPE;
     // without per-session starts the slots are known here
     if (start == nullptr && (slot0 < 0 || static_cast<int64_t>(slot0) + seq > cache->capacity)) return SFB_ERR_SHAPE;
     if (p.c.B == 0 || seq == 0) return SFB_OK;

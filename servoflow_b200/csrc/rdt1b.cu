@@ -989,7 +989,11 @@ int sfb_rdt1b_set_cache(void* handle, int32_t bits) {
     if (m == nullptr || (bits != 16 && bits != 4)) return SFB_ERR_INVALID;
     SFB_MODEL_ENTRY(m);
     if (bits == m->cache_bits) return SFB_OK;
-    if (bits == 4) SFB_TRY(rdt::alloc_kv4(*m));
+    try {
+        if (bits == 4) SFB_TRY(rdt::alloc_kv4(*m));
+    } catch (const std::bad_alloc&) {
+        return SFB_ERR_CUDA;
+    }
     // captured graphs hold the other cache's kernels
     cudaError_t e = cudaStreamSynchronize(m->own);
     for (auto& g : m->graphs) cudaGraphExecDestroy(g.second);

@@ -117,7 +117,7 @@ BAD_CACHES = [
     (dict(k_codes=0), _capi.SFB_ERR_INVALID), (dict(v_scale=0), _capi.SFB_ERR_INVALID),
     (dict(head_dim=96), _capi.SFB_ERR_SHAPE), (dict(head_dim=0), _capi.SFB_ERR_SHAPE),
     (dict(heads_kv=0), _capi.SFB_ERR_SHAPE), (dict(capacity=-1), _capi.SFB_ERR_SHAPE),
-    (dict(capacity=66), _capi.SFB_ERR_SHAPE),
+    (dict(capacity=66), _capi.SFB_ERR_SHAPE), (dict(capacity=0x7ffffffc), _capi.SFB_ERR_SHAPE),
     (dict(k_codes=0x1008), _capi.SFB_ERR_ALIGN), (dict(v_scale=0x1002), _capi.SFB_ERR_ALIGN),
     ({"code_stride[1]": 2056}, _capi.SFB_ERR_ALIGN), ({"scale_stride[0]": 514}, _capi.SFB_ERR_ALIGN),
 ]
@@ -154,6 +154,9 @@ def test_append_and_read_refusals():
     assert append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 1, 64) == E.SFB_ERR_SHAPE
     assert append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 1, -1) == E.SFB_ERR_SHAPE
     assert append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 2 ** 31 - 1, 2 ** 31 - 1) == E.SFB_ERR_SHAPE
+    assert append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 2 ** 31 - 1, 0) == E.SFB_ERR_SHAPE
+    # with per-session starts the slots are known on the device alone
+    assert lib.sfb_kv4_append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 2 ** 31 - 1, 0x2000, 0, None, None) == E.SFB_ERR_SHAPE
     assert append(c, 0x2008, st, 0x2000, st, E.SFB_BF16, 1, 0) == E.SFB_ERR_ALIGN
     assert append(c, 0x2000, st, 0x2000, odd, E.SFB_BF16, 1, 0) == E.SFB_ERR_ALIGN
     assert append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 0, 0) == E.SFB_OK              # nothing to do

@@ -39,6 +39,10 @@ def held(s):
     for l in range(s["cfg"].num_layers):
         n = s["cfg"].max_lang_len if l % 2 == 0 else s["cfg"].img_len
         k, v = (x[:, :, :n].transpose(1, 2).reshape(2, n, -1).float().cpu() for x in s["model"].kv4_cache(l).dequantize())
+        if l % 2 == 0:                                 # slots past a session's length are never written
+            for b, n in enumerate(s["lens"].tolist()):
+                k[b, n:] = 0
+                v[b, n:] = 0
         out.append((k, v))
     return out
 
