@@ -26,10 +26,10 @@
 // than 8: a comparison a value with one vote of the group finds that out.
 // (The vote of a tile cast one tile ahead, so that no warp waits for the others',
 // takes the logits out of TMEM twice, or twice the registers: 32 sessions of 67
-// rows by 4374 slots of 32 heads took 324 and 365 µs instead of 268.)
+// rows by 4374 slots of 32 heads took 324 and 365 µs.)
 //
-// Measured: 32 sessions of 67 rows by 4374 slots, 32 heads of 64, 244 µs (315
-// TFLOP/s); one session 15.4 µs; 8 sessions of 16 heads of 128, 48 µs (399). The
+// Measured: 32 sessions of 67 rows by 4374 slots, 32 heads of 64, 244 to 272 µs
+// from one GPU to another (315 to 281 TFLOP/s); one session 15.4 µs; 8 sessions of 16 heads of 128, 48 µs (399). The
 // bound is a tile's chain of waits (S, softmax, P, P·V), about 1900 clocks where
 // the exponents alone are 640: the warps of an SM run it nearly in step, one CTA
 // per SM being all that TMEM, shared memory and registers allow.
@@ -564,7 +564,9 @@ int launch(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     const int tiles = (p.Sk + kKeys - 1) / kKeys;
     int sp = num_splits;
     if (sp == 0) {
-        // as many as keep every CTA in one wave (one per SM), two tiles each at least
+        // as many as keep every CTA in one wave (one per SM), two tiles each at least.
+        // (More, where one wave is passed by little: 176 row tiles of 17 key tiles took
+        // 54 µs in three rounds of halves instead of 48 in two.)
         sp = static_cast<int>(std::min<int64_t>(16, std::max<int64_t>(1, dev.num_sms / units)));
         sp = std::min(sp, std::max(1, tiles / 2));
     }
