@@ -566,7 +566,7 @@ int launch(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     if (sp == 0) {
         // as many as keep every CTA in one wave (one per SM), two tiles each at least.
         // (More, where one wave is passed by little: 176 row tiles of 17 key tiles took
-        // 54 µs in three rounds of halves instead of 48 in two.)
+        // 54 µs in three rounds of halves, 48 in two rounds.)
         sp = static_cast<int>(std::min<int64_t>(16, std::max<int64_t>(1, dev.num_sms / units)));
         sp = std::min(sp, std::max(1, tiles / 2));
     }
@@ -589,12 +589,21 @@ int launch(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     return SFB_OK;
 }
 
-// The column count that pads the equal row tiles least.
+// The column count that takes the least time: rounds of the SMs (or the share of a
+// round that splitting a CTA's keys leaves) times a tile's, which grows as nq + 88
+// (16 × 32 units of 40 rows: 126 µs with 48 columns, 150 with 80; 2060 rows of 8
+// units: 43.6 µs with 80, 47.7 with 96, 51.9 with 48; 67 rows of 32 units: 15.6 µs
+// with 80, 17.7 with 48, of 1024 units 271 and 427).
 template <typename T>
 int pick(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
-    auto cost = [&](int nq) { return static_cast<int64_t>((p.R + nq - 1) / nq) * (nq + 16); };
-    const int64_t c48 = cost(48), c80 = cost(80), c96 = cost(96);
     if (p.R <= 16) return p.c.D == 128 ? launch<T, 128, 16>(p, num_splits, s) : launch<T, 64, 16>(p, num_splits, s);
+    const int64_t sms = std::max(device_info().num_sms, 1);
+    auto cost = [&](int nq) {
+        const int64_t units = std::max<int64_t>(1, static_cast<int64_t>((p.R + nq - 1) / nq) * p.c.B * p.c.Hkv);
+        const double rounds = units <= sms ? 1.0 / std::min<int64_t>(16, sms / units) : static_cast<double>((units + sms - 1) / sms);
+        return rounds * (nq + 88);
+    };
+    const double c48 = cost(48), c80 = cost(80), c96 = cost(96);
     if (p.c.D == 128) return c80 <= c48 ? launch<T, 128, 80>(p, num_splits, s) : launch<T, 128, 48>(p, num_splits, s);
     if (c96 <= c80 && c96 <= c48) return launch<T, 64, 96>(p, num_splits, s);
     if (c80 <= c48) return launch<T, 64, 80>(p, num_splits, s);

@@ -204,11 +204,12 @@ int launch(NormRopeParams& p, cudaStream_t s) {
 
 template <typename T, int kLanes>
 int pick_rot(NormRopeParams& p, bool inter, cudaStream_t s) {
-    // Four heads per thread once that still leaves half the GPU's threads busy:
-    // four loads in flight each, the angles' loads and the index arithmetic a
-    // quarter. One head per thread below that, where a call is latency.
+    // Four heads per thread once one per thread would be 1536 threads an SM: four
+    // loads in flight each, the angles' loads and the index arithmetic a quarter.
+    // Below that a call is latency. 64 heads of 64, one and four heads per thread: 4
+    // × 67 tokens 2.7 and 3.4 µs, 32 × 16 tokens 3.6 and 3.0, 32 × 67 11.2 and 7.9.
     const int64_t one = static_cast<int64_t>(p.tokens) * (p.side[0].heads + p.side[1].heads) * kLanes;
-    const bool many = one >= static_cast<int64_t>(std::max(device_info().num_sms, 1)) * 1024 * 4;
+    const bool many = one >= static_cast<int64_t>(std::max(device_info().num_sms, 1)) * 1536;
     if (p.rot == 0) return many ? launch<T, kLanes, 4, 0>(p, s) : launch<T, kLanes, 1, 0>(p, s);
     if (inter) return many ? launch<T, kLanes, 4, 2>(p, s) : launch<T, kLanes, 1, 2>(p, s);
     return many ? launch<T, kLanes, 4, 1>(p, s) : launch<T, kLanes, 1, 1>(p, s);

@@ -469,7 +469,8 @@ int pick_nt(const W4Params& p, int act, cudaStream_t s) {
         return two ? few<T, G, 2, 2>(p, act, s)
                    : few<T, G, 2, 1>(p, act, s);
     }
-    // 64 channels a CTA once those fill half the SMs
+    // 64 channels a CTA once those fill half the SMs. 67 rows, 2048 inputs, 64 and 32
+    // channels a CTA: 4096 outputs 18.3 and 14.3 µs, 6144 20.9 and 27.0.
     const int64_t tiles = (static_cast<int64_t>(p.M) + 71) / 72;
     const bool wide = (p.N + 63) / 64 * tiles * 2 >= std::max(device_info().num_sms, 1);
     if (p.M <= 32) return wide ? many<T, G, 4, 4>(p, act, s)
