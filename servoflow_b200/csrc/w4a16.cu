@@ -24,9 +24,10 @@
 //
 // Measured: one row of 16384 × 8192, groups of 128, 26.6 µs (2.6 TB/s of codes and
 // scales); one of 2048² 3.0 µs; 8 of 8192² 19.2 µs; 67 of 6144 × 2048 20.1 µs. What
-// bounds few rows is the issue of instructions, about 150 a KB of codes: more bytes
-// in flight (warp-private rings of asynchronous copies, 4 stages deep) gave 24.3,
-// 3.8 and 20.8 µs for the first three.
+// bounds few rows is the loads' latency and the issue of instructions together, 165
+// a KB of codes in 43 % of the slots: more bytes in flight (warp-private rings of
+// asynchronous copies, 4 stages deep, 204 a KB) gave 24.3, 3.8 and 20.8 µs for the
+// first three.
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 
