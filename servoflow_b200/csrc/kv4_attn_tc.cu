@@ -61,7 +61,7 @@ __host__ __device__ constexpr int off_v(int d) { return d / 64 * max_q(d) * 128;
 __host__ __device__ constexpr int off_p(int d) { return off_v(d) + stages(d) * v_bytes(d); }     // [tile & 1][2 blocks]
 __host__ __device__ constexpr int off_col(int d) { return off_p(d) + 2 * 2 * kBlock64; }       // per column: −m, m, alpha, limit
 __host__ __device__ constexpr int off_bar(int d) { return off_col(d) + max_q(d) * 4 * (4 + 4); }   // and [4 windows] maxima, then row sums
-constexpr int kNumBars = 2 * kMaxStages + 2 + 2 + 1 + 1;
+constexpr int kNumBars = 2 * kMaxStages + 2 + 2 + 1 + 1 + 1;
 __host__ __device__ constexpr int off_tmem(int d) { return off_bar(d) + 8 * kNumBars; }
 __host__ __device__ constexpr int smem_bytes(int d) { return off_tmem(d) + 16 + 1024; }        // + alignment slack
 __host__ __device__ constexpr bool layout_ok(int d) {
@@ -77,7 +77,8 @@ __host__ __device__ constexpr int bar_free(int s) { return kMaxStages + s; }    
 __host__ __device__ constexpr int bar_s(int u) { return 2 * kMaxStages + u; }      // Sᵀ of a tile, u = tile & 1
 __host__ __device__ constexpr int bar_p(int u) { return 2 * kMaxStages + 2 + u; }  // Sᵀ read and Pᵀ written
 constexpr int kBarO = 2 * kMaxStages + 4;                                          // P·V of a tile done
-constexpr int kBarDrain = kBarO + 1;
+constexpr int kBarDone = kBarO + 1;                                                // P·V of the last tile done
+constexpr int kBarDrain = kBarDone + 1;                                            // every MMA issued is done
 constexpr float kUnseen = 1e30f;
 constexpr uint64_t kWaitNs = 1000000000ull, kDrainNs = 100000000ull;
 
@@ -163,6 +164,7 @@ __global__ void __launch_bounds__(threads(D, NQ), 1) kv4_attn_tc_kernel(const Kv
             mbar_init(&bars[bar_p(u)], kSoftWarps);
         }
         mbar_init(&bars[kBarO], 1);
+        mbar_init(&bars[kBarDone], 1);
         mbar_init(&bars[kBarDrain], 1);
         fence_mbarrier_init();
     }
@@ -349,7 +351,10 @@ __global__ void __launch_bounds__(threads(D, NQ), 1) kv4_attn_tc_kernel(const Kv
                 if (nx < ntl && wait_all(bar_ready(nx % kStages), (nx / kStages) & 1)) issue_s(nx);
             }
             // every MMA is done before TMEM and shared memory are let go
-            if (elect_one()) mma_commit(&bars[kBarDrain]);
+            if (elect_one()) {
+                if (ok) mma_commit(&bars[kBarDone]);
+                mma_commit(&bars[kBarDrain]);
+            }
             __syncwarp();
             if (!mbar_wait(&bars[kBarDrain], 0, kDrainNs)) ok = false;
         }
@@ -427,7 +432,9 @@ __global__ void __launch_bounds__(threads(D, NQ), 1) kv4_attn_tc_kernel(const Kv
                     l[i].x *= al.x; l[i].y *= al.y;
                 }
                 if (j > 0) {
-                    wait(kBarO, (j - 1) & 1);                       // the accumulator is at rest
+                    // the accumulator is at rest (P·V of tile j − 2 is done, its commit
+                    // came before that of S: one phase at most is open)
+                    wait(kBarO, (j - 1) & 1);
                     tc_fence_after_sync();
                     float a[kC];
                     tmem_ld16(tO, a);
@@ -469,8 +476,12 @@ __global__ void __launch_bounds__(threads(D, NQ), 1) kv4_attn_tc_kernel(const Kv
             const float t = reduce16(v, lane, [](float a, float c) { return a + c; });
             if (lane < kC) wred[win * kMaxQ + c0 + lane] = t;
         }
-        // every P·V is done: P's memory becomes the partial result
-        if (ntl >= 1) wait(kBarO, (ntl - 1) & 1);
+        // every P·V is done: P's memory becomes the partial result. kBarDone has one
+        // phase. kBarO cannot say this: here P·V of tile ntl − 3 is known to be done
+        // (S of tile ntl − 1 was committed behind it) and no later one, so kBarO may be
+        // two phases short of ntl, where a wait for the last one's parity is answered
+        // by the phase two before it.
+        if (ntl > 0) wait(kBarDone, 0);
         tc_fence_after_sync();
         named_bar_sync(7, kSoftThreads);
         {

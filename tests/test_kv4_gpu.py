@@ -421,3 +421,17 @@ def test_nan_slots_do_not_reach_rows_before_them(be, gpu, D, Sq, Sk):
         assert torch.equal(out[:, :, ~sees], clean[:, :, ~sees])
         assert out[:, :, sees].isnan().any(-1).all()
     assert be.device_error() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sk", [100, 256, 300, 512])
+@pytest.mark.parametrize("Sq", [16, 40, 75, 90])
+def test_few_key_tiles_a_cta(be, gpu, D, Sk, Sq):
+    """One to four tiles of 128 slots in a CTA (no splits), where the last products are
+    the only ones in flight when the softmax is done with its last tile; 100 CTAs of every
+    row form (16, 48, 80 and, with 64 channels, 96 rows on 148 SMs), the same bits every time."""
+    q, cache, out = run_attn(be, gpu, 4, 25, 25, Sq, Sk, D, torch.bfloat16, splits=1, seed=Sq + Sk)
+    again = torch.empty_like(out)
+    for _ in range(20):
+        be.kv4_attention(q, cache, again.fill_(0), seq_k=Sk, num_splits=1)
+        assert torch.equal(out, again)
