@@ -18,7 +18,7 @@
 // ones) and the index arithmetic. Blocks of q come before blocks of k, so that
 // which of the two a thread works on costs nothing per head.
 // Measured: 32 × 67 tokens of 32 + 32 heads of 64, 7.9 µs; 2 × 4374 tokens of 32 +
-// 8 heads of 128, 35.0 µs (5.2 TB/s, 80 % of a copy's rate); one token 1.5 µs.
+// 8 heads of 128, 35.1 µs (5.2 TB/s, 79 % of a copy's rate); one token 1.5 µs.
 #include "common.cuh"
 
 namespace sfb {
@@ -123,16 +123,19 @@ norm_rope_kernel(const NormRopeParams p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) g[i] = 1.f;
     if (sd.w != nullptr && act) load8(static_cast<const T*>(sd.w) + d0, g);
-    // the token's angles: 8 (half-split) or 4 (interleaved) pairs for this lane;
-    // cosine 1 and sine 0 past the rotated channels
+    // the token's angles: 8 (half-split) or 4 (interleaved) pairs for this lane. Lanes
+    // past the rotated channels take no part: a product with a sine of 0 would make
+    // NaN of an infinity there, and of its neighbour. (Left out by selecting the result
+    // where pairs are interleaved, by a branch where halves are paired: the other way
+    // round 2 × 4374 tokens of 40 heads took 35.9 µs for 35.1, 32 × 67 tokens 8.5 for 7.8.)
     float c[8], sn[8];
     bool bad = false;
-    const bool first = d0 < p.rot / 2;
+    const bool first = d0 < p.rot / 2, turns = d0 < p.rot;
     if constexpr (kRot != 0) {
         bad = pos < 0 || pos >= p.table_len;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { c[i] = 1.f; sn[i] = 0.f; }
-        if (d0 < p.rot && !bad) {
+        for (int i = 0; i < 8; ++i) c[i] = sn[i] = 0.f;
+        if (turns && !bad) {
             const int64_t base = pos * (p.rot / 2);
             if constexpr (kRot == 2) {
                 const float4 cc = *reinterpret_cast<const float4*>(p.cos_t + base + d0 / 2);
@@ -150,7 +153,7 @@ norm_rope_kernel(const NormRopeParams p) {
     }
     // the lane of the pair's other half (this one where nothing is rotated)
     const int lane = threadIdx.x & 31, hop = p.rot / 16;
-    const int peer = d0 < p.rot ? (first ? lane + hop : lane - hop) : lane;
+    const int peer = turns ? (first ? lane + hop : lane - hop) : lane;
     T* dst = static_cast<T*>(sd.out) + b * sd.so[0] + h0 * ho + s * sd.so[2] + d0;
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
@@ -169,14 +172,14 @@ norm_rope_kernel(const NormRopeParams p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float a = f[2 * i], bb = f[2 * i + 1];
-                f[2 * i]     = a * c[i] - bb * sn[i];
-                f[2 * i + 1] = bb * c[i] + a * sn[i];
+                f[2 * i]     = turns ? a * c[i] - bb * sn[i] : a;
+                f[2 * i + 1] = turns ? bb * c[i] + a * sn[i] : bb;
             }
         } else if constexpr (kRot == 1) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float o = __shfl_sync(0xffffffffu, f[i], peer);
-                f[i] = f[i] * c[i] + o * sn[i];
+                if (turns) f[i] = f[i] * c[i] + o * sn[i];
             }
         }
         if (j < nh && !bad) store8(dst + j * ho, f);

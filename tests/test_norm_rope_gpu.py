@@ -174,3 +174,27 @@ def test_wrapper_refusals(be, gpu):
         be.qk_norm_rope(q, None, q, None, cos=cos.cpu(), sin=sin.cpu())
     with pytest.raises(ValueError):
         be.qk_norm_rope(q, None, q, None, layout="hbsd")
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D,rot", [(64, 32), (128, 16), (256, 96), (72, 64)])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("B,S", [(1, 3), (40, 100)])
+def test_channels_past_the_rotated_ones_pass_through(be, gpu, dt, D, rot, inter, B, S):
+    """The rotation covers the first rotary_dim channels: without a norm the others are
+    copies, infinities, NaN and the sign of a zero included, and touch no neighbour."""
+    H = 16                                             # 40 x 100 tokens take four heads a thread
+    x = torch.randn(B, S, H, D, generator=torch.Generator().manual_seed(D)).to(dt).to(gpu)
+    x[:, :, 0, rot] = float("inf")
+    x[:, :, 1, D - 1] = -float("inf")
+    x[:, :, 2, rot + 3] = float("nan")
+    x[:, :, H - 1, rot + 4] = -0.0
+    out = torch.empty_like(x)
+    cos, sin = tables(S, rot, gpu)
+    be.qk_norm_rope(x, None, out, None, cos=cos, sin=sin, norm=False, interleaved=inter, layout="bshd")
+    bits = torch.int32 if dt == torch.float32 else torch.int16
+    same = (out.view(bits) == x.view(bits)) | (out.isnan() & x.isnan())
+    assert same[..., rot:].all()
+    pos = torch.arange(S, device=gpu).expand(B, S)
+    ref, size = ref64(x, None, cos, sin, pos, 0.0, inter, norm=False)
+    check(out[..., :rot], ref[..., :rot], size[..., :rot], dt)
