@@ -126,7 +126,8 @@ struct Model {
     int32_t* lang_len;
     std::vector<__nv_bfloat16*> kv;
     // the cache's form: 16 bits in `kv`, or 4 bits in `kv4` (made by the first
-    // set_cache(4)); what the last encode filled
+    // set_cache(4)); the form that holds valid conditions, 0 for none (since a change
+    // of form or an encode that failed)
     int cache_bits = 16, enc_bits = 16;
     std::vector<sfb_kv4_cache> kv4;
     // step workspaces
@@ -583,7 +584,9 @@ static int encode(Model& m, int B, const void* lang, const int32_t* lang_len, co
     SFB_TRY(linear(m.img2, m.enc_h, D, Mi, m.img_c, D, 0, nullptr, 0, s));
     SFB_TRY(launch_kernel(rdt::add_rows_kernel, grid_for(static_cast<int64_t>(Mi) * D / 8, 256), 256, 0, s, true,
         m.img_c, m.img_pos, B, c.img_len, D));
-    // per-block cross-attention K/V cache: kv = cond·Wkvᵀ + b, K k-normed in place
+    // per-block cross-attention K/V cache: kv = cond·Wkvᵀ + b, K k-normed in place;
+    // m.kv is written with either form, so neither is valid until the last block is done
+    m.enc_bits = 0;
     for (int l = 0; l < c.num_layers; ++l) {
         const bool lang_blk = (l % 2 == 0);
         const int rows = lang_blk ? Ml : Mi;
@@ -620,6 +623,14 @@ static int encode(Model& m, int B, const void* lang, const int32_t* lang_len, co
     return SFB_OK;
 }
 
+// Refuses a network evaluation on a cache that no encode has filled in its
+// present form.
+static int conditions_valid(const Model& m) {
+    if (m.enc_bits == m.cache_bits) return SFB_OK;
+    snprintf(last_error_buf(), 256, "no conditions are encoded in the %d-bit cache: encode again", m.cache_bits);
+    return SFB_ERR_INVALID;
+}
+
 // One denoising network evaluation (rdt1b.cpp:254-369, test_rdt1b_alignment.py:181-210)
 // on the current x_t (m.xact) at timestep t, leaving the x0 prediction in m.yfin.
 // step >= 0: sampling step `step` of the schedule (t == tsteps[step]), whose
@@ -629,10 +640,7 @@ static int forward(Model& m, int B, float t, cudaStream_t s, int step = -1) {
     const int D = c.hidden, S = m.S(), T = c.horizon, A = c.action_dim;
     const int M = B * S, Ma = B * (T + 1);
     const float eps = 1e-6f;
-    if (m.enc_bits != m.cache_bits) {
-        snprintf(last_error_buf(), 256, "the conditions were encoded into the %d-bit cache: encode again", m.enc_bits);
-        return SFB_ERR_INVALID;
-    }
+    SFB_TRY(conditions_valid(m));
     // state adaptor on [state, x_t] with an all-ones action mask
     prefer_max_shared(rdt::adaptor_input_kernel);
     prefer_max_shared(rdt::sincos_kernel);
@@ -834,6 +842,7 @@ int sfb_rdt1b_sample(void* handle, int32_t sessions, const float* noise, float* 
     if (m == nullptr || noise == nullptr || actions == nullptr) return SFB_ERR_INVALID;
     SFB_MODEL_ENTRY(m);
     if (sessions < 1 || sessions > m->c.max_sessions) return SFB_ERR_SHAPE;
+    SFB_TRY(rdt::conditions_valid(*m));            // (a replayed graph would not ask)
     cudaStream_t caller = static_cast<cudaStream_t>(stream);
     // all work runs on the model's stream, ordered after the caller's prior work
     cudaStream_t s = m->own;
@@ -933,6 +942,7 @@ int sfb_rdt1b_tick(void* handle, int32_t sessions, uint64_t frame_id, const void
             cudaMemcpyAsync(m->st_len, lang_len, len_b, cudaMemcpyDefault, m->enc) != cudaSuccess ||
             cudaMemcpyAsync(m->st_state, state, state_b, cudaMemcpyDefault, m->enc) != cudaSuccess)
             return fail_cuda("tick condition copy");
+        m->cond_valid = false;                     // until the encode has gone through
         SFB_TRY(rdt::encode(*m, sessions, m->st_lang, static_cast<const int32_t*>(m->st_len), m->st_img,
                             m->st_state, m->enc));
         if (cudaEventRecord(m->ev_enc, m->enc) != cudaSuccess || cudaStreamWaitEvent(caller, m->ev_enc, 0) != cudaSuccess)
@@ -1000,6 +1010,7 @@ int sfb_rdt1b_set_cache(void* handle, int32_t bits) {
     m->graphs.clear();
     m->graph_kernels.clear();
     m->cache_bits = bits;
+    m->enc_bits = 0;
     m->cond_valid = false;
     if (e != cudaSuccess) { record_cuda_error(e, "rdt1b set cache"); return SFB_ERR_CUDA; }
     return SFB_OK;

@@ -162,3 +162,24 @@ def test_tick_re_encodes_after_the_change(setup):
     _, e1 = m.tick_stats()
     torch.cuda.synchronize()
     assert e1 == e0 + 1 and torch.equal(out[1], out[2]) and not torch.equal(out[0], out[1])
+
+
+def test_a_change_and_back_without_an_encode_is_refused(setup):
+    """What the caches hold after a change of form is not vouched for until an encode."""
+    s, m = setup, setup["model"]
+    x = torch.empty_like(s["noise"])
+    for form, other in ((16, 4), (4, 16)):
+        m.set_cache(form)
+        encode(s)
+        m.sample(s["noise"], x)                        # (captures the graph)
+        m.set_cache(other)
+        m.set_cache(form)
+        with pytest.raises(_capi.SfbError):
+            m.forward(s["noise"], 1.0, x)
+        for graph in (True, False):
+            with pytest.raises(_capi.SfbError):
+                m.sample(s["noise"], x, use_graph=graph)
+        encode(s)
+        m.forward(s["noise"], 1.0, x)
+        m.set_cache(form)                              # no change: nothing to encode again
+        m.forward(s["noise"], 1.0, x)
