@@ -518,12 +518,15 @@ static int attention(const Model& m, const __nv_bfloat16* q, int64_t q_sb, int64
     return attention_tc_launch(a, s, o);
 }
 
-// The 4-bit form of every block's cross-attention cache (setup time).
+// The 4-bit form of every block's cross-attention cache (setup time): all blocks'
+// memory, or none and the model as it was.
 static int alloc_kv4(Model& m) {
     const auto& c = m.c;
     if (!m.kv4.empty()) return SFB_OK;
     std::vector<sfb_kv4_cache> made(c.num_layers);
-    for (int l = 0; l < c.num_layers; ++l) {
+    const size_t before = m.allocs.size();
+    m.allocs.reserve(before + 4 * static_cast<size_t>(c.num_layers));      // (nothing below throws)
+    auto block = [&](int l) {
         sfb_kv4_cache& k = made[l];
         const int64_t cap = ((l % 2 == 0 ? c.max_lang_len : c.img_len) + 31) / 32 * 32;
         const int64_t rows = static_cast<int64_t>(c.max_sessions) * c.heads * cap;
@@ -532,8 +535,16 @@ static int alloc_kv4(Model& m) {
         k.scale_stride[1] = cap * 2; k.scale_stride[0] = c.heads * k.scale_stride[1];
         SFB_TRY(dalloc(m, &k.k_codes, rows * 32)); SFB_TRY(dalloc(m, &k.v_codes, rows * 32));
         SFB_TRY(dalloc(m, &k.k_scale, rows * 4));  SFB_TRY(dalloc(m, &k.v_scale, rows * 4));
+        return static_cast<int>(SFB_OK);
+    };
+    for (int l = 0; l < c.num_layers; ++l) {
+        const int rc = block(l);
+        if (rc == SFB_OK) continue;
+        for (size_t i = before; i < m.allocs.size(); ++i) cudaFree(m.allocs[i]);
+        m.allocs.resize(before);
+        return rc;
     }
-    m.kv4 = made;
+    m.kv4.swap(made);
     return SFB_OK;
 }
 

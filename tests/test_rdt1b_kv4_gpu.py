@@ -183,3 +183,27 @@ def test_a_change_and_back_without_an_encode_is_refused(setup):
         m.forward(s["noise"], 1.0, x)
         m.set_cache(form)                              # no change: nothing to encode again
         m.forward(s["noise"], 1.0, x)
+
+
+def test_a_change_that_finds_no_memory_keeps_none(gpu):
+    """The 4-bit caches are allocated all or not at all, and the handle stays as it was."""
+    cfg = default_config(num_layers=2, max_lang_len=64, img_len=4374, max_sessions=4)
+    model, ballast = RDT1B(cfg, seed=5), None
+    try:
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        # of 40 MB for the image block (18 + 18 for its codes) 24 MB are there
+        ballast = torch.empty(torch.cuda.mem_get_info()[0] - (24 << 20), dtype=torch.uint8, device=gpu)
+        before = torch.cuda.mem_get_info()[0]
+        for _ in range(3):
+            with pytest.raises(_capi.SfbError):
+                model.set_cache(4)
+            assert torch.cuda.mem_get_info()[0] == before
+        ballast = None
+        torch.cuda.empty_cache()
+        model.set_cache(4)
+        assert model.kv4_cache(1).shape == (4, 32, 4384, 64)
+    finally:
+        del ballast
+        model.close()
+        torch.cuda.empty_cache()
