@@ -81,6 +81,7 @@ class RDT1B:
         self.lib = _capi.lib()
         _declare(self.lib)
         self.cfg = cfg
+        self.device = torch.cuda.current_device()      # the model's, as the library takes it
         h = ctypes.c_void_p()
         _capi.check(self.lib.sfb_rdt1b_create(ctypes.byref(cfg), seed, ctypes.byref(h)), "rdt1b create")
         self.h = h
@@ -148,16 +149,16 @@ class RDT1B:
         _capi.check(self.lib.sfb_rdt1b_set_cache(self.h, int(bits)), "set_cache")
 
     def kv4_cache(self, layer: int):
-        """A copy (quant4.KV4Cache) of a block's 4-bit cross-attention cache."""
+        """A copy (quant4.KV4Cache, on the model's device) of a block's 4-bit cross-attention cache."""
         from .quant4 import KV4Cache
         buf = ctypes.create_string_buffer(_capi.KV4_CACHE.size)
         _capi.check(self.lib.sfb_rdt1b_kv4_cache(self.h, int(layer), buf), "kv4_cache")
         kc, vc, ks, vs, _, _, _, _, B, H, C, D = _capi.KV4_CACHE.unpack(buf.raw)
-        torch.cuda.synchronize()
+        torch.cuda.synchronize(self.device)
         out = []
         for ptr, shape, dt in ((kc, (B, H, C, D // 2), torch.uint8), (vc, (B, H, C, D // 2), torch.uint8),
                                (ks, (B, H, C, D // 32), torch.float16), (vs, (B, H, C, D // 32), torch.float16)):
-            t = torch.empty(shape, dtype=dt, device="cuda")
+            t = torch.empty(shape, dtype=dt, device=f"cuda:{self.device}")
             _copy_d2d(t.data_ptr(), ptr, t.numel() * t.element_size())
             out.append(t)
         return KV4Cache(*out)

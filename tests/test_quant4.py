@@ -238,3 +238,25 @@ def test_linear_refusals():
     assert call(ldx=260) == E.SFB_ERR_ALIGN
     assert call(y=0x5001) == E.SFB_ERR_ALIGN
     assert call(M=0) == E.SFB_OK
+
+
+def test_copies_of_a_models_cache_are_on_its_device(monkeypatch):
+    """With another device current: the model's is waited for, and holds the copy (fakes
+    of the library and of torch's device calls)."""
+    from servoflow_b200 import rdt1b
+    shape, seen = (2, 3, 32, 64), []
+
+    class Lib:
+        def sfb_rdt1b_kv4_cache(self, h, layer, buf):
+            buf.raw = _capi.KV4_CACHE.pack(0x1000, 0x2000, 0x3000, 0x4000, 3072, 1024, 192, 64, *shape)
+            return 0
+
+    model = rdt1b.RDT1B.__new__(rdt1b.RDT1B)
+    model.lib, model.h, model.device = Lib(), None, 5
+    empty = torch.empty
+    monkeypatch.setattr(rdt1b.torch.cuda, "synchronize", lambda device=None: seen.append(("wait", device)))
+    monkeypatch.setattr(rdt1b.torch, "empty", lambda s, dtype, device: seen.append(("copy", device)) or empty(s, dtype=dtype))
+    monkeypatch.setattr(rdt1b, "_copy_d2d", lambda dst, src, n: None)
+    cache = model.kv4_cache(0)
+    assert cache.shape == shape
+    assert seen == [("wait", 5)] + 4 * [("copy", "cuda:5")]
