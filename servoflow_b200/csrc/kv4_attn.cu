@@ -51,6 +51,7 @@ struct Kv4AttnParams {
     int64_t q_st[3], o_st[3];
     int32_t H, g, Sq, Sk, R;          // g = H / Hkv query heads per K/V head, R = Sq · g rows
     int32_t rtiles, splits, causal;
+    int32_t rt0, ytiles;              // of a launch: first row tile, row tiles
     float sl2;                        // scale · log2(e)
     const int32_t* kv_len;
     const uint8_t* key_mask;
@@ -504,6 +505,32 @@ __global__ void __launch_bounds__(attn_threads(D), 2) kv4_attn_kernel(const Kv4A
     if (!ok) atomicExch(&g_sfb_device_error, SFB_ERR_DEVICE_TIMEOUT);
 }
 
+// Launches `kern` on a grid of (splits, K/V heads × row tiles, sessions). A grid's y
+// and z end at 65535: longer ones are cut into several launches, whose pointers and
+// first row tile are moved along.
+inline int launch_ranges(void (*kern)(Kv4AttnParams), cudaLaunchConfig_t& cfg, const Kv4AttnParams& all, const char* what) {
+    constexpr int kMax = 65535;
+    const int heads = std::max(1, kMax / all.rtiles), rows = std::min(kMax, all.rtiles);
+    for (int64_t b = 0; b < all.c.B; b += kMax)
+        for (int64_t h = 0; h < all.c.Hkv; h += heads)
+            for (int64_t t = 0; t < all.rtiles; t += rows) {
+                Kv4AttnParams p = all;
+                const int64_t code = b * p.c.code_sb + h * p.c.code_sh, scale = b * p.c.sc_sb + h * p.c.sc_sh;
+                p.c.kc += code; p.c.vc += code; p.c.ks += scale; p.c.vs += scale;
+                p.q = static_cast<const uint16_t*>(p.q) + b * p.q_st[0] + h * p.g * p.q_st[1];
+                p.out = static_cast<uint16_t*>(p.out) + b * p.o_st[0] + h * p.g * p.o_st[1];
+                if (p.kv_len != nullptr) p.kv_len += b;
+                if (p.key_mask != nullptr) p.key_mask += b * p.mask_sb;
+                p.rt0 = static_cast<int32_t>(t);
+                p.ytiles = static_cast<int32_t>(std::min<int64_t>(rows, p.rtiles - t));
+                cfg.gridDim = dim3(p.splits, static_cast<unsigned>(std::min<int64_t>(heads, p.c.Hkv - h) * p.ytiles),
+                                   static_cast<unsigned>(std::min<int64_t>(kMax, p.c.B - b)));
+                const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+                if (e != cudaSuccess) { record_cuda_error(e, what); return SFB_ERR_LAUNCH; }
+            }
+    return SFB_OK;
+}
+
 template <typename T, int D>
 int launch_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     const DeviceInfo& dev = device_info();
@@ -538,9 +565,7 @@ int launch_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
         if (fine > sp) sp = static_cast<int>(std::min<int64_t>(fine, 8));
     }
     p.splits = std::min(sp, std::max(1, blocks));
-    if (p.c.Hkv > 65535 || p.c.B > 65535) return SFB_ERR_SHAPE;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.splits, p.c.Hkv, p.c.B);
     cfg.blockDim = dim3(attn_threads(D), 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -551,9 +576,8 @@ int launch_attn(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1 + pdl_attr(&attr[1], true);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-    if (e != cudaSuccess) { record_cuda_error(e, "kv4 attention launch"); return SFB_ERR_LAUNCH; }
-    return SFB_OK;
+    p.rtiles = 1;
+    return launch_ranges(kern, cfg, p, "kv4 attention launch");
 }
 
 template <typename T>

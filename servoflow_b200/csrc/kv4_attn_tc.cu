@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(threads(D, NQ), 1) kv4_attn_tc_kernel(const Kv
     float* wred = alpha + 2 * kMaxQ;                               // [4 windows][kMaxQ]
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int split = blockIdx.x, hk = blockIdx.y / p.rtiles, rt = blockIdx.y - hk * p.rtiles, b = blockIdx.z;
+    const int split = blockIdx.x, hk = blockIdx.y / p.ytiles, rt = p.rt0 + blockIdx.y - hk * p.ytiles, b = blockIdx.z;
     // rows in equal tiles of at most NQ
     const int r0 = static_cast<int>(static_cast<int64_t>(p.R) * rt / p.rtiles);
     const int rows = static_cast<int>(static_cast<int64_t>(p.R) * (rt + 1) / p.rtiles) - r0;
@@ -582,9 +582,7 @@ int launch(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
         sp = std::min(sp, std::max(1, tiles / 2));
     }
     p.splits = std::min(sp, std::max(1, tiles));
-    if (static_cast<int64_t>(p.c.Hkv) * p.rtiles > 65535 || p.c.B > 65535) return SFB_ERR_SHAPE;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.splits, p.c.Hkv * p.rtiles, p.c.B);
     cfg.blockDim = dim3(threads(D, NQ), 1, 1);
     cfg.dynamicSmemBytes = smem_bytes(D);
     cfg.stream = s;
@@ -595,9 +593,7 @@ int launch(Kv4AttnParams& p, int num_splits, cudaStream_t s) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1 + pdl_attr(&attr[1], true);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-    if (e != cudaSuccess) { record_cuda_error(e, "kv4 attention (tcgen05) launch"); return SFB_ERR_LAUNCH; }
-    return SFB_OK;
+    return kv4::launch_ranges(kern, cfg, p, "kv4 attention (tcgen05) launch");
 }
 
 // The column count that takes the least time: rounds of the SMs (or the share of a

@@ -435,3 +435,40 @@ def test_few_key_tiles_a_cta(be, gpu, D, Sk, Sq):
     for _ in range(20):
         be.kv4_attention(q, cache, again.fill_(0), seq_k=Sk, num_splits=1)
         assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("B,Hkv,Sq", [(65600, 1, 1), (65600, 1, 17), (1, 65600, 1), (1, 33000, 97)])
+def test_more_heads_sessions_and_row_tiles_than_65535(be, gpu, B, Hkv, Sq):
+    D, n = 64, 20
+    cache = KV4Cache.allocate(B, Hkv, n, D, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(Sq)
+    for codes, scale in ((cache.k_codes, cache.k_scale), (cache.v_codes, cache.v_scale)):
+        codes.copy_(torch.randint(0, 256, codes.shape, generator=g, device=gpu, dtype=torch.uint8))
+        scale.copy_((torch.rand(scale.shape, generator=g, device=gpu) * 0.2).bfloat16().half())
+    q = torch.randn(B, Hkv, Sq, D, generator=g, device=gpu, dtype=torch.float32).half()
+    out = torch.full_like(q, float("nan"))
+    be.kv4_attention(q, cache, out, seq_k=n)
+    # heads and sessions from all over the grid, the last among them
+    b = torch.tensor([0, B // 2, B - 1], device=gpu)
+    h = torch.tensor([0, 1, Hkv // 2, Hkv - 2, Hkv - 1], device=gpu).clamp(0, Hkv - 1)
+    pick = lambda t: t[b][:, h]
+    part = KV4Cache(*(pick(t).contiguous() for t in (cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale)))
+    ref, mag, vmax = attn64(pick(q), part, None, n, False, None, 1 / math.sqrt(D))
+    tol = 2.0 ** -11 * ref.abs() + (2.0 ** -11 + 2.0 ** -15) * mag + n * 2.0 ** -25 * vmax
+    assert ((pick(out).double() - ref).abs() <= tol).all()
+    assert not out.isnan().any()
+
+
+def test_more_row_tiles_of_one_head_than_65535(be, gpu):
+    # 400 thousand tokens of 16 heads that share one: 66667 tiles of 96 rows
+    D, n, H, Sq = 64, 20, 16, 400_000
+    cache = KV4Cache.allocate(1, 1, n, D, device=gpu)
+    fill(cache, 61)
+    q = torch.randn(1, H, Sq, D, generator=torch.Generator(device=gpu).manual_seed(3), device=gpu).half()
+    out = torch.full_like(q, float("nan"))
+    be.kv4_attention(q, cache, out, seq_k=n)
+    assert not out.isnan().any()
+    i = torch.tensor([0, 1, Sq // 3, Sq - 7000, Sq - 6500, Sq - 6000, Sq - 1], device=gpu)
+    ref, mag, vmax = attn64(q[:, :, i], cache, None, n, False, None, 1 / math.sqrt(D))
+    tol = 2.0 ** -11 * ref.abs() + (2.0 ** -11 + 2.0 ** -15) * mag + n * 2.0 ** -25 * vmax
+    assert ((out[:, :, i].double() - ref).abs() <= tol).all()
