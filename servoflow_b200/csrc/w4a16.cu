@@ -436,8 +436,7 @@ __global__ void __launch_bounds__(many_threads(WM)) w4a16_many_kernel(const W4Pa
 
 template <auto Kern>
 int launch(int smem, int threads, int channels, int rows, const W4Params& p, int act, cudaStream_t s) {
-    const int64_t bx = (static_cast<int64_t>(p.N) + channels - 1) / channels, by = (static_cast<int64_t>(p.M) + rows - 1) / rows;
-    if (by > 65535) return SFB_ERR_SHAPE;
+    const int64_t bx = (static_cast<int64_t>(p.N) + channels - 1) / channels;
     static std::atomic<bool> done[64];             // kernel attributes, once per device (idempotent)
     std::atomic<bool>& set = done[device_info().ordinal & 63];
     if (!set.load(std::memory_order_acquire)) {
@@ -446,7 +445,18 @@ int launch(int smem, int threads, int channels, int rows, const W4Params& p, int
         prefer_max_shared(Kern);
         set.store(true, std::memory_order_release);
     }
-    return launch_kernel(Kern, dim3(static_cast<unsigned>(bx), static_cast<unsigned>(by)), threads, smem, s, true, p, act);
+    // a grid's y ends at 65535 row tiles: more rows are several launches
+    const int64_t most = 65535ll * rows, ysz = p.y_f32 ? 4 : 2;
+    for (int64_t m = 0; m < p.M; m += most) {
+        W4Params q = p;
+        q.M = static_cast<int32_t>(std::min<int64_t>(most, p.M - m));
+        q.x = static_cast<const uint16_t*>(p.x) + m * p.ldx;
+        q.y = static_cast<uint8_t*>(p.y) + m * p.ldy * ysz;
+        if (p.residual != nullptr) q.residual = static_cast<const uint8_t*>(p.residual) + m * p.ldr * ysz;
+        SFB_TRY(launch_kernel(Kern, dim3(static_cast<unsigned>(bx), static_cast<unsigned>((q.M + rows - 1) / rows)), threads,
+                              smem, s, true, q, act));
+    }
+    return SFB_OK;
 }
 
 template <typename T, int G, int NT, int MT>

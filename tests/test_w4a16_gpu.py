@@ -151,3 +151,19 @@ def test_wrapper_refusals(be, gpu):
         be.w4a16_linear(x, wq, s, y, act="relu")
     with pytest.raises(ValueError):
         be.w4a16_linear(x, wq.cpu(), s, y)
+
+
+def test_more_row_tiles_than_65535(be, gpu):
+    """Any M: 4.8 million rows are 66 thousand tiles of 72."""
+    M, N, K, G = 4_800_001, 8, 32, 32
+    g = torch.Generator().manual_seed(1)
+    codes = torch.randint(-8, 8, (N, K), generator=g, dtype=torch.int32)
+    s = (torch.rand(N, 1, generator=g) * 0.02).half()
+    x = torch.randn(M, K, generator=torch.Generator(device=gpu).manual_seed(2), device=gpu).bfloat16()
+    r = torch.randn(M, N, generator=torch.Generator(device=gpu).manual_seed(3), device=gpu)
+    out = torch.full((M, N), float("nan"), dtype=torch.float32, device=gpu)
+    be.w4a16_linear(x, pack_codes(codes).to(gpu), s.to(gpu), out, residual=r)
+    w = (codes.double() * s.double()).to(gpu)
+    y = x.double() @ w.t() + r.double()
+    tol = (1.2 * 2.0 ** -17 + 2.0 ** -24) * (x.double().abs() @ w.abs().t()) + (2.0 ** -20 + 2.0 ** -24) * y.abs()
+    assert ((out.double() - y).abs() <= tol).all()
