@@ -380,8 +380,8 @@ int sfb_kv4_attention(const sfb_kv4_cache* cache, const sfb_kv4_attn_args* args,
  * contiguous in scale_dtype (SFB_F16, SFB_BF16 or SFB_F32); group: 32, 64 or
  * 128; K % group == 0. bias: x_dtype [N] or NULL; residual: [M, N] in y_dtype
  * with row stride ldr, or NULL (may alias y); y: y_dtype (x_dtype or SFB_F32)
- * [M, N], row stride ldy. act as sfb_w8a16_linear. Any M and N. Codes enter the
- * products exactly; sums and scales are fp32. Meant for few rows (it is bound
+ * [M, N], row stride ldy. act as sfb_w8a16_linear. Any M, N and K (N and K up
+ * to 2^31 - 1024). Codes enter the products exactly; sums and scales are fp32. Meant for few rows (it is bound
  * by the weights up to about 64). */
 int sfb_w4a16_linear(const void* x, int64_t ldx, int32_t x_dtype, const void* w, const void* w_scale,
                      int32_t scale_dtype, int32_t group, const void* bias, const void* residual, int64_t ldr,

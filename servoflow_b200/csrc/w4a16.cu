@@ -503,7 +503,8 @@ int w4a16_linear_launch(const void* x, int64_t ldx, int32_t x_dtype, const void*
                         int32_t scale_dtype, int32_t group, const void* bias, const void* residual, int64_t ldr,
                         void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t N, int32_t K, int32_t act,
                         cudaStream_t stream) {
-    if (M < 0 || N <= 0 || K <= 0) return SFB_ERR_SHAPE;
+    // (the kernels' 32-bit indexes go up to a tile of channels or 512 inputs past the last)
+    if (M < 0 || N <= 0 || K <= 0 || N > 0x7ffffc00 || K > 0x7ffffc00) return SFB_ERR_SHAPE;
     if (group != 32 && group != 64 && group != 128) return SFB_ERR_SHAPE;
     if (K % group != 0) return SFB_ERR_SHAPE;
     if (x_dtype != SFB_BF16 && x_dtype != SFB_F16) return SFB_ERR_DTYPE;

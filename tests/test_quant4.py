@@ -260,3 +260,17 @@ def test_copies_of_a_models_cache_are_on_its_device(monkeypatch):
     cache = model.kv4_cache(0)
     assert cache.shape == shape
     assert seen == [("wait", 5)] + 4 * [("copy", "cuda:5")]
+
+
+def test_linear_sizes_next_to_2_31_are_refused():
+    """The kernels index channels and inputs in 32 bits, up to a tile past the last one."""
+    lib, E = _capi.lib(), _capi
+
+    def call(N, K, G):
+        return lib.sfb_w4a16_linear(0x1000, 2 ** 31, E.SFB_BF16, 0x2000, 0x3000, E.SFB_F16, G, None, None, 0, 0x5000,
+                                    2 ** 31, E.SFB_BF16, 1, N, K, 0, None)
+
+    for n in (2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 64, 2 ** 31 - 1023):
+        assert call(n, 64, 64) == E.SFB_ERR_SHAPE
+    for k in (2 ** 31 - 128, 2 ** 31 - 512, 2 ** 31 - 896):
+        assert call(16, k, 128) == E.SFB_ERR_SHAPE
