@@ -300,7 +300,7 @@ int sfb_qk_norm_rope(const sfb_norm_rope_args* args, void* stream);
  * Layout: codes [batch, heads_kv, capacity, head_dim/2] bytes and scales
  * [batch, heads_kv, capacity, head_dim/32] fp16, the last two dimensions
  * contiguous; K and V share the strides. head_dim 64 or 128; capacity a multiple
- * of 4. Code pointers and strides are multiples of 16 bytes, scale pointers and
+ * of 4, at most 2^31 - 512. Code pointers and strides are multiples of 16 bytes, scale pointers and
  * strides too. */
 typedef struct sfb_kv4_cache {
     void* k_codes;

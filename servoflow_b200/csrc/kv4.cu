@@ -232,7 +232,8 @@ int kv4_cache_check(const sfb_kv4_cache* c, Kv4Params& p) {
     if (!empty && (c->k_codes == nullptr || c->v_codes == nullptr || c->k_scale == nullptr || c->v_scale == nullptr))
         return SFB_ERR_INVALID;
     if (c->head_dim != 64 && c->head_dim != 128) return SFB_ERR_SHAPE;
-    if (c->batch < 0 || c->heads_kv < 1 || c->capacity < 0 || c->capacity > 0x7fffff00 || c->capacity % 4 != 0) return SFB_ERR_SHAPE;
+    // (slots are counted in 32 bits, up to two blocks of 128 past the last one)
+    if (c->batch < 0 || c->heads_kv < 1 || c->capacity < 0 || c->capacity > 0x7ffffe00 || c->capacity % 4 != 0) return SFB_ERR_SHAPE;
     auto al = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
     if (!al(c->k_codes) || !al(c->v_codes) || !al(c->k_scale) || !al(c->v_scale)) return SFB_ERR_ALIGN;
     if (c->code_stride[0] % 16 || c->code_stride[1] % 16 || c->scale_stride[0] % 8 || c->scale_stride[1] % 8)

@@ -274,3 +274,13 @@ def test_linear_sizes_next_to_2_31_are_refused():
         assert call(n, 64, 64) == E.SFB_ERR_SHAPE
     for k in (2 ** 31 - 128, 2 ** 31 - 512, 2 ** 31 - 896):
         assert call(16, k, 128) == E.SFB_ERR_SHAPE
+
+
+@pytest.mark.parametrize("capacity", [2 ** 31 - 256, 2 ** 31 - 508])
+def test_capacities_next_to_2_31_are_refused(capacity):
+    """The attention looks two blocks of 128 slots ahead, counted in 32 bits."""
+    lib, E = _capi.lib(), _capi
+    c, st = _cache(capacity=capacity), I3(8192, 64, 256)
+    assert lib.sfb_kv4_attention(c, _attn(seq_k=capacity), None) == E.SFB_ERR_SHAPE
+    assert lib.sfb_kv4_append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 1, None, capacity - 1, None, None) == E.SFB_ERR_SHAPE
+    assert lib.sfb_kv4_read(c, 0x2000, st, 0x2000, st, E.SFB_F16, capacity - 1, 1, None) == E.SFB_ERR_SHAPE
