@@ -144,6 +144,14 @@ def _order(layout: str):
         raise ValueError(f"unknown layout {layout!r}") from None
 
 
+def _i32(name: str, v) -> int:
+    """v as an argument of 32 bits: ctypes would cut a longer one short without a word."""
+    v = int(v)
+    if not -0x80000000 <= v <= 0x7fffffff:
+        raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"{name} {v} does not fit 32 bits")
+    return v
+
+
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
@@ -334,7 +342,8 @@ class B200Backend:
             if t is not None and (t.dtype is not torch.int32 or t.shape != (B,) or not t.is_contiguous()):
                 raise _capi.SfbError(_capi.SFB_ERR_SHAPE, f"{n} must be contiguous int32 [B]")
         _call(self._lib.sfb_kv4_append, "kv4_append", dev, stream, c, K.data_ptr(), ks, V.data_ptr(), vs,
-              _DTYPE_CODE[K.dtype], K.shape[o[2]], _ptr(start_t), 0 if start_t is not None else int(start), _ptr(lens))
+              _DTYPE_CODE[K.dtype], _i32("seq", K.shape[o[2]]), _ptr(start_t),
+              0 if start_t is not None else _i32("start", start), _ptr(lens))
 
     def kv4_read(self, cache, K=None, V=None, slot0: int = 0, layout: str = "bhsd", stream=None) -> None:
         """Writes the values of slots [slot0, slot0 + S) into K and V ([B, Hkv,
@@ -352,7 +361,7 @@ class B200Backend:
         ks = None if K is None else self._kv4_side(K, "K", o, B, Hkv, D)
         vs = None if V is None else self._kv4_side(V, "V", o, B, Hkv, D)
         _call(self._lib.sfb_kv4_read, "kv4_read", dev, stream, c, _ptr(K), ks, _ptr(V), vs, _DTYPE_CODE[x.dtype],
-              int(slot0), x.shape[o[2]])
+              _i32("slot0", slot0), _i32("seq", x.shape[o[2]]))
 
     def kv4_attention(self, Q, cache, out, seq_k: Optional[int] = None, kv_len=None, mask=None,
                       scale: float = 0.0, is_causal: bool = False, num_splits: int = 0,
@@ -372,7 +381,7 @@ class B200Backend:
             raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "Q and out must be 4-D and fit the cache")
         if st[3] != 1 or so[3] != 1:
             raise _capi.SfbError(_capi.SFB_ERR_SHAPE, "head_dim must be contiguous")
-        sk = cap if seq_k is None else int(seq_k)
+        sk = cap if seq_k is None else _i32("seq_k", seq_k)
         lens = keep = keep_sb = 0
         if kv_len is not None:
             if kv_len.dtype is not torch.int32 or kv_len.shape != (B,) or not kv_len.is_contiguous():
@@ -426,7 +435,8 @@ class B200Backend:
                 ldr = residual.stride(0)
         _call(self._lib.sfb_w4a16_linear, "w4a16_linear", dev, stream, x.data_ptr(), ldx, _DTYPE_CODE[x.dtype],
               w_q.data_ptr(), w_scale.data_ptr(), _DTYPE_CODE[w_scale.dtype], K // groups, _ptr(bias),
-              _ptr(residual), ldr, out.data_ptr(), ldy, _DTYPE_CODE[out.dtype], M, N, K, _ACTS[act])
+              _ptr(residual), ldr, out.data_ptr(), ldy, _DTYPE_CODE[out.dtype], _i32("M", M), _i32("N", N), _i32("K", K),
+              _ACTS[act])
 
     # Graph hooks (backend.h:227-229; CUDABackend keeps one graph per stream,
     # cuda_backend.cu:592-608).

@@ -472,3 +472,26 @@ def test_more_row_tiles_of_one_head_than_65535(be, gpu):
     ref, mag, vmax = attn64(q[:, :, i], cache, None, n, False, None, 1 / math.sqrt(D))
     tol = 2.0 ** -11 * ref.abs() + (2.0 ** -11 + 2.0 ** -15) * mag + n * 2.0 ** -25 * vmax
     assert ((out[:, :, i].double() - ref).abs() <= tol).all()
+
+
+def test_slots_past_32_bits_are_refused(be, gpu):
+    """Slots and lengths that the C call's 32-bit arguments would cut short."""
+    cache = KV4Cache.allocate(1, 1, 32, 64)
+    fill(cache, 3)
+    before = [t.clone() for t in (cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale)]
+    x = torch.ones(1, 1, 1, 64, dtype=torch.float16, device=gpu)
+    for start in (2 ** 32, 2 ** 32 + 5, -2 ** 32, 2 ** 31):
+        with pytest.raises(_capi.SfbError):
+            be.kv4_append(cache, x, x, start=start)
+        with pytest.raises(_capi.SfbError):
+            be.kv4_read(cache, x, slot0=start)
+    long = x.expand(1, 1, 2 ** 32 + 1, 64)             # not one token
+    with pytest.raises(_capi.SfbError):
+        be.kv4_append(cache, long, long)
+    with pytest.raises(_capi.SfbError):
+        be.kv4_read(cache, long)
+    for sk in (2 ** 32 + 32, 2 ** 31, -1):
+        with pytest.raises(_capi.SfbError):
+            be.kv4_attention(x, cache, x, seq_k=sk)
+    for got, want in zip((cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale), before):
+        assert torch.equal(got, want)

@@ -284,3 +284,11 @@ def test_capacities_next_to_2_31_are_refused(capacity):
     assert lib.sfb_kv4_attention(c, _attn(seq_k=capacity), None) == E.SFB_ERR_SHAPE
     assert lib.sfb_kv4_append(c, 0x2000, st, 0x2000, st, E.SFB_BF16, 1, None, capacity - 1, None, None) == E.SFB_ERR_SHAPE
     assert lib.sfb_kv4_read(c, 0x2000, st, 0x2000, st, E.SFB_F16, capacity - 1, 1, None) == E.SFB_ERR_SHAPE
+
+
+def test_arguments_past_32_bits_are_refused():
+    from servoflow_b200.backend import _i32
+    assert _i32("N", 2 ** 31 - 1) == 2 ** 31 - 1 and _i32("start", -2 ** 31) == -2 ** 31
+    for v in (2 ** 31, 2 ** 32 + 16, -2 ** 31 - 1):        # 2^32 + 16 was taken for 16
+        with pytest.raises(SfbError):
+            _i32("N", v)
