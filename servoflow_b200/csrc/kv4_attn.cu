@@ -31,9 +31,14 @@
 // (0x6400 | n = 1024 + n), the scale is one exact fp16 product (kv4.cu).
 // Pᵀ moves from the accumulator's layout to the B operand's by two movmatrix.
 //
-// Softmax in base 2: the running reference of a row is raised only when a
-// logit passes it by more than 8, so that P <= 256 fits fp16 and the rescaling
-// of Oᵀ is rare; row sums are fp32 from the unrounded probabilities.
+// Softmax in base 2, P = exp2(x − m) against a row's running reference m, rounded to
+// fp16 for the tensor cores (half a step is 2^-11 of it: lost beside a bf16 result's
+// rounding, not beside an fp16 one's). m is put 7 below the largest logit and raised
+// only when one passes it by more than 15: rescaling Oᵀ is rare, P <= 2^15 fits, and a
+// probability keeps all of its bits down to 2^-21 of the row's largest, some down to
+// 2^-31. (With m at the largest that ended at 2^-14 and 2^-24, and a row whose largest
+// probability had a V near 0 lost the result of the others.) Row sums are fp32 from the
+// unrounded probabilities.
 //
 // Work split: a CTA takes a range of 16-key tiles of one (session, K/V head,
 // row tile), its warps interleaved; partial (m, l, O) are joined in shared
@@ -91,6 +96,8 @@ __device__ __forceinline__ void contain(__half2& ks, __half2& vs) {
 }
 
 constexpr float kUnseen = 1e30f;
+// A row's reference is put kBelow under its largest logit, and raised when one passes it by more than kOver.
+constexpr float kBelow = 7.f, kOver = 15.f;
 constexpr int kRows = 8;                                         // rows of a CTA
 constexpr int kWarps = 8;                                        // computing
 __host__ __device__ constexpr bool uses_ring(int D) { return D == 128; }
@@ -232,7 +239,7 @@ __global__ void __launch_bounds__(attn_threads(D), 2) kv4_attn_kernel(const Kv4A
             // the reference −kUnseen, so that its first key passes it
             float x[4] = {fmaf(c[0], p.sl2, nm[0]), fmaf(c[1], p.sl2, nm[1]), fmaf(c[2], p.sl2, nm[0]),
                           fmaf(c[3], p.sl2, nm[1])};
-            if (__any_sync(0xffffffffu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > 8.f)) {
+            if (__any_sync(0xffffffffu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > kOver)) {
                 float ma = fmaxf(c[0] * p.sl2, c[2] * p.sl2), mb = fmaxf(c[1] * p.sl2, c[3] * p.sl2);
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) {
@@ -240,8 +247,8 @@ __global__ void __launch_bounds__(attn_threads(D), 2) kv4_attn_kernel(const Kv4A
                     mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, off));
                 }
                 float aa = 1.f, ab = 1.f;
-                if (ma + nm[0] > 8.f) { aa = nm[0] == kUnseen ? 0.f : ptx::ex2(-nm[0] - ma); nm[0] = -ma; }
-                if (mb + nm[1] > 8.f) { ab = nm[1] == kUnseen ? 0.f : ptx::ex2(-nm[1] - mb); nm[1] = -mb; }
+                if (ma + nm[0] > kOver) { aa = nm[0] == kUnseen ? 0.f : ptx::ex2(kBelow - ma - nm[0]); nm[0] = kBelow - ma; }
+                if (mb + nm[1] > kOver) { ab = nm[1] == kUnseen ? 0.f : ptx::ex2(kBelow - mb - nm[1]); nm[1] = kBelow - mb; }
                 l[0] *= aa; l[1] *= ab;
 #pragma unroll
                 for (int i = 0; i < kMT; ++i) {

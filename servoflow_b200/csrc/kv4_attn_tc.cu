@@ -21,9 +21,9 @@
 // owners), four that dequantise for every 64 channels, one that issues the MMAs. Sᵀ and Pᵀ are double-
 // buffered; Sᵀ of tile j + 2 is issued behind P·V of tile j, so that one barrier
 // tells a group both that its logits are there and that its P buffer is free.
-// The reference of a row (the m of exp2(x − m)) is shared by a group's 128
-// threads through shared memory and raised only when a logit passes it by more
-// than 8: a comparison a value with one vote of the group finds that out.
+// The reference of a row (the m of exp2(x − m), kv4_attn.cu) is shared by a group's
+// 128 threads through shared memory and raised only when a logit passes it by more
+// than 15: a comparison a value with one vote of the group finds that out.
 // (The vote of a tile cast one tile ahead, so that no warp waits for the others',
 // takes the logits out of TMEM twice, or twice the registers: 32 sessions of 67
 // rows by 4374 slots of 32 heads took 324 and 365 µs.)
@@ -398,12 +398,12 @@ __global__ void __launch_bounds__(threads(D, NQ), 1) kv4_attn_tc_kernel(const Kv
             };
             if (edge) hide();
             to_exponents();
-            // does any logit pass its row's reference by more than 8? (a row that saw
+            // does any logit pass its row's reference by more than kOver? (a row that saw
             // no key yet has the reference −kUnseen)
             float over[2] = {x[0], x[1]};
 #pragma unroll
             for (int i = 2; i < kC; i += 2) over[(i / 2) & 1] = fmaxf(fmaxf(over[(i / 2) & 1], x[i]), x[i + 1]);
-            if (bar_or(1 + grp, fmaxf(over[0], over[1]) > 8.f)) {
+            if (bar_or(1 + grp, fmaxf(over[0], over[1]) > kv4::kOver)) {
                 // raise the references: column maxima of the tile, over a warp's keys, then its group's warps
                 tmem_ld16(tS + 96 * u, x);
                 tmem_ld_wait();
@@ -418,10 +418,11 @@ __global__ void __launch_bounds__(threads(D, NQ), 1) kv4_attn_tc_kernel(const Kv
                     const float t = fmaxf(fmaxf(cm[0], cm[kMaxQ]), fmaxf(cm[2 * kMaxQ], cm[3 * kMaxQ])) * sl2;
                     const float old = colm[c0 + row];
                     float al = 1.f;
-                    if (t > old + 8.f) {
-                        al = old == -INFINITY ? 0.f : ex2(old - t);
-                        colm[c0 + row] = t;
-                        negm[c0 + row] = -t;
+                    if (t > old + kv4::kOver) {
+                        const float m = t - kv4::kBelow;
+                        al = old == -INFINITY ? 0.f : ex2(old - m);
+                        colm[c0 + row] = m;
+                        negm[c0 + row] = -m;
                     }
                     alpha[c0 + row] = al;
                 }

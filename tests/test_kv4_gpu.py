@@ -495,3 +495,37 @@ def test_slots_past_32_bits_are_refused(be, gpu):
             be.kv4_attention(x, cache, x, seq_k=sk)
     for got, want in zip((cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale), before):
         assert torch.equal(got, want)
+
+
+def constant_cache(B, Hkv, cap, D, gpu, k_code, v_code):
+    """A cache of scale-1 groups: integer codes [cap, D] of K and V in every head and session."""
+    from servoflow_b200.quant4 import pack_codes
+    cache = KV4Cache.allocate(B, Hkv, cap, D, device=gpu)
+    for codes, scale, c in ((cache.k_codes, cache.k_scale, k_code), (cache.v_codes, cache.v_scale, v_code)):
+        codes.copy_(pack_codes(c.to(torch.int32).to(gpu)).expand_as(codes))
+        scale.fill_(1.0)
+    return cache
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq", [1, 12, 40])
+@pytest.mark.parametrize("gap", [14.0, 17.5])
+@pytest.mark.parametrize("splits", [1, 0])
+def test_small_probabilities_beside_a_dominant_slot(be, gpu, D, Sq, gap, splits):
+    """One slot takes nearly all of a row and has V = 0, 16383 others share what is left
+    (each e^-gap of it, 2^-20 and 2^-25) and carry the whole result. P is rounded to fp16
+    after a factor of at least 2^7, so one is off by 2^-12 of itself (half a step) or by
+    2^-25 · 2^-7 where that is fp16's subnormal range."""
+    n = 16384
+    k, v = torch.zeros(n, D), torch.ones(n, D)
+    k[0, 0], v[0] = 7, 0
+    v[1::3] = 3
+    cache = constant_cache(1, 2, n, D, gpu, k, v)
+    q = torch.zeros(1, 2, Sq, D, dtype=torch.float16, device=gpu)
+    q[..., 0] = gap / 7
+    out = torch.empty_like(q)
+    be.kv4_attention(q, cache, out, scale=1.0, num_splits=splits)
+    ref, mag, vmax = attn64(q, cache, None, n, False, None, 1.0)
+    tol = 2.0 ** -11 * ref.abs() + (2.0 ** -11 + 2.0 ** -15) * mag + n * 2.0 ** -32 * vmax + 2.0 ** -25
+    err = (out.double() - ref).abs()
+    assert (err <= tol).all(), f"max err {err.max().item():.3e}, tol {tol.max().item():.3e}, ref {ref.abs().max().item():.3e}"
