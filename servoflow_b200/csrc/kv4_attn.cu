@@ -95,6 +95,13 @@ __device__ __forceinline__ void contain(__half2& ks, __half2& vs) {
     if (not_finite(v) || not_finite(v >> 16)) { ks = u2h(0x7fff7fffu); vs = u2h(0u); }
 }
 
+// A query's infinity as NaN: it makes every logit of its row an infinity or NaN, and
+// so the row NaN, but logits that are minus infinity throughout would pass for masked.
+__device__ __forceinline__ uint32_t inf_to_nan(uint32_t q2) {
+    const __half2 q = u2h(q2);
+    return h2u(__hadd2(q, __hsub2(q, q)));
+}
+
 constexpr float kUnseen = 1e30f;
 // A row's reference is put kBelow under its largest logit, and raised when one passes it by more than kOver.
 constexpr float kBelow = 7.f, kOver = 15.f;
@@ -170,14 +177,15 @@ __global__ void __launch_bounds__(attn_threads(D), 2) kv4_attn_kernel(const Kv4A
             const int rr = r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
             const T* src = static_cast<const T*>(p.q) + b * p.q_st[0] + h * p.q_st[1] + qi * p.q_st[2] + d;
             u = *reinterpret_cast<const uint4*>(src);
-            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+            uint32_t* w = reinterpret_cast<uint32_t*>(&u);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
                     const float lo = __uint_as_float(w[e] << 16), hi = __uint_as_float(w[e] & 0xffff0000u);
                     bad |= (fabsf(lo) > 65504.f && !isinf(lo)) | (fabsf(hi) > 65504.f && !isinf(hi));
                     w[e] = h2u(__floats2half2_rn(lo, hi));
                 }
+                w[e] = inf_to_nan(w[e]);
             }
         }
         *reinterpret_cast<uint4*>(sQ + r * kPad + d) = u;

@@ -202,6 +202,7 @@ __global__ void __launch_bounds__(threads(D, NQ), 1) kv4_attn_tc_kernel(const Kv
                     bad |= (fabsf(lo) > 65504.f && !isinf(lo)) | (fabsf(hi) > 65504.f && !isinf(hi));
                     w[e] = kv4::h2u(__floats2half2_rn(lo, hi));
                 }
+                w[e] = kv4::inf_to_nan(w[e]);
                 if (p.sl2 < 0.f) w[e] ^= 0x80008000u;      // the kernel's scale is |scale|
             }
         }

@@ -529,3 +529,23 @@ def test_small_probabilities_beside_a_dominant_slot(be, gpu, D, Sq, gap, splits)
     tol = 2.0 ** -11 * ref.abs() + (2.0 ** -11 + 2.0 ** -15) * mag + n * 2.0 ** -32 * vmax + 2.0 ** -25
     err = (out.double() - ref).abs()
     assert (err <= tol).all(), f"max err {err.max().item():.3e}, tol {tol.max().item():.3e}, ref {ref.abs().max().item():.3e}"
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq", [2, 20])
+@pytest.mark.parametrize("inf", [float("inf"), -float("inf")])
+def test_infinite_queries_make_their_rows_nan(be, gpu, dt, D, Sq, inf):
+    """Every logit of such a row is an infinity or NaN, so its softmax is NaN; also where
+    each is minus infinity. A row that sees no slot stays zero."""
+    n = 40
+    cache = constant_cache(2, 1, 64, D, gpu, torch.full((64, D), 3.0), torch.ones(64, D))
+    q = torch.ones(2, 1, Sq, D, dtype=dt, device=gpu)
+    q[:, :, 1, 5] = inf
+    out = torch.empty_like(q)
+    be.device_error(reset=True)
+    be.kv4_attention(q, cache, out, seq_k=n, kv_len=torch.tensor([n, 0], dtype=torch.int32, device=gpu))
+    assert out[0, 0, 1].isnan().all() and (out[1] == 0).all()
+    out[0, 0, 1] = 1
+    assert (out[0] == 1).all()
+    assert be.device_error() == 0
