@@ -549,3 +549,14 @@ def test_infinite_queries_make_their_rows_nan(be, gpu, dt, D, Sq, inf):
     out[0, 0, 1] = 1
     assert (out[0] == 1).all()
     assert be.device_error() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,Hkv,Sq", [(25, 25, 75), (25, 25, 80), (25, 25, 81), (25, 25, 96), (100, 25, 24)])
+def test_every_row_form_with_masks(be, gpu, D, dt, H, Hkv, Sq):
+    """Calls of 100 units, which take 80 columns up to 80 rows and, with 64 channels, 96
+    above (128 channels: twice 48); lengths, causal order and dropped keys in each."""
+    run_attn(be, gpu, 4, H, Hkv, Sq, 261, D, dt, causal=True, lens=[261, 100, Sq + 3, 7], seed=Sq)
+    run_attn(be, gpu, 4, H, Hkv, Sq, 261, D, dt, mask_p=0.4, lens=[261, 0, 128, 129], layout="bshd", seed=Sq + 1)
+    run_attn(be, gpu, 4, H, Hkv, Sq, 530, D, dt, scale=-0.2, splits=3, seed=Sq + 2)

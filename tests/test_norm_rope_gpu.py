@@ -198,3 +198,16 @@ def test_channels_past_the_rotated_ones_pass_through(be, gpu, dt, D, rot, inter,
     pos = torch.arange(S, device=gpu).expand(B, S)
     ref, size = ref64(x, None, cos, sin, pos, 0.0, inter, norm=False)
     check(out[..., :rot], ref[..., :rot], size[..., :rot], dt)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D,rot,S", [(64, 64, 1100), (64, 0, 1100), (96, 32, 550), (128, 128, 550), (256, 256, 300)])
+@pytest.mark.parametrize("H,Hkv", [(6, 1), (5, 3)])
+@pytest.mark.parametrize("inter", [False, True])
+def test_four_heads_a_thread(be, gpu, dt, D, rot, S, H, Hkv, inter):
+    """Sizes at which a thread takes four heads (1536 threads an SM with one head each),
+    with head counts that leave its last group part empty."""
+    B, lanes = 4, 8 if D <= 64 else 16 if D <= 128 else 32
+    assert B * S * (H + Hkv) * lanes >= torch.cuda.get_device_properties(gpu).multi_processor_count * 1536
+    run(be, gpu, B, S, H, Hkv, D, rot, dt, inter, seed=S + H)
+    run(be, gpu, B, S, H, Hkv, D, rot, dt, inter, layout="bhsd", norm=False, weights=False, inplace=True, seed=S + H + 1)

@@ -167,3 +167,23 @@ def test_more_row_tiles_than_65535(be, gpu):
     y = x.double() @ w.t() + r.double()
     tol = (1.2 * 2.0 ** -17 + 2.0 ** -24) * (x.double().abs() @ w.abs().t()) + (2.0 ** -20 + 2.0 ** -24) * y.abs()
     assert ((out.double() - y).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("G,K", [(32, 288), (64, 320), (128, 384)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [1, 8, 13, 16])
+def test_few_rows_of_a_wide_layer(be, gpu, G, K, dt, M):
+    """Up to 16 rows with 32 channels a CTA: taken from two such CTAs an SM."""
+    N = 2 * torch.cuda.get_device_properties(gpu).multi_processor_count * 32 + 5
+    check(be, gpu, M, N, K, G, dt, act="silu", res=True, seed=M)
+    check(be, gpu, M, N, K, G, dt, ydt=torch.float32, sdt=torch.bfloat16, seed=M + 1)
+
+
+@pytest.mark.parametrize("G,K", [(32, 608), (64, 1088), (128, 640)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [17, 32, 67, 72, 150])
+def test_more_rows_of_a_wide_layer(be, gpu, G, K, dt, M):
+    """More rows with 64 channels a CTA: taken once those fill half the SMs."""
+    N = torch.cuda.get_device_properties(gpu).multi_processor_count * 32 + 7
+    check(be, gpu, M, N, K, G, dt, act="gelu", res=True, seed=M)
+    check(be, gpu, M, N, K, G, dt, ydt=torch.float32, sdt=torch.float32, seed=M + 1)
