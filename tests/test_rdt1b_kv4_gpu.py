@@ -187,22 +187,23 @@ def test_a_change_and_back_without_an_encode_is_refused(setup):
 
 def test_a_change_that_finds_no_memory_keeps_none(gpu):
     """The 4-bit caches are allocated all or not at all, and the handle stays as it was."""
-    cfg = default_config(num_layers=2, max_lang_len=64, img_len=4374, max_sessions=4)
+    cfg = default_config(num_layers=2, max_lang_len=64, img_len=4374, max_sessions=8)
     model, ballast = RDT1B(cfg, seed=5), None
     try:
         torch.cuda.synchronize()
         torch.cuda.empty_cache()
-        # of 40 MB for the image block (18 + 18 for its codes) 24 MB are there
-        ballast = torch.empty(torch.cuda.mem_get_info()[0] - (24 << 20), dtype=torch.uint8, device=gpu)
+        # of 81 MB for the image block (36 + 36 for its codes) 48 MB are there
+        ballast = torch.empty(torch.cuda.mem_get_info()[0] - (48 << 20), dtype=torch.uint8, device=gpu)
         before = torch.cuda.mem_get_info()[0]
         for _ in range(3):
             with pytest.raises(_capi.SfbError):
                 model.set_cache(4)
-            assert torch.cuda.mem_get_info()[0] == before
+            # (more where the driver gives back a slab that was partly in use)
+            assert torch.cuda.mem_get_info()[0] >= before
         ballast = None
         torch.cuda.empty_cache()
         model.set_cache(4)
-        assert model.kv4_cache(1).shape == (4, 32, 4384, 64)
+        assert model.kv4_cache(1).shape == (8, 32, 4384, 64)
     finally:
         del ballast
         model.close()
