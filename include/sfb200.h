@@ -339,7 +339,11 @@ int sfb_kv4_read(const sfb_kv4_cache* cache, void* k, const int64_t* k_stride, v
  * - q, out: dtype SFB_BF16 or SFB_F16 by element strides (batch, head, seq),
  *   16-byte aligned, strides multiples of 16 bytes. Queries enter the products
  *   as fp16: bf16 queries beyond 65504 are not supported (the kernel then
- *   records SFB_ERR_RANGE in the device error word).
+ *   records SFB_ERR_RANGE in the device error word), and bf16 queries below
+ *   2^-17 are rounded to a multiple of 2^-24. An infinite query makes its row NaN.
+ *   Probabilities are rounded to fp16 before they meet V (2^-12 on average of a
+ *   result, beside the 2^-11 or 2^-8 of its type), with their bits kept down to
+ *   2^-21 of the row's largest.
  * - kv_len (optional, int32 [batch], device): slots j >= kv_len[b] are masked.
  * - key_mask (optional, uint8 [batch, seq_k], device): as in sfb_attn_args.
  * - is_causal: the queries are the last seq_q tokens of the session, query i
@@ -381,8 +385,9 @@ int sfb_kv4_attention(const sfb_kv4_cache* cache, const sfb_kv4_attn_args* args,
  * 128; K % group == 0. bias: x_dtype [N] or NULL; residual: [M, N] in y_dtype
  * with row stride ldr, or NULL (may alias y); y: y_dtype (x_dtype or SFB_F32)
  * [M, N], row stride ldy. act as sfb_w8a16_linear. Any M, N and K (N and K up
- * to 2^31 - 1024). Codes enter the products exactly; sums and scales are fp32. Meant for few rows (it is bound
- * by the weights up to about 64). */
+ * to 2^31 - 1024). Codes enter the products exactly; sums and scales are fp32.
+ * Meant for few rows: faster than sfb_w8a16_linear up to about 24, slower from
+ * 67 on. */
 int sfb_w4a16_linear(const void* x, int64_t ldx, int32_t x_dtype, const void* w, const void* w_scale,
                      int32_t scale_dtype, int32_t group, const void* bias, const void* residual, int64_t ldr,
                      void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t N, int32_t K, int32_t act,
@@ -480,7 +485,8 @@ int sfb_rdt1b_set_path(void* handle, int32_t path);
  * of 4 bits). The first change to 4 allocates the 4-bit caches (setup time); the
  * 16-bit ones stay, so that it can be changed back.
  * Drops the captured graphs and the tick's condition: encode again before the
- * next forward or sample, which otherwise return SFB_ERR_INVALID. With 4 bits
+ * next forward or sample, which otherwise return SFB_ERR_INVALID (as they do
+ * after an encode that failed midway). With 4 bits
  * every session count takes the per-projection kernels (path 1). No counterpart
  * in the reference. */
 int sfb_rdt1b_set_cache(void* handle, int32_t bits);

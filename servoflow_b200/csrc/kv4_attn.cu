@@ -18,15 +18,18 @@
 // key_of(m) of its tile, chosen so that either kind of load touches one
 // contiguous run of shared memory.
 // A tile is 16 keys; blocks of 128 give one to each of a CTA's eight warps. With
-// 64 channels a lane loads its codes of the next tile straight into registers
-// while it works on this one. With 128 those registers would cost the second CTA
+// 64 channels a lane loads its codes straight into registers, two tiles ahead of
+// the one it works on. With 128 those registers would cost the second CTA
 // per SM, so blocks go through a ring in shared memory, four untiled bulk copies
 // each (codes and scales of K and V), issued by a ninth warp. 32 sessions of 8 to
 // 16 k slots of 8 heads: 178 µs from registers, 153 through the ring (144 as it is
 // now: 3.2 TB/s of codes and scales); 32 sessions of 4374 slots of 32 64-channel
-// heads: 105 µs from registers (101 now, 3.2 TB/s), 111 through the ring. What
-// bounds both is the issue of instructions, about 210 a tile and warp of 64
-// channels and 440 of 128, most of them to make fragments of the codes.
+// heads: 105 µs from registers (101 now, 3.2 TB/s), 111 through the ring; one session
+// of those 7.9 µs, 1.5 of them the launch. (Device times, calls back to back from a
+// graph; an eager call costs the host 11 µs.) What bounds both is the issue of
+// instructions, most of them to make fragments of the codes, together with the
+// dependence of a tile's steps on one another: with 128 channels 400 instructions a
+// tile and warp are 56 % of the issue slots, at 24 % of an SM's warps.
 // A nibble becomes fp16 exactly with one bit operation and one add or fma
 // (0x6400 | n = 1024 + n), the scale is one exact fp16 product (kv4.cu).
 // Pᵀ moves from the accumulator's layout to the B operand's by two movmatrix.
@@ -40,8 +43,8 @@
 // probability had a V near 0 lost the result of the others.) Row sums are fp32 from the
 // unrounded probabilities.
 //
-// Work split: a CTA takes a range of 16-key tiles of one (session, K/V head,
-// row tile), its warps interleaved; partial (m, l, O) are joined in shared
+// Work split: a CTA takes a range of the 128-key blocks of one (session, K/V head),
+// a 16-key tile of each block to a warp; partial (m, l, O) are joined in shared
 // memory, and across a cluster of up to 16 CTAs through distributed shared
 // memory: no workspace, no atomics, an order that does not change.
 #include "common.cuh"
@@ -54,7 +57,7 @@ struct Kv4AttnParams {
     const void* q;
     void* out;
     int64_t q_st[3], o_st[3];
-    int32_t H, g, Sq, Sk, R;          // g = H / Hkv query heads per K/V head, R = Sq · g rows
+    int32_t g, Sq, Sk, R;             // g query heads per K/V head, R = Sq · g rows
     int32_t rtiles, splits, causal;
     int32_t rt0, ytiles;              // of a launch: first row tile, row tiles
     float sl2;                        // scale · log2(e)
@@ -174,7 +177,7 @@ __global__ void __launch_bounds__(attn_threads(D), 2) kv4_attn_kernel(const Kv4A
         const int r = i / (D / 8), d = (i % (D / 8)) * 8;
         uint4 u = make_uint4(0, 0, 0, 0);
         if (r < rows) {
-            const int rr = r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
+            const int qi = r / p.g, h = hk * p.g + (r - qi * p.g);
             const T* src = static_cast<const T*>(p.q) + b * p.q_st[0] + h * p.q_st[1] + qi * p.q_st[2] + d;
             u = *reinterpret_cast<const uint4*>(src);
             uint32_t* w = reinterpret_cast<uint32_t*>(&u);
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(attn_threads(D), 2) kv4_attn_kernel(const Kv4A
     __syncthreads();
     T* out = static_cast<T*>(p.out);
     auto store = [&](int r, int d, float4 a, float inv) {
-        const int rr = r, qi = rr / p.g, h = hk * p.g + (rr - qi * p.g);
+        const int qi = r / p.g, h = hk * p.g + (r - qi * p.g);
         T* dst = out + b * p.o_st[0] + h * p.o_st[1] + qi * p.o_st[2] + d;
         uint2 u;
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
@@ -622,7 +625,7 @@ int kv4_attention_launch(const sfb_kv4_cache* cache, const sfb_kv4_attn_args& a,
     if (!is_sm100(device_info())) return SFB_ERR_UNSUPPORTED;
     p.q = a.q; p.out = a.out;
     for (int i = 0; i < 3; ++i) { p.q_st[i] = a.q_stride[i]; p.o_st[i] = a.out_stride[i]; }
-    p.H = a.heads; p.g = a.heads / p.c.Hkv; p.Sq = a.seq_q; p.Sk = a.seq_k; p.R = static_cast<int32_t>(R);
+    p.g = a.heads / p.c.Hkv; p.Sq = a.seq_q; p.Sk = a.seq_k; p.R = static_cast<int32_t>(R);
     p.causal = a.is_causal ? 1 : 0;
     p.sl2 = (a.scale == 0.f ? 1.f / sqrtf(static_cast<float>(p.c.D)) : a.scale) * 1.4426950408889634f;
     p.kv_len = a.kv_len; p.key_mask = a.key_mask; p.mask_sb = a.key_mask_stride_b;

@@ -29,10 +29,19 @@
 // rows by 4374 slots of 32 heads took 324 and 365 µs.)
 //
 // Measured: 32 sessions of 67 rows by 4374 slots, 32 heads of 64, 244 to 272 µs
-// from one GPU to another (315 to 281 TFLOP/s); one session 15.4 µs; 8 sessions of 16 heads of 128, 48 µs (399). The
-// bound is a tile's chain of waits (S, softmax, P, P·V), about 1900 clocks where
-// the exponents alone are 640: the warps of an SM run it nearly in step, one CTA
-// per SM being all that TMEM, shared memory and registers allow.
+// from one GPU to another (315 to 281 TFLOP/s); one session 15.4 µs; 8 sessions of 16
+// heads of 128, 48 µs (399). A tile of 80 columns takes about 1900 clocks where the
+// exponents alone are 640, one of 16 about 1450. What bounds it, by leaving parts out (64
+// channels; µs, whole | without the softmax | without the loads of codes | without the
+// softmax and all of the dequantisation but its barriers):
+//   16 rows, 64 heads, 8192 slots       28.5 |  28.4 |  21.0 |  18.4
+//   40 rows, 512 heads, 4374 slots     123   | 120   | 102   |  84
+//   67 rows, 1024 heads, 4374 slots    266   | 244   | 237   | 164
+//   96 rows, 128 heads, 4374 slots      40.3 |  34.9 |  38.1 |  24.7
+// Few columns wait for the codes: the dequantising warps have one tile of them in
+// flight. More columns wait for the softmax as well, neither chain hiding the other;
+// the last column is the hand-overs between the warps, the MMAs, launch and join. One
+// CTA per SM is all that TMEM, shared memory and registers allow.
 //
 // With M = 64 the accumulator's row d is in lane 32·(d / 16) + d % 16, with 128 in
 // lane d.
@@ -220,7 +229,7 @@ __global__ void __launch_bounds__(threads(D, NQ), 1) kv4_attn_tc_kernel(const Kv
         if (mbar_try_wait(smem_u32(&bars[bar]), parity)) return;
         if (!ok || !mbar_wait(&bars[bar], parity, kWaitNs)) ok = false;
     };
-    float* pO = reinterpret_cast<float*>(smem + kOffP);            // [NQ][64]
+    float* pO = reinterpret_cast<float*>(smem + kOffP);            // [NQ][D]
     float* pM = pO + kMaxQ * D;
     float* pL = pM + kMaxQ;
 

@@ -17,7 +17,8 @@
 // they share its position's cos / sin values (8 + 8 fp32 loads beside 8 16-bit
 // ones) and the index arithmetic. Blocks of q come before blocks of k, so that
 // which of the two a thread works on costs nothing per head.
-// Measured: 32 × 67 tokens of 32 + 32 heads of 64, 7.9 µs; 2 × 4374 tokens of 32 +
+// Measured (device times, calls back to back from a graph; an eager call costs the host
+// 18 µs): 32 × 67 tokens of 32 + 32 heads of 64, 7.9 µs; 2 × 4374 tokens of 32 +
 // 8 heads of 128, 35.1 µs (5.2 TB/s, 79 % of a copy's rate); one token 1.5 µs.
 #include "common.cuh"
 

@@ -22,9 +22,13 @@
 // 8·NT rows, X goes through a ring of shared memory that the warps of the channel
 // tiles share, and the warps left over split the inputs.
 //
-// Measured: one row of 16384 × 8192, groups of 128, 26.6 µs (2.6 TB/s of codes and
-// scales); one of 2048² 3.0 µs; 8 of 8192² 19.2 µs; 67 of 6144 × 2048 20.1 µs. What
-// bounds few rows is the loads' latency and the issue of instructions together, 165
+// Measured (device times, calls back to back from a graph; an eager call costs the host
+// 12 µs): one row of 16384 × 8192, groups of 128, 26.6 µs (2.6 TB/s of codes and
+// scales); one of 2048² 3.0 µs; 8 of 8192² 19.2 µs (21.7 with other buffers); 67 of 6144 × 2048 20.1 µs; 2144
+// of 2048² 120 µs. The int8 layer takes 8.6, 32 (8 of 8192²), 12.7 and 22 µs: it is the
+// faster one from about 32 rows on. More rows are bound by X from L2, the conversion of
+// the codes by every warp for each 72 rows and mma.sync's rate, 67 of 6144 × 2048 also by
+// 96 CTAs for 148 SMs. What bounds few rows is the loads' latency and the issue of instructions together, 165
 // a KB of codes in 43 % of the slots: more bytes in flight (warp-private rings of
 // asynchronous copies, 4 stages deep, 204 a KB) gave 24.3, 3.8 and 20.8 µs for the
 // first three.
@@ -123,14 +127,9 @@ constexpr int kThreads = kWarps * 32;
 // block, word w of the four belongs to block w / kQ. Groups are whole blocks.
 __host__ __device__ constexpr int block_of(int G) { return G < 64 ? 32 : 64; }
 
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, int bytes_in, int size_) {
-    // size_ bytes, of which bytes_in are read and the rest zeros
-    if (size_ == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes_in) : "memory");
-    else if (size_ == 8)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes_in) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes_in) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes_in) {
+    // 16 bytes, of which bytes_in are read and the rest zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes_in) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -365,7 +364,7 @@ __global__ void __launch_bounds__(many_threads(WM)) w4a16_many_kernel(const W4Pa
             const int r = e / (kSpan / 8), c = e % (kSpan / 8), k = i * kSpan + c * 8;
             const bool in = m0 + r < p.M && k < p.K;
             const T* src = static_cast<const T*>(p.x) + (in ? static_cast<int64_t>(m0 + r) * p.ldx + k : 0);
-            cp_async(sbase + (stage * kRows + r) * kPitch + c * 16, src, in ? 16 : 0, 16);
+            cp_async16(sbase + (stage * kRows + r) * kPitch + c * 16, src, in ? 16 : 0);
         }
     };
     struct Set { uint32_t a[4], b[4]; float sa[kU], sb[kU]; };
