@@ -74,7 +74,8 @@ constexpr int kNumBars = 2 * kMaxStages + 2 + 2 + 1 + 1 + 1;
 __host__ __device__ constexpr int off_tmem(int d) { return off_bar(d) + 8 * kNumBars; }
 __host__ __device__ constexpr int smem_bytes(int d) { return off_tmem(d) + 16 + 1024; }        // + alignment slack
 __host__ __device__ constexpr bool layout_ok(int d) {
-    return smem_bytes(d) <= 227 * 1024 && kTmemO + max_q(d) <= tmem_k(d) && max_q(d) <= 128 && off_v(d) % 1024 == 0 &&
+    // (more than half of an SM's: two kernels that take tensor memory never share one)
+    return smem_bytes(d) <= 227 * 1024 && smem_bytes(d) > 114 * 1024 && kTmemO + max_q(d) <= tmem_k(d) && max_q(d) <= 128 && off_v(d) % 1024 == 0 &&
            off_p(d) % 1024 == 0 && off_col(d) % 16 == 0 && off_bar(d) % 8 == 0 &&
            // the partial result of a CTA, over P once every MMA is done: [NQ][D] O, [NQ] m, l
            max_q(d) * d * 4 + 2 * max_q(d) * 4 <= 4 * kBlock64;
