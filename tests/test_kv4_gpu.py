@@ -560,3 +560,33 @@ def test_every_row_form_with_masks(be, gpu, D, dt, H, Hkv, Sq):
     run_attn(be, gpu, 4, H, Hkv, Sq, 261, D, dt, causal=True, lens=[261, 100, Sq + 3, 7], seed=Sq)
     run_attn(be, gpu, 4, H, Hkv, Sq, 261, D, dt, mask_p=0.4, lens=[261, 0, 128, 129], layout="bshd", seed=Sq + 1)
     run_attn(be, gpu, 4, H, Hkv, Sq, 530, D, dt, scale=-0.2, splits=3, seed=Sq + 2)
+
+
+def test_scales_and_codes_at_ties(be, gpu):
+    """Exact ties of fp32 input go to even, and their neighbours of one unit in the last
+    place to the right side: of the scale (max|x| = 7 · t with t halfway between two
+    bf16 values) and of the codes (x / s as fp32 division gives it, next to k + 1/2)."""
+    n = 4096
+    g = torch.Generator().manual_seed(71)
+    x = torch.zeros(n, 32)
+    t = (torch.randint(128, 256, (n,), generator=g) * 2 + 1).float()            # 9 bits, the last one set
+    e = 2.0 ** torch.randint(-20, 3, (n,), generator=g).float()
+    top = 7 * t * e
+    step = torch.randint(-1, 2, (n,), generator=g)
+    top = torch.where(step < 0, torch.nextafter(top, torch.zeros_like(top)),
+                      torch.where(step > 0, torch.nextafter(top, torch.full_like(top, 1e30)), top))
+    x[: n // 2, 0] = top[: n // 2]
+    # the other half: scales of 8 bits, values next to every half step
+    s = torch.randint(128, 256, (n,), generator=g).float() * 2.0 ** torch.randint(-30, 5, (n,), generator=g).float()
+    x[n // 2:, 0] = 7 * s[n // 2:]
+    half = torch.arange(-6.5, 7, 1.0)                                           # 14 halves, exact times s
+    v = half[None] * s[n // 2:, None]
+    x[n // 2:, 1:15] = v
+    x[n // 2:, 15:29] = torch.nextafter(v, torch.full_like(v, 1e30))
+    x[n // 2:, 29:32] = torch.nextafter(v[:, 5:8], torch.full_like(v[:, 5:8], -1e30))
+    x = x.view(1, 1, n // 2, 64)
+    cache = KV4Cache.allocate(1, 1, n // 2, 64)
+    be.kv4_append(cache, x.to(gpu), (-x).to(gpu))
+    for val, codes, scale in ((x, cache.k_codes, cache.k_scale), (-x, cache.v_codes, cache.v_scale)):
+        c, sc = quantize64(val)
+        assert torch.equal(scale.cpu(), sc) and torch.equal(unpack_codes(codes).cpu(), c)
