@@ -251,7 +251,7 @@ int sfb_w8a16_mlp_noalloc(const void* x, int64_t ldx, const int8_t* w1, const fl
  * - dtype of q, k, the outputs and the weights: SFB_BF16, SFB_F16 or SFB_F32.
  *   head_dim: a multiple of 8, at most 256, contiguous; the other dimensions
  *   by element strides (batch, head, seq). Pointers 16-byte aligned, strides
- *   multiples of 16 bytes. */
+ *   multiples of 16 bytes; batch · seq · heads below 2^31 - 256. */
 typedef struct sfb_norm_rope_args {
     const void* q;
     const void* k;
@@ -386,8 +386,8 @@ int sfb_kv4_attention(const sfb_kv4_cache* cache, const sfb_kv4_attn_args* args,
  * with row stride ldr, or NULL (may alias y); y: y_dtype (x_dtype or SFB_F32)
  * [M, N], row stride ldy. act as sfb_w8a16_linear. Any M, N and K (N and K up
  * to 2^31 - 1024). Codes enter the products exactly; sums and scales are fp32.
- * Meant for few rows: faster than sfb_w8a16_linear up to about 24, slower from
- * 67 on. */
+ * Meant for few rows: faster than sfb_w8a16_linear up to 16, level with it or
+ * slower beyond. */
 int sfb_w4a16_linear(const void* x, int64_t ldx, int32_t x_dtype, const void* w, const void* w_scale,
                      int32_t scale_dtype, int32_t group, const void* bias, const void* residual, int64_t ldr,
                      void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t N, int32_t K, int32_t act,

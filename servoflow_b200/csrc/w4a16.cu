@@ -24,14 +24,15 @@
 //
 // Measured (device times, calls back to back from a graph; an eager call costs the host
 // 12 µs): one row of 16384 × 8192, groups of 128, 26.6 µs (2.6 TB/s of codes and
-// scales); one of 2048² 3.0 µs; 8 of 8192² 19.2 µs (21.7 with other buffers); 67 of 6144 × 2048 20.1 µs; 2144
-// of 2048² 120 µs. The int8 layer takes 8.6, 32 (8 of 8192²), 12.7 and 22 µs: it is the
-// faster one from about 32 rows on. More rows are bound by X from L2, the conversion of
-// the codes by every warp for each 72 rows and mma.sync's rate, 67 of 6144 × 2048 also by
-// 96 CTAs for 148 SMs. What bounds few rows is the loads' latency and the issue of instructions together, 165
-// a KB of codes in 43 % of the slots: more bytes in flight (warp-private rings of
-// asynchronous copies, 4 stages deep, 204 a KB) gave 24.3, 3.8 and 20.8 µs for the
-// first three.
+// scales); one of 2048² 3.0; 8 of 8192² 19.2 (21.7 with other buffers); 67 of 6144 × 2048
+// 20.1; 2144 of 2048² 120. The int8 layer takes 57.8, 8.6, 32.3, 12.7 and 22.2 µs: this
+// one is faster up to 16 rows; 24 take 11.6 and 11.6 µs (6144 × 2048), 44.5 and 32.3
+// (8192²). What bounds few rows is the loads' latency and the issue of instructions
+// together, 165 a KB of codes in 43 % of the slots: more bytes in flight (warp-private
+// rings of asynchronous copies, 4 stages deep, 204 a KB) gave 24.3, 3.8 and 20.8 µs for
+// the first three. More rows are bound by X from L2, the conversion of the codes by
+// every warp for each 72 rows and mma.sync's rate, 67 of 6144 × 2048 also by 96 CTAs for
+// 148 SMs.
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 
