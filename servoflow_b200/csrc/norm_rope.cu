@@ -127,8 +127,8 @@ norm_rope_kernel(const NormRopeParams p) {
     // the token's angles: 8 (half-split) or 4 (interleaved) pairs for this lane. Lanes
     // past the rotated channels take no part: a product with a sine of 0 would make
     // NaN of an infinity there, and of its neighbour. (Left out by selecting the result
-    // where pairs are interleaved, by a branch where halves are paired: the other way
-    // round 2 × 4374 tokens of 40 heads took 35.9 µs for 35.1, 32 × 67 tokens 8.5 for 7.8.)
+    // where pairs are interleaved, by a branch where halves are paired. Exchanged,
+    // 2 × 4374 tokens of 40 heads took 35.9 µs for 35.1, 32 × 67 tokens 8.5 for 7.8.)
     float c[8], sn[8];
     bool bad = false;
     const bool first = d0 < p.rot / 2, turns = d0 < p.rot;

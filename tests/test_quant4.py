@@ -244,11 +244,11 @@ def test_copies_of_a_models_cache_are_on_its_device(monkeypatch):
     """With another device current: the model's is waited for, and holds the copy (fakes
     of the library and of torch's device calls)."""
     from servoflow_b200 import rdt1b
-    shape, seen = (2, 3, 32, 64), []
+    shape, seen = (2, 2, 32, 64), []
 
     class Lib:
         def sfb_rdt1b_kv4_cache(self, h, layer, buf):
-            buf.raw = _capi.KV4_CACHE.pack(0x1000, 0x2000, 0x3000, 0x4000, 3072, 1024, 192, 64, *shape)
+            buf.raw = _capi.KV4_CACHE.pack(0x1000, 0x2000, 0x3000, 0x4000, 2048, 1024, 128, 64, *shape)
             return 0
 
     model = rdt1b.RDT1B.__new__(rdt1b.RDT1B)
